@@ -41,7 +41,7 @@ macro_rules! opaque {
     ($($name:ident),*) => { $( #[repr(C)] pub struct $name { _private: [u8; 0] } )* };
 }
 opaque!(pg_ctx, pg_qtensor, pg_gguf_tensor, pg_mxfp4_expert, pg_gguf_file, pg_huffman_tensor, pg_huffman_kv_chunk,
-        pg_huffman_kv_cache, pg_rope, pg_kv_cache, pg_llama_block);
+        pg_huffman_kv_cache, pg_paged_kv4, pg_rope, pg_kv_cache, pg_llama_block);
 
 // ---- generated from include/peregrine_hip.h: begin ----
 extern "C" {
@@ -143,6 +143,28 @@ extern "C" {
     pub fn pg_huffman_kv_cache_chunk(c: *const pg_huffman_kv_cache, value_side: c_int, index: usize, out: *mut *const pg_huffman_kv_chunk) -> pg_status;
     pub fn pg_huffman_kv_cache_get_kv(ctx: *mut pg_ctx, c: *const pg_huffman_kv_cache, k: *mut f32, v: *mut f32) -> pg_status;
     pub fn pg_huffman_kv_cache_get_kv_dev(ctx: *mut pg_ctx, c: *const pg_huffman_kv_cache, k_dev: *mut f32, v_dev: *mut f32) -> pg_status;
+    pub fn pg_block_tables_extend(ctx: *mut pg_ctx, seq_lens: *const i32, new_lens: *const i32, batch: usize, block_size: usize, free_list: *const i32, free_count: *const i32, num_blocks: usize, block_table: *mut i32, max_blocks: usize, seq_lens_out: *mut i32, free_count_out: *mut i32, query_start: *mut i32, granted: *mut i32, slots: *mut i32, max_tokens: usize) -> pg_status;
+    pub fn pg_block_tables_extend_dev(ctx: *mut pg_ctx, seq_lens_dev: *const i32, new_lens_dev: *const i32, batch: usize, block_size: usize, free_list_dev: *const i32, free_count_dev: *const i32, num_blocks: usize, block_table_dev: *mut i32, max_blocks: usize, seq_lens_out_dev: *mut i32, free_count_out_dev: *mut i32, query_start_dev: *mut i32, granted_dev: *mut i32, slots_dev: *mut i32, max_tokens: usize) -> pg_status;
+    pub fn pg_block_tables_release(ctx: *mut pg_ctx, release: *const i32, seq_lens: *mut i32, batch: usize, block_size: usize, block_table: *mut i32, max_blocks: usize, free_list: *mut i32, free_count: *mut i32, num_blocks: usize) -> pg_status;
+    pub fn pg_block_tables_release_dev(ctx: *mut pg_ctx, release_dev: *const i32, seq_lens_dev: *mut i32, batch: usize, block_size: usize, block_table_dev: *mut i32, max_blocks: usize, free_list_dev: *mut i32, free_count_dev: *mut i32, num_blocks: usize) -> pg_status;
+    pub fn pg_paged_kv4_create(ctx: *mut pg_ctx, num_blocks: usize, block_size: usize, num_kv_heads: usize, head_dim: usize, out: *mut *mut pg_paged_kv4) -> pg_status;
+    pub fn pg_paged_kv4_free(ctx: *mut pg_ctx, cache: *mut pg_paged_kv4);
+    pub fn pg_paged_kv4_info(cache: *const pg_paged_kv4, num_blocks: *mut usize, block_size: *mut usize, num_kv_heads: *mut usize, head_dim: *mut usize, bytes: *mut usize) -> pg_status;
+    pub fn pg_paged_kv4_append(ctx: *mut pg_ctx, cache: *mut pg_paged_kv4, k: *const f32, v: *const f32, tokens: usize, slots: *const i32) -> pg_status;
+    pub fn pg_paged_kv4_append_dev(ctx: *mut pg_ctx, cache: *mut pg_paged_kv4, k_dev: *const f32, v_dev: *const f32, token_stride: usize, head_stride: usize, tokens: usize, slots_dev: *const i32) -> pg_status;
+    pub fn pg_paged_kv4_read(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, slots: *const i32, n: usize, k: *mut f32, v: *mut f32) -> pg_status;
+    pub fn pg_paged_kv4_read_dev(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, slots_dev: *const i32, n: usize, k_dev: *mut f32, v_dev: *mut f32) -> pg_status;
+    pub fn pg_paged_kv4_attention_scratch(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, num_q_heads: usize, batch: usize, max_query: usize, max_blocks: usize, bytes: *mut usize) -> pg_status;
+    pub fn pg_paged_kv4_attention(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, q: *const f32, num_q_heads: usize, query_start: *const i32, seq_lens: *const i32, batch: usize, tokens: usize, block_table: *const i32, max_blocks: usize, scale: f32, mask_kind: c_int, window: usize, sink_tokens: usize, logit_cap: f32, out: *mut f32) -> pg_status;
+    pub fn pg_paged_kv4_attention_dev(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, q_dev: *const f32, q_token_stride: usize, q_head_stride: usize, num_q_heads: usize, query_start_dev: *const i32, seq_lens_dev: *const i32, batch: usize, tokens: usize, max_query: usize, block_table_dev: *const i32, max_blocks: usize, scale: f32, mask_kind: c_int, window: usize, sink_tokens: usize, logit_cap: f32, scratch_dev: *mut c_void, scratch_bytes: usize, out_dev: *mut f32) -> pg_status;
+    pub fn pg_paged_kv4_summarise(ctx: *mut pg_ctx, cache: *mut pg_paged_kv4, query_start: *const i32, seq_lens: *const i32, batch: usize, block_table: *const i32, max_blocks: usize) -> pg_status;
+    pub fn pg_paged_kv4_summarise_dev(ctx: *mut pg_ctx, cache: *mut pg_paged_kv4, query_start_dev: *const i32, seq_lens_dev: *const i32, batch: usize, tokens: usize, block_table_dev: *const i32, max_blocks: usize) -> pg_status;
+    pub fn pg_paged_kv4_read_summaries_dev(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, blocks_dev: *const i32, n: usize, lo_dev: *mut f32, hi_dev: *mut f32) -> pg_status;
+    pub fn pg_paged_kv4_select(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, q: *const f32, num_q_heads: usize, query_start: *const i32, seq_lens: *const i32, batch: usize, tokens: usize, block_table: *const i32, max_blocks: usize, top_k: usize, first_blocks: usize, recent_blocks: usize, selected: *mut i32) -> pg_status;
+    pub fn pg_paged_kv4_select_dev(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, q_dev: *const f32, q_token_stride: usize, q_head_stride: usize, num_q_heads: usize, query_start_dev: *const i32, seq_lens_dev: *const i32, batch: usize, tokens: usize, block_table_dev: *const i32, max_blocks: usize, top_k: usize, first_blocks: usize, recent_blocks: usize, selected_dev: *mut i32) -> pg_status;
+    pub fn pg_paged_kv4_selected_scratch(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, num_q_heads: usize, tokens: usize, top_k: usize, bytes: *mut usize) -> pg_status;
+    pub fn pg_paged_kv4_attention_selected(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, q: *const f32, num_q_heads: usize, query_start: *const i32, seq_lens: *const i32, batch: usize, tokens: usize, block_table: *const i32, max_blocks: usize, selected: *const i32, top_k: usize, scale: f32, logit_cap: f32, out: *mut f32) -> pg_status;
+    pub fn pg_paged_kv4_attention_selected_dev(ctx: *mut pg_ctx, cache: *const pg_paged_kv4, q_dev: *const f32, q_token_stride: usize, q_head_stride: usize, num_q_heads: usize, query_start_dev: *const i32, seq_lens_dev: *const i32, batch: usize, tokens: usize, block_table_dev: *const i32, max_blocks: usize, selected_dev: *const i32, top_k: usize, scale: f32, logit_cap: f32, scratch_dev: *mut c_void, scratch_bytes: usize, out_dev: *mut f32) -> pg_status;
     pub fn pg_moe_ffn(ctx: *mut pg_ctx, x: *const f32, T: usize, router_logits: *const f32, E: usize, top_k: usize, gate: *const *const pg_gguf_tensor, up: *const *const pg_gguf_tensor, down: *const *const pg_gguf_tensor, act: c_int, out: *mut f32) -> pg_status;
     pub fn pg_moe_ffn_dev(ctx: *mut pg_ctx, x_dev: *const f32, T: usize, router_logits_dev: *const f32, E: usize, top_k: usize, gate: *const *const pg_gguf_tensor, up: *const *const pg_gguf_tensor, down: *const *const pg_gguf_tensor, act: c_int, out_dev: *mut f32) -> pg_status;
     pub fn pg_moe_ffn_routed(ctx: *mut pg_ctx, x: *const f32, T: usize, expert_idx: *const i32, weight: *const f32, E: usize, top_k: usize, gate: *const *const pg_gguf_tensor, up: *const *const pg_gguf_tensor, down: *const *const pg_gguf_tensor, act: c_int, shared: *const f32, out: *mut f32) -> pg_status;

@@ -417,6 +417,128 @@ pg_status pg_huffman_kv_cache_chunk(const pg_huffman_kv_cache *c, int value_side
 pg_status pg_huffman_kv_cache_get_kv(pg_ctx *ctx, const pg_huffman_kv_cache *c, float *k, float *v);
 pg_status pg_huffman_kv_cache_get_kv_dev(pg_ctx *ctx, const pg_huffman_kv_cache *c, float *k_dev, float *v_dev);
 
+/* ---- block tables, and a key/value cache in 4 bits that many requests share ----------------------
+ * No counterpart in the reference, whose caches (StandardKVCache, HuffmanKVCache) belong to one
+ * sequence each.  A cache holds `num_blocks` blocks of `block_size` tokens (16, 32, 64, 128 or 256);
+ * a request's block table [max_blocks] names its blocks in the order of its tokens, and a slot is
+ * block * block_size + place in the block.  A step packs its requests' new rows one behind the
+ * other: request b's are query_start[b] .. query_start[b + 1] - 1, the last tokens of the
+ * seq_lens[b] that it has with them.  The _dev forms read lengths, tables and slots on the device
+ * only, so that a captured step can be replayed with others in their place; what does not fit them
+ * (a table entry that is no block, a length behind the table) is left out and never faults, and
+ * the host forms refuse it. */
+
+/* Lengths and tables for a step that adds new_lens[b] tokens to request b.  A request whose new blocks
+ * the pool holds -- needs counted in the order of requests, those that get none included -- and whose
+ * table has room is granted: its next table entries are taken from the free list (the i-th block
+ * handed out is free_list[free_count - 1 - i]) and seq_lens_out[b] = seq_lens[b] + new_lens[b].
+ * One that needs no block is always granted; one that is not keeps its length and entries and its
+ * rows get slot -1.  slots [max_tokens]: a slot per packed row, -1 behind the last (query_start is
+ * cut at max_tokens, which the sum of new_lens is not to pass).  seq_lens_out may be seq_lens and
+ * free_count_out may be free_count; all else is distinct.  free_list [num_blocks] is only read. */
+pg_status pg_block_tables_extend(pg_ctx *ctx, const int32_t *seq_lens, const int32_t *new_lens, size_t batch, size_t block_size,
+                                 const int32_t *free_list, const int32_t *free_count, size_t num_blocks, int32_t *block_table,
+                                 size_t max_blocks, int32_t *seq_lens_out, int32_t *free_count_out, int32_t *query_start,
+                                 int32_t *granted, int32_t *slots, size_t max_tokens);
+pg_status pg_block_tables_extend_dev(pg_ctx *ctx, const int32_t *seq_lens_dev, const int32_t *new_lens_dev, size_t batch,
+                                     size_t block_size, const int32_t *free_list_dev, const int32_t *free_count_dev,
+                                     size_t num_blocks, int32_t *block_table_dev, size_t max_blocks, int32_t *seq_lens_out_dev,
+                                     int32_t *free_count_out_dev, int32_t *query_start_dev, int32_t *granted_dev,
+                                     int32_t *slots_dev, size_t max_tokens);
+/* The blocks of every request with release[b] != 0 back onto the free list, in order; its length becomes
+ * 0 and its entries -1.  A block that two tables share is the caller's to give back once. */
+pg_status pg_block_tables_release(pg_ctx *ctx, const int32_t *release, int32_t *seq_lens, size_t batch, size_t block_size,
+                                  int32_t *block_table, size_t max_blocks, int32_t *free_list, int32_t *free_count,
+                                  size_t num_blocks);
+pg_status pg_block_tables_release_dev(pg_ctx *ctx, const int32_t *release_dev, int32_t *seq_lens_dev, size_t batch,
+                                      size_t block_size, int32_t *block_table_dev, size_t max_blocks, int32_t *free_list_dev,
+                                      int32_t *free_count_dev, size_t num_blocks);
+
+/* The cache: a row -- one head of one token, keys and values alike -- is codes n of 0 .. 15 with a centre z and
+ * a step d in bfloat16, value = z + d (n - 7.5) (4.25 bits a value at head_dim 128):
+ *   z = bf16(lo / 2 + hi / 2), h = max(hi - z, z - lo) over the row's least and most, d = h * (1 / 7.5) rounded up
+ *   to bfloat16 (at least 2^-120, or 0 where h is 0), n = clamp(rint((x - z) * (1 / d) + 7.5), 0, 15), every
+ *   operation rounded to f32.
+ * A row with a value that is not finite is NaN as a whole.  head_dim <= 256; num_blocks * block_size < 2^31. */
+typedef struct pg_paged_kv4 pg_paged_kv4;
+pg_status pg_paged_kv4_create(pg_ctx *ctx, size_t num_blocks, size_t block_size, size_t num_kv_heads, size_t head_dim,
+                              pg_paged_kv4 **out);
+void pg_paged_kv4_free(pg_ctx *ctx, pg_paged_kv4 *cache);
+pg_status pg_paged_kv4_info(const pg_paged_kv4 *cache, size_t *num_blocks, size_t *block_size, size_t *num_kv_heads,
+                            size_t *head_dim, size_t *bytes);
+/* Rows into their slots: k, v [tokens, num_kv_heads, head_dim] (host), or with token t's head h at
+ * k_dev + t * token_stride + h * head_stride (floats; the same for v).  A row of slot -1 is left out.  No slot is
+ * named twice in one call: the host form refuses it, the _dev form leaves a mixture of the two rows. */
+pg_status pg_paged_kv4_append(pg_ctx *ctx, pg_paged_kv4 *cache, const float *k, const float *v, size_t tokens,
+                              const int32_t *slots);
+pg_status pg_paged_kv4_append_dev(pg_ctx *ctx, pg_paged_kv4 *cache, const float *k_dev, const float *v_dev, size_t token_stride,
+                                  size_t head_stride, size_t tokens, const int32_t *slots_dev);
+/* The values of n slots: k, v [n, num_kv_heads, head_dim]; _dev: rows of a slot that is none are 0. */
+pg_status pg_paged_kv4_read(pg_ctx *ctx, const pg_paged_kv4 *cache, const int32_t *slots, size_t n, float *k, float *v);
+pg_status pg_paged_kv4_read_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, const int32_t *slots_dev, size_t n, float *k_dev,
+                                float *v_dev);
+
+/* Attention of a step's rows over their requests: q [tokens, num_q_heads, head_dim] (host), or with row t's head h at
+ * q_dev + t * q_token_stride + h * q_head_stride; out [tokens, num_q_heads, head_dim] is written (not added to), rows behind
+ * query_start[batch] are left as they were.  Query head h reads key head h / (num_q_heads / num_kv_heads).  Masks as in
+ * pg_gqa_attention without LocalGlobal, a row's position being its token's; a row that sees no key is 0.  logit_cap as there.
+ * max_query: no request has more rows (those beyond are not computed).  scratch_dev: 16-byte aligned, at least what
+ * pg_paged_kv4_attention_scratch says for these sizes (it may be 0); calls that may run at once have one each. */
+pg_status pg_paged_kv4_attention_scratch(pg_ctx *ctx, const pg_paged_kv4 *cache, size_t num_q_heads, size_t batch,
+                                         size_t max_query, size_t max_blocks, size_t *bytes);
+pg_status pg_paged_kv4_attention(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q, size_t num_q_heads,
+                                 const int32_t *query_start, const int32_t *seq_lens, size_t batch, size_t tokens,
+                                 const int32_t *block_table, size_t max_blocks, float scale, int mask_kind, size_t window,
+                                 size_t sink_tokens, float logit_cap, float *out);
+pg_status pg_paged_kv4_attention_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q_dev, size_t q_token_stride,
+                                     size_t q_head_stride, size_t num_q_heads, const int32_t *query_start_dev,
+                                     const int32_t *seq_lens_dev, size_t batch, size_t tokens, size_t max_query,
+                                     const int32_t *block_table_dev, size_t max_blocks, float scale, int mask_kind, size_t window,
+                                     size_t sink_tokens, float logit_cap, void *scratch_dev, size_t scratch_bytes, float *out_dev);
+
+/* Attention over part of a long context.  A block's summary holds, for each key head and channel, the least and the most of
+ * its keys, as int8 with one scale m * (1 / 127) (m the largest of their magnitudes): lo = rint(least * ((1 / m) * 127)), hi likewise.
+ * pg_paged_kv4_summarise brings those of the blocks up to date that a step's rows fill or end in (after its append);
+ * pg_paged_kv4_read_summaries_dev gives lo and hi [n, num_kv_heads, head_dim] of n blocks as values (0 for none). */
+pg_status pg_paged_kv4_summarise(pg_ctx *ctx, pg_paged_kv4 *cache, const int32_t *query_start, const int32_t *seq_lens,
+                                 size_t batch, const int32_t *block_table, size_t max_blocks);
+pg_status pg_paged_kv4_summarise_dev(pg_ctx *ctx, pg_paged_kv4 *cache, const int32_t *query_start_dev,
+                                     const int32_t *seq_lens_dev, size_t batch, size_t tokens, const int32_t *block_table_dev,
+                                     size_t max_blocks);
+pg_status pg_paged_kv4_read_summaries_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, const int32_t *blocks_dev, size_t n,
+                                          float *lo_dev, float *hi_dev);
+/* For each row and key head the top_k blocks that score highest among those that begin at or before its token:
+ *   score = max over the key head's query rows q of (sum_i x_i (x_i >= 0 ? hi_i : lo_i)) * (a * (1 / 127)) * scale,
+ *   x = rint(q * ((1 / a) * 127)), a the row's largest magnitude
+ * (a whole number and two f32 products, in this order, so that the choice does not depend on how it is computed; a bound of the
+ * row's scores in the block but for the roundings).  The first `first_blocks` and the last `recent_blocks` (at least 1: the
+ * row's own) are always among them; of equal scores the earlier block.  selected [tokens, num_kv_heads, top_k]: block numbers
+ * within the request, ascending, -1 behind them.  A block that holds a key that is not finite scores infinity; a query row
+ * that is not finite scores 0.  max_blocks <= 36864 (PG_EUNSUPPORTED). */
+pg_status pg_paged_kv4_select(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q, size_t num_q_heads,
+                              const int32_t *query_start, const int32_t *seq_lens, size_t batch, size_t tokens,
+                              const int32_t *block_table, size_t max_blocks, size_t top_k, size_t first_blocks,
+                              size_t recent_blocks, int32_t *selected);
+pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q_dev, size_t q_token_stride,
+                                  size_t q_head_stride, size_t num_q_heads, const int32_t *query_start_dev,
+                                  const int32_t *seq_lens_dev, size_t batch, size_t tokens, const int32_t *block_table_dev,
+                                  size_t max_blocks, size_t top_k, size_t first_blocks, size_t recent_blocks,
+                                  int32_t *selected_dev);
+/* pg_paged_kv4_attention, causal, over the selected blocks alone.  An entry that is not above the one before it, or
+ * behind the row's own block, contributes nothing (the host form refuses it). */
+pg_status pg_paged_kv4_selected_scratch(pg_ctx *ctx, const pg_paged_kv4 *cache, size_t num_q_heads, size_t tokens, size_t top_k,
+                                        size_t *bytes);
+pg_status pg_paged_kv4_attention_selected(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q, size_t num_q_heads,
+                                          const int32_t *query_start, const int32_t *seq_lens, size_t batch, size_t tokens,
+                                          const int32_t *block_table, size_t max_blocks, const int32_t *selected, size_t top_k,
+                                          float scale, float logit_cap, float *out);
+pg_status pg_paged_kv4_attention_selected_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q_dev, size_t q_token_stride,
+                                              size_t q_head_stride, size_t num_q_heads, const int32_t *query_start_dev,
+                                              const int32_t *seq_lens_dev, size_t batch, size_t tokens,
+                                              const int32_t *block_table_dev, size_t max_blocks, const int32_t *selected_dev,
+                                              size_t top_k, float scale, float logit_cap, void *scratch_dev, size_t scratch_bytes,
+                                              float *out_dev);
+
 /* ---- grouped MoE expert FFN ------------------------------------------------- */
 
 /* MoELayer::forward after the router matmul  examples/grok1/moe.rs:70-109

@@ -78,6 +78,28 @@ SIGNATURES = {
     "pg_gemm_w8a8_force_tile": [_vp, _int],
     "pg_gemv_w8a8_force_shape": [_vp, _int, _int],
     "pg_gguf_hmm_force": [_vp, _int],
+    "pg_block_tables_extend": [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz],
+    "pg_block_tables_extend_dev": [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz],
+    "pg_block_tables_release": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz],
+    "pg_block_tables_release_dev": [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _vp, _sz],
+    "pg_paged_kv4_create": [_vp, _sz, _sz, _sz, _sz, _pp],
+    "pg_paged_kv4_free": [_vp, _vp],
+    "pg_paged_kv4_info": [_vp, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)],
+    "pg_paged_kv4_append": [_vp, _vp, _vp, _vp, _sz, _vp],
+    "pg_paged_kv4_append_dev": [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp],
+    "pg_paged_kv4_read": [_vp, _vp, _vp, _sz, _vp, _vp],
+    "pg_paged_kv4_read_dev": [_vp, _vp, _vp, _sz, _vp, _vp],
+    "pg_paged_kv4_attention_scratch": [_vp, _vp, _sz, _sz, _sz, _sz, C.POINTER(_sz)],
+    "pg_paged_kv4_attention": [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, C.c_float, _int, _sz, _sz, C.c_float, _vp],
+    "pg_paged_kv4_attention_dev": [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _sz, C.c_float, _int, _sz, _sz, C.c_float, _vp, _sz, _vp],
+    "pg_paged_kv4_summarise": [_vp, _vp, _vp, _vp, _sz, _vp, _sz],
+    "pg_paged_kv4_summarise_dev": [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz],
+    "pg_paged_kv4_read_summaries_dev": [_vp, _vp, _vp, _sz, _vp, _vp],
+    "pg_paged_kv4_select": [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _sz, _sz, _vp],
+    "pg_paged_kv4_select_dev": [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _sz, _sz, _vp],
+    "pg_paged_kv4_selected_scratch": [_vp, _vp, _sz, _sz, _sz, C.POINTER(_sz)],
+    "pg_paged_kv4_attention_selected": [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, C.c_float, C.c_float, _vp],
+    "pg_paged_kv4_attention_selected_dev": [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, C.c_float, C.c_float, _vp, _sz, _vp],
     "pg_matmul_dequant_i8": [_vp, _vp, _sz, _sz, _vp, _vp],
     "pg_matmul_dequant_i8_dev": [_vp, _vp, _sz, _sz, _vp, _vp],
     "pg_f16_to_f32": [_vp, _vp, _sz, _vp],
@@ -195,6 +217,7 @@ _OTHER_RESTYPE = {
     "pg_huffman_kv_cache_num_chunks": _sz,
     "pg_mxfp4_expert_free": None,
     "pg_kv_cache_free": None,
+    "pg_paged_kv4_free": None,
     "pg_llama_block_free": None,
     "pg_kv_cache_len": _sz,
     "pg_fixed_scratch_bytes": _sz,

@@ -1,0 +1,972 @@
+// Attention over the paged cache in 4 bits, and over the blocks of it that a score selects for each query.
+//
+// With a key row's values z + d (n - 7.5) a score is  d (q . (n - 8)) + (z + d / 2) sum(q):  a product of small whole
+// numbers, which the int8 matrix cores do exactly once q is in fixed point (23 bits under its row's largest, as three digits of
+// 8), and two FMAs.  With a value row's the output is  sum_t (p_t d_t) (n_t - 7.5) + sum_t p_t z_t:  the f16 matrix cores
+// take n - 7.5 as it is and p_t d_t as two f16 (22 bits).  No key or value is dequantised; one pass over the rows keeps
+// the running maximum and sum of the softmax.
+//
+// The lanes' operands come straight from the rows as they lie in memory.  S^T = K Q^T: a lane holds 16 bytes of one of 16
+// tokens' keys, (x & 0x0f0f0f0f) and (x >> 4 & 0x0f0f0f0f) are 8 int8 channels in an order that the digits of q share.
+// The scores come out with a query row a lane and 4 tokens in it, which is how O^T = V^T P^T takes its probabilities, so
+// none crosses a lane.  For V a lane loads 8 tokens' word of 8 channels; the pair of one channel of two tokens is a byte
+// permute, a mask and an FMA away.
+#include <math.h>
+#include <new>
+#include "pg_kv4.h"
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float Q_UNITS = 8323072.f;     // 127 * 2^16: the largest of a query row in fixed point
+constexpr float P_TOP = 1024.f;          // what p d is scaled to where p = 1 and d is the largest step seen
+constexpr float P_MOST = 32768.f;        // ... and may grow to before the running maximum follows
+constexpr float CODE = 1.f / 512.f;      // the value operand is (n - 7.5) / 512: its low codes are f16 subnormals on their way
+
+struct kv4_attn {
+    const float *q;
+    size_t q_token, q_head;
+    kv4_view c;
+    kv4_batch ba;
+    const int *selected;  // [tokens][heads][top], or null
+    int top;
+    float scale, cap;
+    int mask, window, sinks, group, q_heads, max_query, splits, row_tiles;
+    float *part, *out;
+};
+
+// A wavefront's 16 query rows (row = lane & 15) as the B operands of the score products.
+template <int D>
+struct q_rows {
+    static constexpr int NJ = D / 64;
+    i32x4 digit[3][NJ];
+    int sum_hi2, sum_hi1, sum_lo;  // -8 times the sums of each digit over the row: (n - 8) for n
+    float unit, sum;               // value of a unit, sum of the row in units
+};
+
+__device__ __forceinline__ float over_groups(float v) {  // sum over the four lanes of a row
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ int over_groups(int v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float max_groups(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+
+// First channel of the 16 that lane group g holds for the j-th product.
+template <int D>
+__device__ __forceinline__ constexpr int q_base(int j, int g) {
+    return D == 64 ? 16 * g : 128 * (j >> 1) + 32 * g + 16 * (j & 1);
+}
+
+// x: the row (or null: zeros).  A row with a value that is not finite gets a NaN unit.
+template <int D>
+__device__ __forceinline__ void load_q(const float *x, int head_dim, int g, q_rows<D> &r) {
+    constexpr int NJ = D / 64;
+    float a[NJ][16];
+    float most = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int d = q_base<D>(j, g) + e;
+            a[j][e] = x && d < head_dim ? x[d] : 0.f;
+            most = fmaxf(most, fabsf(a[j][e]));
+            bad |= !(fabsf(a[j][e]) <= 3.402823466e38f);
+        }
+    most = max_groups(most);
+    bad = max_groups(bad ? 1.f : 0.f) != 0.f;
+    const bool none = bad || most < 7.88860905e-31f;  // 2^-100: scores of 0
+    const float inv = none ? 0.f : Q_UNITS / most;
+    int s2 = 0, s1 = 0, s0 = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint32_t p2 = 0, p1 = 0, p0 = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int e = 8 * (w >> 1) + 2 * b + (w & 1);  // even channels of 8, then the odd ones
+                const int v = bad ? 0 : (int)rintf(a[j][e] * inv);
+                const int d0 = (int)(int8_t)v, v1 = (v - d0) >> 8, d1 = (int)(int8_t)v1, d2 = (v1 - d1) >> 8;
+                s2 += d2, s1 += d1, s0 += d0;
+                p2 |= (uint32_t)(d2 & 255) << (8 * b);
+                p1 |= (uint32_t)(d1 & 255) << (8 * b);
+                p0 |= (uint32_t)(d0 & 255) << (8 * b);
+            }
+            r.digit[2][j][w] = (int)p2;
+            r.digit[1][j][w] = (int)p1;
+            r.digit[0][j][w] = (int)p0;
+        }
+    s2 = over_groups(s2), s1 = over_groups(s1), s0 = over_groups(s0);
+    r.sum_hi2 = -8 * s2, r.sum_hi1 = -8 * s1, r.sum_lo = -8 * s0;
+    r.unit = bad ? __builtin_nanf("") : most / Q_UNITS;
+    r.sum = fmaf((float)(s2 * 256 + s1), 256.f, (float)s0);
+}
+
+// 32 tokens of one key head as they lie in memory: two runs of 16, each within a block.
+template <int D>
+struct kv_tile {
+    static constexpr int NC = D == 256 ? 2 : 1;
+    uint32_t k[2][NC][4];  // (D = 64: two words)
+    uint32_t v[2][4][NC];
+    uint4 km[2], vm[2];
+    int pos[2];  // position of a run's first token; beyond every query where there is none
+};
+
+template <int D>
+__device__ __forceinline__ void load_tile(const uint8_t *const (&rec)[2], const int (&at)[2], int shift, int lane, kv_tile<D> &t) {
+    using R = kv4_rec<D>;
+    const int row = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const uint8_t *kp = rec[s] + (size_t)at[s] * R::ROW;
+        const uint8_t *vp = kp + R::v(shift);
+        const uint32_t ko = row * R::ROW + g * (D == 64 ? 8 : 16);
+        if (D == 64) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(kp + ko);
+            t.k[s][0][0] = x.x, t.k[s][0][1] = x.y, t.k[s][0][2] = t.k[s][0][3] = 0;
+        } else {
+#pragma unroll
+            for (int c = 0; c < kv_tile<D>::NC; ++c) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(kp + ko + 64 * c);
+                t.k[s][c][0] = x.x, t.k[s][c][1] = x.y, t.k[s][c][2] = x.z, t.k[s][c][3] = x.w;
+            }
+        }
+        const uint32_t vo = 4 * g * R::ROW + (D == 64 ? row >> 1 : row) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < kv_tile<D>::NC; ++c) t.v[s][i][c] = *reinterpret_cast<const uint32_t *>(vp + vo + i * R::ROW + 64 * c);
+        t.km[s] = *reinterpret_cast<const uint4 *>(rec[s] + R::k_meta(shift) + 4 * (size_t)at[s] + 16 * g);
+        t.vm[s] = *reinterpret_cast<const uint4 *>(rec[s] + R::v_meta(shift) + 4 * (size_t)at[s] + 16 * g);
+    }
+}
+
+// The running softmax of a wavefront's 16 rows: O^T in the accumulators (this lane's row, channels of D / 4 in a run).
+template <int D>
+struct softmax_rows {
+    static constexpr int NV = D / 16;
+    f32x4 o[NV];
+    float m, l, zsum;  // maximum (log2), sums over this lane's tokens
+    bool set;          // whether m is one (the same in a row's four lanes)
+    float step;        // power of two over every value step seen, 0 if none (the same in all lanes)
+    float norm;        // P_TOP / step
+};
+
+__device__ __forceinline__ uint32_t meta_at(const uint4 &m, int i) { return i == 0 ? m.x : i == 1 ? m.y : i == 2 ? m.z : m.w; }
+
+struct row_view {
+    int pos;              // this lane's row sees keys up to here (-1: no row)
+    int window, sinks;    // and, where window >= 0, from window behind it or below sinks
+};
+
+template <int D, bool CAP, bool MASKED>
+__device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &q, softmax_rows<D> &a, const row_view &rv, float c1, float sq, float cap_log2e, float inv_cap,
+                                          int lane) {
+    constexpr int NJ = D / 64, NV = D / 16, NC = kv_tile<D>::NC;
+    const int g = lane >> 4;
+    float s[8], dv[8], zv[8];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        i32x4 hi, lo;
+        i32x4 k8[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const uint32_t x = t.k[r][j >> 1][2 * (j & 1)], y = t.k[r][j >> 1][2 * (j & 1) + 1];
+            k8[j] = i32x4{(int)(x & 0x0f0f0f0fu), (int)(x >> 4 & 0x0f0f0f0fu), (int)(y & 0x0f0f0f0fu), (int)(y >> 4 & 0x0f0f0f0fu)};
+        }
+        hi = i32x4{q.sum_hi2, q.sum_hi2, q.sum_hi2, q.sum_hi2};
+        lo = i32x4{q.sum_lo, q.sum_lo, q.sum_lo, q.sum_lo};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[2][j], hi, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[0][j], lo, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hi[i] = (hi[i] << 8) + q.sum_hi1;  // |hi| < 2^26: 256 channels of 15 x 128 x 256 at most
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[1][j], hi, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = fmaf((float)hi[i], 256.f, (float)lo[i]);
+            const uint32_t km = meta_at(t.km[r], i), vm = meta_at(t.vm[r], i);
+            const float d = kv4_d(km), w = fmaf(0.5f, d, kv4_z(km));
+            float y;
+            if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(d * c1, x, w * sq) * inv_cap), -a.m);
+            else y = fmaf(d * c1, x, fmaf(w, sq, -a.m));
+            float z = kv4_z(vm), e = kv4_d(vm);
+            if (MASKED) {
+                const int key = t.pos[r] + 4 * g + i, far = rv.pos - key;
+                const bool seen = far >= 0 && (rv.window < 0 || far <= rv.window || key < rv.sinks);
+                y = seen ? y : -INFINITY;
+                z = seen ? z : 0.f;  // what is masked may be anything
+                e = seen ? e : 0.f;
+            }
+            s[4 * r + i] = y;
+            zv[4 * r + i] = z;
+            dv[4 * r + i] = e;
+        }
+    }
+    float p[8], pd[8], sum, top;
+    auto weigh = [&] {
+        sum = 0.f;
+        top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(s[i]);
+            sum += p[i];
+            pd[i] = p[i] * (dv[i] * a.norm);
+            top = fmaxf(top, pd[i]);
+        }
+    };
+    weigh();
+    bool off = !(top <= P_MOST) || !(sum < 1.2676506e30f);  // 2^100; a NaN is off too
+    if (!a.set) off = true;
+    {
+        float most = dv[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) most = fmaxf(most, dv[i]);
+        off |= most > a.step;
+        if (__ballot(off)) {
+            // The slow way: the rows' maxima and the largest step follow, what was summed is brought to them.
+            float at = s[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) at = fmaxf(at, s[i]);
+            at = max_groups(at);
+            float f = 1.f, shift = 0.f;
+            if (at > -INFINITY && (!a.set || at > 0.f)) {
+                f = a.set ? __builtin_amdgcn_exp2f(-at) : 1.f;
+                shift = at;
+                a.m += at;
+                a.set = true;
+            }
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+            float fo = f;
+            if (most > a.step) {
+                const float step = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+                fo *= a.step / step;
+                a.step = step;
+                a.norm = P_TOP / step;
+            }
+            a.l *= f;
+            a.zsum *= f;
+#pragma unroll
+            for (int n = 0; n < NV; ++n) a.o[n] *= fo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] -= shift;
+            weigh();
+        }
+    }
+    a.l += sum;
+    float zs = 0.f;
+    f16x8 ph, pl;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        zs = fmaf(p[i], zv[i], zs);
+        ph[i] = (_Float16)pd[i];
+    }
+    a.zsum += zs;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pl[i] = (_Float16)fmaf(-1.f, (float)ph[i], pd[i]);
+    // Values: of two tokens' words the byte that holds two channels, beside each other in 16 bits each.
+    const f16x2 low_by = {(_Float16)32768.f, (_Float16)32768.f}, high_by = {(_Float16)2048.f, (_Float16)2048.f};
+    const f16x2 centre = {(_Float16)(-7.5f * CODE), (_Float16)(-7.5f * CODE)};
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int b = 0; b < (D == 64 ? 2 : 4); ++b) {
+            uint32_t sel = 0x0c040c00u + 0x00010001u * b;
+            if (D == 64) sel += (lane & 1) ? 0x00020002u : 0u;  // an odd row's channels are in the word's upper half
+            f16x8 even, odd;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const uint32_t x = __builtin_amdgcn_perm(t.v[h >> 1][2 * (h & 1) + 1][c], t.v[h >> 1][2 * (h & 1)][c], sel);
+                const f16x2 e = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x000f000fu), low_by, centre);
+                const f16x2 o = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x00f000f0u), high_by, centre);
+                even[2 * h] = e[0], even[2 * h + 1] = e[1];
+                odd[2 * h] = o[0], odd[2 * h + 1] = o[1];
+            }
+            const int n = (D == 64 ? 0 : 8 * c) + 2 * b;
+            a.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph, a.o[n], 0, 0, 0);
+            a.o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph, a.o[n + 1], 0, 0, 0);
+            a.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, pl, a.o[n], 0, 0, 0);
+            a.o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, pl, a.o[n + 1], 0, 0, 0);
+        }
+}
+
+// One workgroup: 16 query rows of one key head (the rows of a request's tokens and of the head's group, token by token; or
+// with SELECTED the group's rows of one token) over one of `splits` runs of their keys, its four wavefronts every fourth
+// tile of 32 tokens.
+template <int D, bool CAP, bool SELECTED>
+__global__ __launch_bounds__(256) void kv4_rows_kernel(kv4_attn A) {
+    using R = kv4_rec<D>;
+    constexpr int STRIDE = D + 4;
+    __shared__ float so[4][16][STRIDE];
+    __shared__ float sm[4][16], sl[4][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    unsigned id = blockIdx.x;
+    const int split = id % A.splits;
+    id /= A.splits;
+    const int rt = id % A.row_tiles;
+    id /= A.row_tiles;
+    const int head = id % A.c.heads;
+    const int unit = id / A.c.heads;
+    const int shift = A.c.shift, bs = 1 << shift;
+
+    const int b = SELECTED ? kv4_request_of(A.ba.starts, A.ba.batch, unit) : unit;
+    if (SELECTED && b < 0) return;
+    const kv4_request rq = kv4_request_at(A.ba, b, shift);
+    const int tok0 = SELECTED ? unit - rq.first : 0;
+    const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group;
+    const int r0 = rt * 16;
+    if (r0 >= rows || (SELECTED && (unsigned)tok0 >= (unsigned)rq.rows)) return;
+    const int behind = rq.len - rq.rows;  // position of the request's first row
+    auto token_of = [&](int r) { return SELECTED ? tok0 : r / A.group; };
+    auto pos_of = [&](int r) { return A.mask == PG_MASK_NONE ? rq.len - 1 : behind + token_of(r); };
+    const int r = r0 + (lane & 15), last = min(r0 + 15, rows - 1);
+    const bool live = r < rows;
+    const int low_pos = pos_of(r0), high_pos = pos_of(last);
+    const bool windowed = A.mask == PG_MASK_CAUSAL_SLIDING_WINDOW;
+    const row_view rv = {live ? pos_of(r) : -1, windowed ? A.window : -1, A.sinks};
+
+    // The tiles that any row can see.
+    int near = 0, sink_tiles = 0, tiles;
+    const int *picked = nullptr;
+    if (SELECTED) {
+        picked = A.selected + ((size_t)unit * A.c.heads + head) * A.top;
+        const int blocks = high_pos < 0 ? 0 : min(A.top, (high_pos >> shift) + 1);
+        tiles = (int)((((long)blocks << shift) + 31) >> 5);
+    } else {
+        const int to = max(high_pos + 1, 0);
+        const int from = windowed ? max((long)low_pos - A.window, 0l) : 0;
+        near = from >> 5;
+        sink_tiles = windowed ? min((int)(((long)A.sinks + 31) >> 5), near) : 0;
+        tiles = to > 0 ? sink_tiles + ((to + 31) >> 5) - near : 0;
+    }
+    const int per = (tiles + A.splits - 1) / A.splits, begin = split * per, end = min(begin + per, tiles);
+
+    q_rows<D> q;
+    load_q<D>(live ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr, A.c.head_dim, g, q);
+    const float c1 = q.unit * A.scale * (CAP ? 1.f : LOG2E), sq = q.sum * c1;
+    const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
+
+    softmax_rows<D> a;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) a.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    a.m = 0.f, a.l = 0.f, a.zsum = 0.f, a.set = false, a.step = 0.f, a.norm = 0.f;
+
+    const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
+    auto fetch = [&](int tile, kv_tile<D> &t) {
+        const uint8_t *rec[2];
+        int at[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            int phys = -1, pos = 0x7fffff00;
+            if (SELECTED) {
+                const int v = 32 * tile + 16 * s, e = v >> shift;
+                if (e < A.top) {
+                    const int block = picked[e], before = e ? picked[e - 1] : -1;
+                    if (block > before && block >= 0 && block <= high_pos >> shift) {
+                        pos = (block << shift) + (v & (bs - 1));
+                        phys = table[block];
+                    }
+                }
+            } else {
+                const int p = 32 * (tile < sink_tiles ? tile : tile - sink_tiles + near) + 16 * s;
+                if (p <= high_pos) {
+                    pos = p;
+                    phys = table[p >> shift];
+                }
+            }
+            phys = __builtin_amdgcn_readfirstlane(phys);
+            pos = __builtin_amdgcn_readfirstlane(pos);
+            if ((unsigned)phys >= (unsigned)A.c.num_blocks) phys = 0, pos = 0x7fffff00;
+            t.pos[s] = pos;
+            at[s] = pos & (bs - 1);
+            if (pos == 0x7fffff00) at[s] = 0;
+            rec[s] = A.c.data + ((size_t)phys * A.c.heads + head) * R::bytes(shift);
+        }
+        load_tile<D>(rec, at, shift, lane, t);
+    };
+    auto take = [&](const kv_tile<D> &t) {
+        const bool whole = max(t.pos[0], t.pos[1]) + 15 <= low_pos && (!windowed || high_pos - min(t.pos[0], t.pos[1]) <= A.window);
+        if (whole) take_tile<D, CAP, false>(t, q, a, rv, c1, sq, cap_log2e, inv_cap, lane);
+        else take_tile<D, CAP, true>(t, q, a, rv, c1, sq, cap_log2e, inv_cap, lane);
+    };
+    kv_tile<D> t0, t1;
+    int tile = begin + wave;
+    if (tile < end) fetch(tile, t0);
+    while (tile < end) {
+        if (tile + 4 < end) fetch(tile + 4, t1);
+        take(t0);
+        tile += 4;
+        if (tile >= end) break;
+        if (tile + 4 < end) fetch(tile + 4, t0);
+        take(t1);
+        tile += 4;
+    }
+
+    // Four wavefronts' sums into one.
+    a.l = over_groups(a.l);
+    a.zsum = over_groups(a.zsum);
+    const float back = a.step * (1.f / (P_TOP * CODE));
+    constexpr int RUN = D / 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            const int d = D == 256 ? 128 * (n >> 3) + 32 * g + 8 * i + (n & 7) : RUN * g + (D / 16) * i + n;
+            so[wave][lane & 15][d] = fmaf(a.o[n][i], back, a.zsum);
+        }
+    if (g == 0) {
+        sm[wave][lane] = a.set ? a.m : a.l == 0.f ? -INFINITY : 0.f;  // (an unset maximum with a sum: NaN scores, which stay)
+        sl[wave][lane] = a.l;
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
+    if (r0 + row >= rows) return;
+    float m = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row])), w[4], l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = sm[i][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][row] - m);
+        l += w[i] == 0.f ? 0.f : w[i] * sl[i][row];
+    }
+    float *out;
+    float by = 1.f;
+    if (A.splits > 1) {
+        float *base = A.part + (size_t)blockIdx.x * (16 * D + 32);
+        out = base + row * D;
+        if (part == 0) base[16 * D + row] = m, base[16 * D + 16 + row] = l;
+    } else {
+        const int rr = r0 + row;
+        out = A.out + ((size_t)(rq.first + token_of(rr)) * A.q_heads + head * A.group + (SELECTED ? rr : rr % A.group)) * A.c.head_dim;
+        by = l == 0.f ? 0.f : 1.f / l;
+    }
+    const int most = A.splits > 1 ? D : A.c.head_dim;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+        const int d = part + 16 * i;
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v += w[j] == 0.f ? 0.f : w[j] * so[j][row][d];
+        if (d < most) out[d] = v * by;
+    }
+}
+
+// The splits of a row into its output, in their order: a wavefront a row.
+template <int D, bool SELECTED>
+__global__ __launch_bounds__(256) void kv4_join_kernel(kv4_attn A) {
+    const int lane = threadIdx.x & 63;
+    const unsigned id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = id & 15;
+    unsigned tile = id >> 4;
+    const size_t first = (size_t)tile * A.splits;
+    const int rt = tile % A.row_tiles;
+    tile /= A.row_tiles;
+    const int head = tile % A.c.heads, unit = tile / A.c.heads;
+    const int b = SELECTED ? kv4_request_of(A.ba.starts, A.ba.batch, unit) : unit;
+    if (b < 0 || (!SELECTED && b >= A.ba.batch)) return;
+    const kv4_request rq = kv4_request_at(A.ba, b, A.c.shift);
+    const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group, r = rt * 16 + row;
+    if (r >= rows || (SELECTED && (unsigned)(unit - rq.first) >= (unsigned)rq.rows)) return;
+    const int token = SELECTED ? unit : rq.first + r / A.group;
+    const float *part = A.part + first * (16 * D + 32);
+    constexpr size_t NEXT = 16 * D + 32;
+    float m = -INFINITY;
+    for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, part[s * NEXT + 16 * D + row]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    float l = 0.f, o[D / 64];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
+    for (int s = 0; s < A.splits; ++s) {
+        const float ms = part[s * NEXT + 16 * D + row];
+        if (ms == -INFINITY) continue;
+        const float w = __builtin_amdgcn_exp2f(ms - m);
+        if (w == 0.f) continue;
+        l += w * part[s * NEXT + 16 * D + 16 + row];
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) o[i] += w * part[s * NEXT + row * D + 64 * i + lane];
+    }
+    const float by = l == 0.f ? 0.f : 1.f / l;
+    float *out = A.out + ((size_t)token * A.q_heads + head * A.group + (SELECTED ? r : r % A.group)) * A.c.head_dim;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+        if (64 * i + lane < A.c.head_dim) out[64 * i + lane] = o[i] * by;
+}
+
+// ---- selection ------------------------------------------------------------------------------
+
+struct kv4_pick {
+    const float *q;
+    size_t q_token, q_head;
+    kv4_view c;
+    kv4_batch ba;
+    int group, top, first, recent;
+    int *selected;
+};
+
+// Blocks in the order of their scores as whole numbers: a larger key is a larger score.
+__device__ __forceinline__ uint32_t score_key(float s) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, s + 0.f);  // -0 counts as 0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// One workgroup: one query token and key head.  Scores of 16 blocks a wavefront at a time -- rows of the product are the
+// group's query rows (x where positive, x where negative), columns the blocks (hi, lo), whole numbers throughout, and two
+// f32 products a score -- then the key that exactly `top` blocks reach by four passes of 8 bits over a histogram in LDS,
+// then the blocks over it, and of those at it the first, in ascending order.
+template <int D, int T>
+__global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
+    using R = kv4_rec<D>;
+    constexpr int NJ = D / 64, W = T / 64;
+    extern __shared__ uint32_t keys[];  // [blocks]
+    __shared__ uint32_t hist[256];
+    __shared__ int above[W], at_key[W], found[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4, tid = threadIdx.x;
+    const int token = blockIdx.x / A.c.heads, head = blockIdx.x % A.c.heads, shift = A.c.shift;
+    int *out = A.selected + ((size_t)token * A.c.heads + head) * A.top;
+    const int b = kv4_request_of(A.ba.starts, A.ba.batch, token);
+    if (b < 0) return;
+    const kv4_request rq = kv4_request_at(A.ba, b, shift);
+    if ((unsigned)(token - rq.first) >= (unsigned)rq.rows) return;
+    const int pos = rq.len - rq.rows + (token - rq.first);
+    const int blocks = pos < 0 ? 0 : (pos >> shift) + 1;
+    if (blocks <= A.top) {
+        for (int j = tid; j < A.top; j += T) out[j] = j < blocks ? j : -1;
+        return;
+    }
+    const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
+    for (int r0 = 0; r0 < A.group; r0 += 16) {
+        const float *x = r0 + row < A.group ? A.q + (size_t)token * A.q_token + (size_t)(head * A.group + r0 + row) * A.q_head : nullptr;
+        i32x4 pos8[NJ], neg8[NJ];
+        float a[NJ][16], most = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int d = 64 * j + 16 * g + e;
+                a[j][e] = x && d < A.c.head_dim ? x[d] : 0.f;
+                most = fmaxf(most, fabsf(a[j][e]));
+                bad |= !(fabsf(a[j][e]) <= 3.402823466e38f);
+            }
+        most = max_groups(most);
+        bad = max_groups(bad ? 1.f : 0.f) != 0.f;
+        const float r = bad || most < 7.88860905e-31f ? 0.f : 1.0f / most * 127.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t up = 0, down = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = bad ? 0 : (int)rintf(a[j][4 * w + e] * r);
+                    up |= (uint32_t)(max(v, 0) & 255) << (8 * e);
+                    down |= (uint32_t)(min(v, 0) & 255) << (8 * e);
+                }
+                pos8[j][w] = (int)up;
+                neg8[j][w] = (int)down;
+            }
+        // a lane's four rows of the result are rows 4 g + i
+        float unit[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unit[i] = __shfl(bad ? 0.f : most * (1.0f / 127.f), 4 * g + i);
+        for (int j0 = 16 * wave; j0 < blocks; j0 += 16 * W) {
+            const int block = j0 + row;
+            const int phys = block < blocks ? table[block] : -1;
+            const bool there = phys >= 0 && phys < A.c.num_blocks;
+            const uint8_t *s = A.c.sums + ((size_t)(there ? phys : 0) * A.c.heads + head) * R::SUM;
+            i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos8[j], *reinterpret_cast<const i32x4 *>(s + 64 * j + 16 * g), acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg8[j], *reinterpret_cast<const i32x4 *>(s + D + 64 * j + 16 * g), acc, 0, 0, 0);
+            }
+            const float scale = *reinterpret_cast<const float *>(s + 2 * D);
+            float score = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + 4 * g + i < A.group) score = fmaxf(score, ((float)acc[i] * unit[i]) * scale);
+            if (scale == INFINITY) score = INFINITY;  // the block holds a key that is not finite: it is not to be missed
+            if (!there) score = -INFINITY;
+            score = max_groups(score);
+            if (g == 0 && block < blocks) {
+                uint32_t key = score_key(score);
+                if (r0) key = max(key, keys[block]);
+                if (block < A.first || block >= blocks - A.recent) key = 0xffffffffu;
+                keys[block] = key;
+            }
+        }
+    }
+    __syncthreads();
+    // The key of the block that is the top-th, and how many blocks at that key are wanted.
+    uint32_t prefix = 0, mask = 0;
+    int want = A.top;
+#pragma unroll 1
+    for (int at = 24; at >= 0; at -= 8) {
+        for (int i = tid; i < 256; i += T) hist[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < blocks; j += T) {
+            const uint32_t key = keys[j];
+            if ((key & mask) == prefix) atomicAdd(&hist[key >> at & 255], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {  // the bins from the top, four a lane
+            uint32_t h[4], mine = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[i] = hist[255 - 4 * lane - i];
+                mine += h[i];
+            }
+            uint32_t upto = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t u = __shfl_up(upto, d);
+                if (lane >= d) upto += u;
+            }
+            uint32_t over = upto - mine;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (over < (uint32_t)want && over + h[i] >= (uint32_t)want) found[0] = 255 - 4 * lane - i, found[1] = want - (int)over;
+                over += h[i];
+            }
+        }
+        __syncthreads();
+        prefix |= (uint32_t)found[0] << at;
+        mask |= 255u << at;
+        want = found[1];
+    }
+    // A thread's run of blocks: how many it has over the key and at it, then where its own go.
+    const int per = (blocks + T - 1) / T, from = min(tid * per, blocks), to = min(from + per, blocks);
+    int over = 0, equal = 0;
+    for (int j = from; j < to; ++j) {
+        over += keys[j] > prefix;
+        equal += keys[j] == prefix;
+    }
+    int over_upto = over, equal_upto = equal;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(over_upto, d), v = __shfl_up(equal_upto, d);
+        if (lane >= d) over_upto += u, equal_upto += v;
+    }
+    if (lane == 63) above[wave] = over_upto, at_key[wave] = equal_upto;
+    __syncthreads();
+    int o = over_upto - over, q = equal_upto - equal;
+    for (int w = 0; w < wave; ++w) o += above[w], q += at_key[w];
+    for (int j = from; j < to; ++j) {
+        const uint32_t key = keys[j];
+        const bool eq = key == prefix;
+        if (key > prefix || (eq && q < want)) out[o + min(q, want)] = j;
+        o += key > prefix;
+        q += eq;
+    }
+}
+
+template <class F>
+pg_status with_width(int D, F f) {
+    if (D == 64) return f(std::integral_constant<int, 64>{});
+    if (D == 128) return f(std::integral_constant<int, 128>{});
+    return f(std::integral_constant<int, 256>{});
+}
+
+size_t part_bytes(int D, size_t tiles, size_t splits) { return splits > 1 ? tiles * splits * (16 * (size_t)D + 32) * sizeof(float) : 0; }
+
+// Runs that a row tile's keys are divided in: as many as fill the chip with workgroups (`per_cu` on each), none shorter
+// than two tiles a wavefront.
+size_t pick_splits(const pg_ctx *ctx, size_t tiles, size_t tokens) {
+    const size_t fill = (size_t)ctx->num_cu * 3;
+    size_t splits = tiles ? (fill + tiles - 1) / tiles : 1;
+    const size_t most = (tokens + 255) / 256;
+    if (splits > most) splits = most;
+    return splits < 1 ? 1 : splits;
+}
+
+struct plan {
+    size_t row_tiles, tiles, splits, bytes;
+};
+plan dense_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t max_query, size_t max_blocks) {
+    plan p;
+    p.row_tiles = (max_query * (num_q_heads / c->heads) + 15) / 16;
+    p.tiles = batch * c->heads * p.row_tiles;
+    p.splits = pick_splits(ctx, p.tiles, max_blocks * c->block_size);
+    p.bytes = part_bytes(c->D, p.tiles, p.splits);
+    return p;
+}
+plan selected_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t tokens, size_t top) {
+    plan p;
+    p.row_tiles = (num_q_heads / c->heads + 15) / 16;
+    p.tiles = tokens * c->heads * p.row_tiles;
+    p.splits = pick_splits(ctx, p.tiles, top * c->block_size);
+    p.bytes = part_bytes(c->D, p.tiles, p.splits);
+    return p;
+}
+
+template <bool SELECTED>
+pg_status launch_rows(pg_ctx *ctx, const char *fn, const pg_paged_kv4 *c, kv4_attn &A, const plan &p) {
+    if (p.tiles * p.splits >= (1u << 24)) return pg_fail(PG_EUNSUPPORTED, "%s: %zu row tiles in %zu runs are more than a launch takes", fn, p.tiles, p.splits);
+    A.splits = (int)p.splits;
+    A.row_tiles = (int)p.row_tiles;
+    return with_width(c->D, [&](auto w) -> pg_status {
+        constexpr int D = decltype(w)::value;
+        PG_TRY(pg_launch(ctx, SELECTED ? "kv4_selected_kernel" : "kv4_rows_kernel", A.cap > 0.f ? kv4_rows_kernel<D, true, SELECTED> : kv4_rows_kernel<D, false, SELECTED>,
+                         dim3((unsigned)(p.tiles * p.splits)), dim3(256), 0, A));
+        if (p.splits == 1) return PG_OK;
+        return pg_launch(ctx, "kv4_join_kernel", kv4_join_kernel<D, SELECTED>, dim3((unsigned)(p.tiles * 4)), dim3(256), 0, A);
+    });
+}
+
+pg_status check_score(const char *fn, float scale, float logit_cap) {
+    PG_CHECK_ARG(isfinite(scale), "%s: scale is not finite", fn);
+    PG_CHECK_ARG(logit_cap >= 0.f && isfinite(logit_cap), "%s: logit_cap is negative or not finite", fn);
+    return PG_OK;
+}
+
+}  // namespace
+
+PG_API pg_status pg_paged_kv4_attention_scratch(pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t max_query, size_t max_blocks, size_t *bytes) {
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step("pg_paged_kv4_attention_scratch", c, num_q_heads, batch, max_query, max_blocks));
+    PG_CHECK_ARG(bytes != nullptr, "pg_paged_kv4_attention_scratch: null output");
+    *bytes = dense_plan(ctx, c, num_q_heads, batch, max_query, max_blocks).bytes;
+    return PG_OK;
+}
+
+PG_API pg_status pg_paged_kv4_selected_scratch(pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t tokens, size_t top_k, size_t *bytes) {
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step("pg_paged_kv4_selected_scratch", c, num_q_heads, 0, tokens, 1));
+    PG_CHECK_ARG(bytes != nullptr, "pg_paged_kv4_selected_scratch: null output");
+    *bytes = selected_plan(ctx, c, num_q_heads, tokens, top_k).bytes;
+    return PG_OK;
+}
+
+PG_API pg_status pg_paged_kv4_attention_dev(pg_ctx *ctx, const pg_paged_kv4 *c, const float *q_dev, size_t q_token_stride, size_t q_head_stride, size_t num_q_heads,
+                                            const int32_t *query_start_dev, const int32_t *seq_lens_dev, size_t batch, size_t tokens, size_t max_query,
+                                            const int32_t *block_table_dev, size_t max_blocks, float scale, int mask_kind, size_t window, size_t sink_tokens, float logit_cap,
+                                            void *scratch_dev, size_t scratch_bytes, float *out_dev) {
+    static const char *fn = "pg_paged_kv4_attention";
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
+    PG_TRY(check_score(fn, scale, logit_cap));
+    PG_CHECK_ARG(mask_kind >= PG_MASK_NONE && mask_kind <= PG_MASK_CAUSAL_SLIDING_WINDOW, "%s: unknown mask kind %d", fn, mask_kind);
+    if (tokens == 0 || batch == 0 || max_query == 0) return PG_OK;
+    PG_CHECK_ARG(q_dev && query_start_dev && seq_lens_dev && block_table_dev && out_dev, "%s: null pointer", fn);
+    PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
+    if (max_query > tokens) max_query = tokens;
+    const plan p = dense_plan(ctx, c, num_q_heads, batch, max_query, max_blocks);
+    PG_CHECK_ARG(p.bytes == 0 || (scratch_dev && scratch_bytes >= p.bytes && ((uintptr_t)scratch_dev & 15) == 0),
+                 "%s: scratch of %zu bytes, %zu are needed (16-byte aligned)", fn, scratch_bytes, p.bytes);
+    c->touch(ctx);
+    kv4_attn A = {};
+    A.q = q_dev, A.q_token = q_token_stride, A.q_head = q_head_stride;
+    A.c = kv4_view_of(c);
+    A.ba = {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks};
+    A.scale = scale, A.cap = logit_cap, A.mask = mask_kind;
+    A.window = (int)(window > 0x3fffffffu ? 0x3fffffffu : window), A.sinks = (int)(sink_tokens > 0x3fffffffu ? 0x3fffffffu : sink_tokens);
+    A.group = (int)(num_q_heads / c->heads), A.q_heads = (int)num_q_heads, A.max_query = (int)max_query;
+    A.part = static_cast<float *>(scratch_dev), A.out = out_dev;
+    return launch_rows<false>(ctx, fn, c, A, p);
+}
+
+PG_API pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *c, const float *q_dev, size_t q_token_stride, size_t q_head_stride, size_t num_q_heads,
+                                         const int32_t *query_start_dev, const int32_t *seq_lens_dev, size_t batch, size_t tokens, const int32_t *block_table_dev,
+                                         size_t max_blocks, size_t top_k, size_t first_blocks, size_t recent_blocks, int32_t *selected_dev) {
+    static const char *fn = "pg_paged_kv4_select";
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
+    PG_CHECK_ARG(top_k > 0 && top_k < (1u << 24) && recent_blocks >= 1 && first_blocks <= top_k && recent_blocks <= top_k && first_blocks + recent_blocks <= top_k,
+                 "%s: %zu blocks with the first %zu and the last %zu of them (the last at least one)", fn, top_k, first_blocks, recent_blocks);
+    if (tokens == 0 || batch == 0) return PG_OK;
+    PG_CHECK_ARG(q_dev && query_start_dev && seq_lens_dev && block_table_dev && selected_dev, "%s: null pointer", fn);
+    PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
+    const size_t lds = max_blocks * sizeof(uint32_t);
+    if (lds > (144u << 10)) return pg_fail(PG_EUNSUPPORTED, "%s: tables of %zu blocks (36864 at most: their scores live in on-chip memory)", fn, max_blocks);
+    if (tokens * c->heads >= (1u << 22)) return pg_fail(PG_EUNSUPPORTED, "%s: %zu rows of %zu key heads are more than a launch takes", fn, tokens, c->heads);
+    c->touch(ctx);
+    kv4_pick A = {q_dev, q_token_stride, q_head_stride, kv4_view_of(c), {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks},
+                  (int)(num_q_heads / c->heads), (int)top_k, (int)first_blocks, (int)recent_blocks, selected_dev};
+    return with_width(c->D, [&](auto w) -> pg_status {
+        constexpr int D = decltype(w)::value;
+        auto go = [&](auto kernel, unsigned threads) -> pg_status {
+            if (lds > (48u << 10)) PG_TRY(pg_allow_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds));
+            return pg_launch(ctx, "kv4_select_kernel", kernel, dim3((unsigned)(tokens * c->heads)), dim3(threads), lds, A);
+        };
+        return max_blocks > 256 && tokens * c->heads <= (size_t)ctx->num_cu * 2 ? go(kv4_select_kernel<D, 1024>, 1024) : go(kv4_select_kernel<D, 256>, 256);
+    });
+}
+
+PG_API pg_status pg_paged_kv4_attention_selected_dev(pg_ctx *ctx, const pg_paged_kv4 *c, const float *q_dev, size_t q_token_stride, size_t q_head_stride, size_t num_q_heads,
+                                                     const int32_t *query_start_dev, const int32_t *seq_lens_dev, size_t batch, size_t tokens,
+                                                     const int32_t *block_table_dev, size_t max_blocks, const int32_t *selected_dev, size_t top_k, float scale,
+                                                     float logit_cap, void *scratch_dev, size_t scratch_bytes, float *out_dev) {
+    static const char *fn = "pg_paged_kv4_attention_selected";
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
+    PG_TRY(check_score(fn, scale, logit_cap));
+    PG_CHECK_ARG(top_k > 0 && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
+    if (tokens == 0 || batch == 0) return PG_OK;
+    PG_CHECK_ARG(q_dev && query_start_dev && seq_lens_dev && block_table_dev && selected_dev && out_dev, "%s: null pointer", fn);
+    PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
+    const plan p = selected_plan(ctx, c, num_q_heads, tokens, top_k);
+    PG_CHECK_ARG(p.bytes == 0 || (scratch_dev && scratch_bytes >= p.bytes && ((uintptr_t)scratch_dev & 15) == 0),
+                 "%s: scratch of %zu bytes, %zu are needed (16-byte aligned)", fn, scratch_bytes, p.bytes);
+    c->touch(ctx);
+    kv4_attn A = {};
+    A.q = q_dev, A.q_token = q_token_stride, A.q_head = q_head_stride;
+    A.c = kv4_view_of(c);
+    A.ba = {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks};
+    A.selected = selected_dev, A.top = (int)top_k;
+    A.scale = scale, A.cap = logit_cap, A.mask = PG_MASK_CAUSAL;
+    A.group = (int)(num_q_heads / c->heads), A.q_heads = (int)num_q_heads, A.max_query = 1;
+    A.part = static_cast<float *>(scratch_dev), A.out = out_dev;
+    return launch_rows<true>(ctx, fn, c, A, p);
+}
+
+// ---- host arrays ----------------------------------------------------------------------------
+
+namespace {
+
+// What a step's host arrays say, refused where a kernel would have had to leave something out.
+pg_status check_host_step(const char *fn, const pg_paged_kv4 *c, const int32_t *query_start, const int32_t *seq_lens, size_t batch, size_t tokens, const int32_t *block_table,
+                          size_t max_blocks) {
+    PG_CHECK_ARG(query_start[0] == 0 && query_start[batch] >= 0 && (size_t)query_start[batch] <= tokens, "%s: rows %d to %d of %zu", fn, query_start[0], query_start[batch], tokens);
+    for (size_t b = 0; b < batch; ++b) {
+        PG_CHECK_ARG(query_start[b + 1] >= query_start[b], "%s: request %zu starts at row %d and ends at %d", fn, b, query_start[b], query_start[b + 1]);
+        PG_CHECK_ARG(seq_lens[b] >= 0 && (size_t)seq_lens[b] <= max_blocks * c->block_size, "%s: request %zu has %d tokens, its table room for %zu", fn, b, seq_lens[b],
+                     max_blocks * c->block_size);
+        PG_CHECK_ARG(query_start[b + 1] - query_start[b] <= seq_lens[b], "%s: request %zu has %d rows and %d tokens", fn, b, query_start[b + 1] - query_start[b], seq_lens[b]);
+        const size_t used = ((size_t)seq_lens[b] + c->block_size - 1) / c->block_size;
+        for (size_t j = 0; j < used; ++j) {
+            const int32_t e = block_table[b * max_blocks + j];
+            PG_CHECK_ARG(e >= 0 && (size_t)e < c->num_blocks, "%s: request %zu's block %zu is %d of %zu", fn, b, j, e, c->num_blocks);
+        }
+    }
+    return PG_OK;
+}
+
+struct host_step {
+    pg_dev_block starts, lens, table;
+    pg_status in(pg_ctx *ctx, const int32_t *query_start, const int32_t *seq_lens, size_t batch, const int32_t *block_table, size_t max_blocks) {
+        PG_TRY(pg_host_in(ctx, query_start, (batch + 1) * sizeof(int32_t), starts));
+        PG_TRY(pg_host_in(ctx, seq_lens, batch * sizeof(int32_t), lens));
+        return pg_host_in(ctx, block_table, batch * max_blocks * sizeof(int32_t), table);
+    }
+};
+
+}  // namespace
+
+PG_API pg_status pg_paged_kv4_summarise(pg_ctx *ctx, pg_paged_kv4 *c, const int32_t *query_start, const int32_t *seq_lens, size_t batch, const int32_t *block_table,
+                                        size_t max_blocks) {
+    static const char *fn = "pg_paged_kv4_summarise";
+    PG_TRY(pg_use(ctx));
+    PG_CHECK_ARG(c != nullptr, "%s: null cache", fn);
+    PG_TRY(pg_kv4_check_step(fn, c, c->heads, batch, 0, max_blocks));
+    if (batch == 0) return PG_OK;
+    PG_CHECK_ARG(query_start && seq_lens && block_table, "%s: null pointer", fn);
+    PG_TRY(check_host_step(fn, c, query_start, seq_lens, batch, 0x7fffffff, block_table, max_blocks));
+    const size_t tokens = (size_t)query_start[batch];
+    host_step h;
+    PG_TRY(h.in(ctx, query_start, seq_lens, batch, block_table, max_blocks));
+    PG_TRY(pg_paged_kv4_summarise_dev(ctx, c, h.starts.as<int32_t>(), h.lens.as<int32_t>(), batch, tokens, h.table.as<int32_t>(), max_blocks));
+    PG_HIP(hipStreamSynchronize(ctx->stream));
+    return PG_OK;
+}
+
+PG_API pg_status pg_paged_kv4_attention(pg_ctx *ctx, const pg_paged_kv4 *c, const float *q, size_t num_q_heads, const int32_t *query_start, const int32_t *seq_lens,
+                                        size_t batch, size_t tokens, const int32_t *block_table, size_t max_blocks, float scale, int mask_kind, size_t window,
+                                        size_t sink_tokens, float logit_cap, float *out) {
+    static const char *fn = "pg_paged_kv4_attention";
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
+    PG_TRY(check_score(fn, scale, logit_cap));
+    PG_CHECK_ARG(mask_kind >= PG_MASK_NONE && mask_kind <= PG_MASK_CAUSAL_SLIDING_WINDOW, "%s: unknown mask kind %d", fn, mask_kind);
+    if (tokens == 0 || batch == 0) return PG_OK;
+    PG_CHECK_ARG(q && query_start && seq_lens && block_table && out, "%s: null pointer", fn);
+    PG_TRY(check_host_step(fn, c, query_start, seq_lens, batch, tokens, block_table, max_blocks));
+    size_t longest = 0;
+    for (size_t b = 0; b < batch; ++b) longest = std::max(longest, (size_t)(query_start[b + 1] - query_start[b]));
+    const size_t rows = (size_t)query_start[batch], row = num_q_heads * c->head_dim, bytes = rows * row * sizeof(float);
+    if (rows == 0) return PG_OK;
+    size_t scratch = 0;
+    PG_TRY(pg_paged_kv4_attention_scratch(ctx, c, num_q_heads, batch, longest, max_blocks, &scratch));
+    host_step h;
+    pg_dev_block dq, dout, ds;
+    PG_TRY(h.in(ctx, query_start, seq_lens, batch, block_table, max_blocks));
+    PG_TRY(pg_host_in(ctx, q, bytes, dq));
+    PG_TRY(dout.alloc(ctx, bytes));
+    PG_TRY(ds.alloc(ctx, scratch));
+    PG_TRY(pg_paged_kv4_attention_dev(ctx, c, dq.as<float>(), row, c->head_dim, num_q_heads, h.starts.as<int32_t>(), h.lens.as<int32_t>(), batch, rows, longest,
+                                      h.table.as<int32_t>(), max_blocks, scale, mask_kind, window, sink_tokens, logit_cap, ds.p, scratch, dout.as<float>()));
+    return pg_host_out(ctx, out, dout.p, bytes);
+}
+
+PG_API pg_status pg_paged_kv4_select(pg_ctx *ctx, const pg_paged_kv4 *c, const float *q, size_t num_q_heads, const int32_t *query_start, const int32_t *seq_lens, size_t batch,
+                                     size_t tokens, const int32_t *block_table, size_t max_blocks, size_t top_k, size_t first_blocks, size_t recent_blocks,
+                                     int32_t *selected) {
+    static const char *fn = "pg_paged_kv4_select";
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
+    if (tokens == 0 || batch == 0) return PG_OK;
+    PG_CHECK_ARG(q && query_start && seq_lens && block_table && selected, "%s: null pointer", fn);
+    PG_TRY(check_host_step(fn, c, query_start, seq_lens, batch, tokens, block_table, max_blocks));
+    const size_t rows = (size_t)query_start[batch], row = num_q_heads * c->head_dim, bytes = rows * c->heads * top_k * sizeof(int32_t);
+    if (rows == 0) return PG_OK;
+    host_step h;
+    pg_dev_block dq, dsel;
+    PG_TRY(h.in(ctx, query_start, seq_lens, batch, block_table, max_blocks));
+    PG_TRY(pg_host_in(ctx, q, rows * row * sizeof(float), dq));
+    PG_CHECK_ARG(top_k < (1u << 24), "%s: %zu blocks: out of range", fn, top_k);
+    PG_TRY(dsel.alloc(ctx, bytes));
+    PG_TRY(pg_paged_kv4_select_dev(ctx, c, dq.as<float>(), row, c->head_dim, num_q_heads, h.starts.as<int32_t>(), h.lens.as<int32_t>(), batch, rows, h.table.as<int32_t>(),
+                                   max_blocks, top_k, first_blocks, recent_blocks, dsel.as<int32_t>()));
+    return pg_host_out(ctx, selected, dsel.p, bytes);
+}
+
+PG_API pg_status pg_paged_kv4_attention_selected(pg_ctx *ctx, const pg_paged_kv4 *c, const float *q, size_t num_q_heads, const int32_t *query_start, const int32_t *seq_lens,
+                                                 size_t batch, size_t tokens, const int32_t *block_table, size_t max_blocks, const int32_t *selected, size_t top_k,
+                                                 float scale, float logit_cap, float *out) {
+    static const char *fn = "pg_paged_kv4_attention_selected";
+    PG_TRY(pg_use(ctx));
+    PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
+    PG_TRY(check_score(fn, scale, logit_cap));
+    PG_CHECK_ARG(top_k > 0 && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
+    if (tokens == 0 || batch == 0) return PG_OK;
+    PG_CHECK_ARG(q && query_start && seq_lens && block_table && selected && out, "%s: null pointer", fn);
+    PG_TRY(check_host_step(fn, c, query_start, seq_lens, batch, tokens, block_table, max_blocks));
+    const size_t rows = (size_t)query_start[batch], row = num_q_heads * c->head_dim, bytes = rows * row * sizeof(float);
+    if (rows == 0) return PG_OK;
+    for (size_t b = 0, t = 0; b < batch; ++b)
+        for (; t < (size_t)query_start[b + 1]; ++t) {
+            const int64_t pos = seq_lens[b] - (query_start[b + 1] - (int64_t)t);
+            for (size_t h = 0; h < c->heads; ++h) {
+                const int32_t *s = selected + (t * c->heads + h) * top_k;
+                for (size_t i = 0; i < top_k; ++i)
+                    PG_CHECK_ARG(s[i] == -1 || (s[i] >= 0 && s[i] <= pos / (int64_t)c->block_size && (i == 0 || s[i] > s[i - 1])),
+                                 "%s: row %zu, key head %zu: block %d as number %zu (ascending, up to the row's own %lld, -1 behind them)", fn, t, h, s[i], i,
+                                 (long long)(pos / (int64_t)c->block_size));
+            }
+        }
+    size_t scratch = 0;
+    PG_TRY(pg_paged_kv4_selected_scratch(ctx, c, num_q_heads, rows, top_k, &scratch));
+    host_step h;
+    pg_dev_block dq, dsel, dout, ds;
+    PG_TRY(h.in(ctx, query_start, seq_lens, batch, block_table, max_blocks));
+    PG_TRY(pg_host_in(ctx, q, bytes, dq));
+    PG_TRY(pg_host_in(ctx, selected, rows * c->heads * top_k * sizeof(int32_t), dsel));
+    PG_TRY(dout.alloc(ctx, bytes));
+    PG_TRY(ds.alloc(ctx, scratch));
+    PG_TRY(pg_paged_kv4_attention_selected_dev(ctx, c, dq.as<float>(), row, c->head_dim, num_q_heads, h.starts.as<int32_t>(), h.lens.as<int32_t>(), batch, rows,
+                                               h.table.as<int32_t>(), max_blocks, dsel.as<int32_t>(), top_k, scale, logit_cap, ds.p, scratch, dout.as<float>()));
+    return pg_host_out(ctx, out, dout.p, bytes);
+}
