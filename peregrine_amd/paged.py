@@ -82,7 +82,8 @@ class PagedKV4Cache:
         k, v = self._rows(k, "k"), self._rows(v, "v")
         if k.shape != v.shape or k.shape[1] != self.num_kv_heads:
             raise ValueError("PagedKV4Cache.append: k and v are not [tokens, num_kv_heads, head_dim]")
-        _ffi.check(_ffi.lib.pg_paged_kv4_append(self.ctx.handle, self._h, _ptr(k.reshape(-1)), _ptr(v.reshape(-1)), k.shape[0], _ptr(_i32(slots, k.shape[0], "slots"))))
+        slots = _i32(slots, k.shape[0], "slots")
+        _ffi.check(_ffi.lib.pg_paged_kv4_append(self.ctx.handle, self._h, _ptr(k.reshape(-1)), _ptr(v.reshape(-1)), k.shape[0], _ptr(slots)))
 
     def read(self, slots):
         """(k, v) of the slots, [n, num_kv_heads, head_dim] each, as the values that the codes stand for."""
