@@ -68,50 +68,69 @@ __device__ __forceinline__ constexpr int q_base(int j, int g) {
     return D == 64 ? 16 * g : 128 * (j >> 1) + 32 * g + 16 * (j & 1);
 }
 
-// x: the row (or null: zeros).  A row with a value that is not finite gets a NaN unit.
+// This lane's channels of a query row in fixed point, as words of which byte b is digit b (signed, -128 .. 127), in the order of
+// the key operand: even channels of 8, then the odd ones.  x + 0x808080 has the digits plus 128 in its bytes.
 template <int D>
-__device__ __forceinline__ void load_q(const float *x, int head_dim, int g, q_rows<D> &r) {
+struct q_fixed {
+    static constexpr int NJ = D / 64;
+    int y[NJ][16];
+    float unit, sum;  // value of a unit (NaN for a row that is not finite), the row's sum in units
+};
+// x: the row, or null (zeros).
+template <int D>
+__device__ __forceinline__ void fix_q(const float *x, int head_dim, int g, q_fixed<D> &r) {
     constexpr int NJ = D / 64;
     float a[NJ][16];
-    float most = 0.f;
-    bool bad = false;
+    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int d = q_base<D>(j, g) + e;
+            const int d = q_base<D>(j, g) + 8 * (e >> 3) + 2 * (e & 3) + (e >> 2 & 1);
             a[j][e] = x && d < head_dim ? x[d] : 0.f;
-            most = fmaxf(most, fabsf(a[j][e]));
-            bad |= !(fabsf(a[j][e]) <= 3.402823466e38f);
+            top = max(top, __builtin_bit_cast(uint32_t, a[j][e]) & 0x7fffffffu);  // (of magnitudes the bits are in order, NaN last)
         }
-    most = max_groups(most);
-    bad = max_groups(bad ? 1.f : 0.f) != 0.f;
-    const bool none = bad || most < 7.88860905e-31f;  // 2^-100: scores of 0
-    const float inv = none ? 0.f : Q_UNITS / most;
-    int s2 = 0, s1 = 0, s0 = 0;
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    const bool bad = top >= 0x7f800000u;
+    const float most = __builtin_bit_cast(float, top);
+    const float inv = bad || most < 7.88860905e-31f ? 0.f : Q_UNITS / most;  // under 2^-100: scores of 0
+    int sum = 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            uint32_t p2 = 0, p1 = 0, p0 = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int e = 8 * (w >> 1) + 2 * b + (w & 1);  // even channels of 8, then the odd ones
-                const int v = bad ? 0 : (int)rintf(a[j][e] * inv);
-                const int d0 = (int)(int8_t)v, v1 = (v - d0) >> 8, d1 = (int)(int8_t)v1, d2 = (v1 - d1) >> 8;
-                s2 += d2, s1 += d1, s0 += d0;
-                p2 |= (uint32_t)(d2 & 255) << (8 * b);
-                p1 |= (uint32_t)(d1 & 255) << (8 * b);
-                p0 |= (uint32_t)(d0 & 255) << (8 * b);
-            }
-            r.digit[2][j][w] = (int)p2;
-            r.digit[1][j][w] = (int)p1;
-            r.digit[0][j][w] = (int)p0;
+        for (int e = 0; e < 16; ++e) {
+            const int v = bad ? 0 : (int)rintf(a[j][e] * inv);
+            sum += v;
+            r.y[j][e] = (v + 0x808080) ^ 0x808080;
         }
-    s2 = over_groups(s2), s1 = over_groups(s1), s0 = over_groups(s0);
-    r.sum_hi2 = -8 * s2, r.sum_hi1 = -8 * s1, r.sum_lo = -8 * s0;
     r.unit = bad ? __builtin_nanf("") : most / Q_UNITS;
-    r.sum = fmaf((float)(s2 * 256 + s1), 256.f, (float)s0);
+    r.sum = over_groups((float)sum);
+}
+// Byte `digit` of four words, in one.
+__device__ __forceinline__ int pick_digit(const int *y, uint32_t sel) {  // sel = (4 + digit) << 8 | digit
+    const uint32_t lo = __builtin_amdgcn_perm((uint32_t)y[1], (uint32_t)y[0], sel), hi = __builtin_amdgcn_perm((uint32_t)y[3], (uint32_t)y[2], sel);
+    return (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+__device__ __forceinline__ int sum_bytes(int x, int s) { return __builtin_amdgcn_sdot4(x, 0x01010101, s, false); }
+
+template <int D>
+__device__ __forceinline__ void load_q(const float *x, int head_dim, int g, q_rows<D> &r) {
+    q_fixed<D> f;
+    fix_q<D>(x, head_dim, g, f);
+    int s[3] = {0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                r.digit[p][j][w] = pick_digit(&f.y[j][4 * w], 0x0400u + 0x0101u * p);
+                s[p] = sum_bytes(r.digit[p][j][w], s[p]);
+            }
+    r.sum_hi2 = -8 * over_groups(s[2]), r.sum_hi1 = -8 * over_groups(s[1]), r.sum_lo = -8 * over_groups(s[0]);
+    r.unit = f.unit;
+    r.sum = f.sum;
 }
 
 // 32 tokens of one key head as they lie in memory: two runs of 16, each within a block.
@@ -217,27 +236,31 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
             dv[4 * r + i] = e;
         }
     }
-    float p[8], pd[8], sum, top;
+    float p[8], pd[8], sum;
+    uint32_t top;
     auto weigh = [&] {
         sum = 0.f;
-        top = 0.f;
+        top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             p[i] = __builtin_amdgcn_exp2f(s[i]);
             sum += p[i];
             pd[i] = p[i] * (dv[i] * a.norm);
-            top = fmaxf(top, pd[i]);
+            top = max(top, __builtin_bit_cast(uint32_t, pd[i]));  // (none is negative: the bits are in order, NaN last)
         }
     };
     weigh();
-    bool off = !(top <= P_MOST) || !(sum < 1.2676506e30f);  // 2^100; a NaN is off too
+    bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < 1.2676506e30f);  // 2^100; a NaN is off too
     if (!a.set) off = true;
     {
-        float most = dv[0];
+        uint32_t steps = 0;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) most = fmaxf(most, dv[i]);
-        off |= most > a.step;
+        for (int i = 0; i < 8; ++i) steps = max(steps, __builtin_bit_cast(uint32_t, dv[i]));
+        off |= steps > __builtin_bit_cast(uint32_t, a.step);
         if (__ballot(off)) {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, dv[i]);
             // The slow way: the rows' maxima and the largest step follow, what was summed is brought to them.
             float at = s[0];
 #pragma unroll
@@ -269,7 +292,8 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
         }
     }
     a.l += sum;
-    float zs = 0.f;
+    float zs = 0.f, minus = -1.f;
+    asm("" : "+s"(minus));  // (not a subtraction, so that one instruction takes the f16 as it is)
     f16x8 ph, pl;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -278,7 +302,7 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
     }
     a.zsum += zs;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) pl[i] = (_Float16)fmaf(-1.f, (float)ph[i], pd[i]);
+    for (int i = 0; i < 8; ++i) pl[i] = (_Float16)fmaf((float)ph[i], minus, pd[i]);
     // Values: of two tokens' words the byte that holds two channels, beside each other in 16 bits each.
     const f16x2 low_by = {(_Float16)32768.f, (_Float16)32768.f}, high_by = {(_Float16)2048.f, (_Float16)2048.f};
     const f16x2 centre = {(_Float16)(-7.5f * CODE), (_Float16)(-7.5f * CODE)};
@@ -309,7 +333,7 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
 // with SELECTED the group's rows of one token) over one of `splits` runs of their keys, its four wavefronts every fourth
 // tile of 32 tokens.
 template <int D, bool CAP, bool SELECTED>
-__global__ __launch_bounds__(256) void kv4_rows_kernel(kv4_attn A) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_rows_kernel(kv4_attn A) {
     using R = kv4_rec<D>;
     constexpr int STRIDE = D + 4;
     __shared__ float so[4][16][STRIDE];
@@ -356,16 +380,6 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(kv4_attn A) {
     }
     const int per = (tiles + A.splits - 1) / A.splits, begin = split * per, end = min(begin + per, tiles);
 
-    q_rows<D> q;
-    load_q<D>(live ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr, A.c.head_dim, g, q);
-    const float c1 = q.unit * A.scale * (CAP ? 1.f : LOG2E), sq = q.sum * c1;
-    const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
-
-    softmax_rows<D> a;
-#pragma unroll
-    for (int n = 0; n < D / 16; ++n) a.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    a.m = 0.f, a.l = 0.f, a.zsum = 0.f, a.set = false, a.step = 0.f, a.norm = 0.f;
-
     const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
     auto fetch = [&](int tile, kv_tile<D> &t) {
         const uint8_t *rec[2];
@@ -399,22 +413,28 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(kv4_attn A) {
         }
         load_tile<D>(rec, at, shift, lane, t);
     };
-    auto take = [&](const kv_tile<D> &t) {
+    kv_tile<D> t;
+    int tile = begin + wave;
+    if (tile < end) fetch(tile, t);  // on its way while the queries are made ready
+    q_rows<D> q;
+    load_q<D>(live ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr, A.c.head_dim, g, q);
+    const float c1 = q.unit * A.scale * (CAP ? 1.f : LOG2E), sq = q.sum * c1;
+    const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
+
+    softmax_rows<D> a;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) a.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    a.m = 0.f, a.l = 0.f, a.zsum = 0.f, a.set = false, a.step = 0.f, a.norm = 0.f;
+
+    auto take = [&] {
         const bool whole = max(t.pos[0], t.pos[1]) + 15 <= low_pos && (!windowed || high_pos - min(t.pos[0], t.pos[1]) <= A.window);
         if (whole) take_tile<D, CAP, false>(t, q, a, rv, c1, sq, cap_log2e, inv_cap, lane);
         else take_tile<D, CAP, true>(t, q, a, rv, c1, sq, cap_log2e, inv_cap, lane);
     };
-    kv_tile<D> t0, t1;
-    int tile = begin + wave;
-    if (tile < end) fetch(tile, t0);
     while (tile < end) {
-        if (tile + 4 < end) fetch(tile + 4, t1);
-        take(t0);
+        take();
         tile += 4;
-        if (tile >= end) break;
-        if (tile + 4 < end) fetch(tile + 4, t0);
-        take(t1);
-        tile += 4;
+        if (tile < end) fetch(tile, t);
     }
 
     // Four wavefronts' sums into one.
@@ -464,13 +484,480 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(kv4_attn A) {
     }
 }
 
-// The splits of a row into its output, in their order: a wavefront a row.
-template <int D, bool SELECTED>
+// ---- up to eight rows -----------------------------------------------------------------------
+// A decoding step has a group's rows alone (4 or 8 for most models), and 16 columns of scores are mostly padding then: the
+// exponentials and everything else that is done by score would be done four times too often.  Here the digits of q are rows
+// of one product instead of three products, 64 tokens at a time: S = Q K^T with rows (digit, head) and columns the
+// tokens of a run.  A lane then has four heads' scores of one digit, and two swaps between lane halves and two between
+// quarters of four runs' results leave it all three digits of one token of its own: 64 tokens x 4 heads are four scores
+// a lane.  For O^T = V^T P^T the probabilities cross the lanes once, through LDS, as f16: columns (high half, head), (low
+// half, head), so that one product takes both.
+
+template <int D>
+struct kv_tile64 {
+    static constexpr int NC = D == 256 ? 2 : 1, KW = D == 64 ? 2 : 4;
+    uint32_t k[4][NC][KW];
+    uint32_t v[4][4][NC];
+    uint32_t km[2], vm[2];  // of this lane's tokens
+    int pos[4];
+};
+
+// Row HB of a wavefront: HB = 4 or 8 heads (rows of the caller), digits of q as rows of A.
+template <int D, int HB>
+struct q_few {
+    static constexpr int NJ = D / 64, SETS = HB == 4 ? 1 : 2;
+    i32x4 digit[SETS][NJ];
+    i32x4 start[SETS];      // -8 times the sums of the digits: (n - 8) for n
+    float unit[4], sum[4];  // of this lane's heads
+};
+
+template <int D, int HB>
+__device__ __forceinline__ void load_q_few(const float *x, int head_dim, int lane, q_few<D, HB> &r) {
+    constexpr int NJ = D / 64, SETS = HB == 4 ? 1 : 2;
+    const int g = lane >> 4, row = lane & 15;
+    q_fixed<D> f;
+    fix_q<D>(x, head_dim, g, f);
+    // HB = 4: rows 0-3 the high digit, 4-7 the middle one, 8-11 the low one, 12-15 nothing
+    // HB = 8: rows 0-7 high, 8-15 middle; second set: rows 0-7 low, 8-15 nothing
+    const int digit0 = HB == 4 ? 2 - (row >> 2) : 2 - (row >> 3);
+    const uint32_t sel0 = digit0 < 0 ? 0x0c0cu : 0x0400u + 0x0101u * (uint32_t)digit0, sel1 = row < 8 ? 0x0400u : 0x0c0cu;
+    int s0 = 0, s1 = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            s0 = sum_bytes(r.digit[0][j][w] = pick_digit(&f.y[j][4 * w], sel0), s0);
+            if (SETS == 2) s1 = sum_bytes(r.digit[SETS - 1][j][w] = pick_digit(&f.y[j][4 * w], sel1), s1);
+        }
+    s0 = -8 * over_groups(s0);
+    if (SETS == 2) s1 = -8 * over_groups(s1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.start[0][i] = __shfl(s0, 4 * g + i);
+        if (SETS == 2) r.start[SETS - 1][i] = __shfl(s1, 4 * g + i);
+        const int from = HB == 4 ? i : 4 * (g & 1) + i;
+        r.unit[i] = __shfl(f.unit, from);
+        r.sum[i] = __shfl(f.sum, from);
+    }
+}
+
+// Lanes 32-63 of a with lanes 0-31 of b; lanes 16-31 and 48-63 of a with lanes 0-15 and 32-47 of b.
+__device__ __forceinline__ void swap_halves(int &a, int &b) {
+    const auto r = __builtin_amdgcn_permlane32_swap((unsigned)a, (unsigned)b, false, false);
+    a = (int)r[0], b = (int)r[1];
+}
+__device__ __forceinline__ void swap_quarters(int &a, int &b) {
+    const auto r = __builtin_amdgcn_permlane16_swap((unsigned)a, (unsigned)b, false, false);
+    a = (int)r[0], b = (int)r[1];
+}
+
+template <int D>
+struct softmax_few {
+    f32x4 o[D / 16];                  // O^T: this lane's column, channels of D / 4 in a run
+    float m[4], l[4], zsum[4];        // of this lane's heads; the sums over this lane's tokens
+    bool set[4];
+    float step, norm;
+};
+
+constexpr int P_ROW = 72;  // f16 from one row of probabilities to the next: 64 and a shift of four banks
+
+template <int HB>
+__device__ __forceinline__ float max_heads(float v) {  // over the lanes that have this lane's heads
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+    if (HB == 4) v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+template <int HB>
+__device__ __forceinline__ float sum_heads(float v) {
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
+    if (HB == 4) v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+template <int D, int HB, bool CAP, bool MASKED>
+__device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D, HB> &q, softmax_few<D> &a, const int (&row_pos)[4], int window, int sinks,
+                                            const float (&c1)[4], const float (&sq)[4], float cap_log2e, float inv_cap, int lane, _Float16 *pbuf) {
+    constexpr int NJ = D / 64, NC = kv_tile64<D>::NC, SETS = HB == 4 ? 1 : 2, NT = HB / 4;  // NT: tokens a lane
+    const int g = lane >> 4, c = lane & 15;
+    i32x4 acc[SETS][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) acc[s][u] = q.start[s];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const uint32_t x = t.k[u][j >> 1][2 * (j & 1)], y = t.k[u][j >> 1][2 * (j & 1) + 1];
+            const i32x4 k8 = {(int)(x & 0x0f0f0f0fu), (int)(x >> 4 & 0x0f0f0f0fu), (int)(y & 0x0f0f0f0fu), (int)(y >> 4 & 0x0f0f0f0fu)};
+#pragma unroll
+            for (int s = 0; s < SETS; ++s) acc[s][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.digit[s][j], k8, acc[s][u], 0, 0, 0);
+        }
+    }
+    float s[NT][4], dv[NT], zv[NT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (HB == 4) {
+            int x0 = acc[0][0][i], x1 = acc[0][1][i], x2 = acc[0][2][i], x3 = acc[0][3][i];
+            swap_halves(x0, x2);
+            swap_halves(x1, x3);
+            swap_quarters(x0, x1);
+            swap_quarters(x2, x3);
+            s[0][i] = fmaf((float)((x0 << 8) + x1), 256.f, (float)x2);
+        } else {
+#pragma unroll
+            for (int p = 0; p < NT; ++p) {
+                int x0 = acc[0][2 * p][i], x1 = acc[0][2 * p + 1][i], y0 = acc[SETS - 1][2 * p][i], y1 = acc[SETS - 1][2 * p + 1][i];
+                swap_halves(x0, x1);
+                swap_halves(y0, y1);
+                s[p][i] = fmaf((float)((x0 << 8) + x1), 256.f, (float)y0);
+            }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < NT; ++p) {
+        const float d = kv4_d(t.km[p]), w = fmaf(0.5f, d, kv4_z(t.km[p]));
+        zv[p] = kv4_z(t.vm[p]);
+        dv[p] = kv4_d(t.vm[p]);
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float y;
+            if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(d * c1[i], s[p][i], w * sq[i]) * inv_cap), -a.m[i]);
+            else y = fmaf(d * c1[i], s[p][i], fmaf(w, sq[i], -a.m[i]));
+            if (MASKED) {
+                const int run = HB == 4 ? (g == 0 ? t.pos[0] : g == 1 ? t.pos[1] : g == 2 ? t.pos[2] : t.pos[3]) : (g < 2 ? t.pos[2 * p] : t.pos[2 * p + 1]);
+                const int key = run + c, far = row_pos[i] - key;
+                const bool seen = far >= 0 && (window < 0 || far <= window || key < sinks);
+                y = seen ? y : -INFINITY;
+                any |= seen;
+            }
+            s[p][i] = y;
+        }
+        if (MASKED) {  // what no row sees may be anything; a row's own mask is on its probability below
+            zv[p] = any ? zv[p] : 0.f;
+            dv[p] = any ? dv[p] : 0.f;
+        }
+    }
+    float pr[NT][4], pd[NT][4], sum[4], total;
+    uint32_t top;
+    auto weigh = [&] {
+        total = 0.f;
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum[i] = 0.f;
+#pragma unroll
+            for (int p = 0; p < NT; ++p) {
+                pr[p][i] = __builtin_amdgcn_exp2f(s[p][i]);
+                sum[i] += pr[p][i];
+                pd[p][i] = pr[p][i] * (dv[p] * a.norm);
+                if (MASKED) pd[p][i] = s[p][i] == -INFINITY ? 0.f : pd[p][i];  // (a step of NaN is not this row's where it is masked)
+                top = max(top, __builtin_bit_cast(uint32_t, pd[p][i]));  // (none is negative: the bits are in order, NaN last)
+            }
+            total += sum[i];
+        }
+    };
+    weigh();
+    bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(total < 1.2676506e30f);  // 2^100; a NaN is off too
+    const uint32_t steps = max(__builtin_bit_cast(uint32_t, dv[0]), __builtin_bit_cast(uint32_t, dv[NT - 1]));
+    off |= !(a.set[0] && a.set[1] && a.set[2] && a.set[3]) || steps > __builtin_bit_cast(uint32_t, a.step);
+    if (__ballot(off)) {
+        float most = fmaxf(0.f, dv[0]);
+        if (NT == 2) most = fmaxf(most, dv[NT - 1]);
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float at = s[0][i];
+            if (NT == 2) at = fmaxf(at, s[NT - 1][i]);
+            at = max_heads<HB>(at);
+            f[i] = 1.f;
+            if (at > -INFINITY && (!a.set[i] || at > 0.f)) {
+                f[i] = a.set[i] ? __builtin_amdgcn_exp2f(-at) : 1.f;
+                a.m[i] += at;
+                a.set[i] = true;
+#pragma unroll
+                for (int p = 0; p < NT; ++p) s[p][i] -= at;
+            }
+            a.l[i] *= f[i];
+            a.zsum[i] *= f[i];
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+        // the column's head: its factor from a lane that has it
+        float fo = 1.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float fi = HB == 4 ? f[i] : __shfl(f[i], 16 * (c >> 2 & 1));
+            fo = (c & 3) == i ? fi : fo;
+        }
+        if (most > a.step) {
+            const float step = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+            fo *= a.step / step;
+            a.step = step;
+            a.norm = P_TOP / step;
+        }
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) a.o[n] *= fo;
+        weigh();
+    }
+    float minus = -1.f;
+    asm("" : "+s"(minus));  // (not a subtraction, so that one instruction takes the f16 as it is)
+    // Probabilities to LDS: row (half, head), the tokens of 32 in the order in which the value operand's lanes have them.
+#pragma unroll
+    for (int p = 0; p < NT; ++p) {
+        const int u = HB == 4 ? g : 2 * p + (g >> 1);
+        const int at = 32 * (u >> 1) + 8 * (c >> 2) + 4 * (u & 1) + (c & 3);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int head = HB == 4 ? i : 4 * (g & 1) + i;
+            const _Float16 hi = (_Float16)pd[p][i];
+            pbuf[head * P_ROW + at] = hi;
+            pbuf[(HB + head) * P_ROW + at] = (_Float16)fmaf((float)hi, minus, pd[p][i]);
+            a.zsum[i] = MASKED ? a.zsum[i] + (s[p][i] == -INFINITY ? 0.f : pr[p][i] * zv[p]) : fmaf(pr[p][i], zv[p], a.zsum[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a.l[i] += sum[i];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const f16x2 low_by = {(_Float16)32768.f, (_Float16)32768.f}, high_by = {(_Float16)2048.f, (_Float16)2048.f};
+    const f16x2 centre = {(_Float16)(-7.5f * CODE), (_Float16)(-7.5f * CODE)};
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const f16x8 ph = *reinterpret_cast<const f16x8 *>(pbuf + (c & (2 * HB - 1)) * P_ROW + 32 * w + 8 * g);
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc)
+#pragma unroll
+            for (int b = 0; b < (D == 64 ? 2 : 4); ++b) {
+                uint32_t sel = 0x0c040c00u + 0x00010001u * b;
+                if (D == 64) sel += (lane & 1) ? 0x00020002u : 0u;
+                f16x8 even, odd;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const uint32_t x = __builtin_amdgcn_perm(t.v[2 * w + (h >> 1)][2 * (h & 1) + 1][cc], t.v[2 * w + (h >> 1)][2 * (h & 1)][cc], sel);
+                    const f16x2 e = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x000f000fu), low_by, centre);
+                    const f16x2 o = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x00f000f0u), high_by, centre);
+                    even[2 * h] = e[0], even[2 * h + 1] = e[1];
+                    odd[2 * h] = o[0], odd[2 * h + 1] = o[1];
+                }
+                const int n = (D == 64 ? 0 : 8 * cc) + 2 * b;
+                a.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ph, a.o[n], 0, 0, 0);
+                a.o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ph, a.o[n + 1], 0, 0, 0);
+            }
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// As kv4_rows_kernel, for up to HB rows of a unit: one row tile, wavefronts every fourth tile of 64 tokens.
+template <int D, int HB, bool CAP, bool SELECTED>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_few_kernel(kv4_attn A) {
+    using R = kv4_rec<D>;
+    constexpr int STRIDE = D + 4;
+    __shared__ __attribute__((aligned(16))) char lds[4 * 2 * HB * STRIDE * 4 > 4 * 2 * HB * P_ROW * 2 ? 4 * 2 * HB * STRIDE * 4 : 4 * 2 * HB * P_ROW * 2];
+    __shared__ float sm[4][HB], sl[4][HB], sz[4][HB], sback[4];
+    auto so = reinterpret_cast<float(*)[2 * HB][STRIDE]>(lds);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+    unsigned id = blockIdx.x;
+    const int split = id % A.splits;
+    id /= A.splits;
+    const int head = id % A.c.heads;
+    const int unit = id / A.c.heads;
+    const int shift = A.c.shift, bs = 1 << shift;
+
+    const int b = SELECTED ? kv4_request_of(A.ba.starts, A.ba.batch, unit) : unit;
+    if (SELECTED && b < 0) return;
+    const kv4_request rq = kv4_request_at(A.ba, b, shift);
+    const int tok0 = SELECTED ? unit - rq.first : 0;
+    const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group;
+    if (rows <= 0 || (SELECTED && (unsigned)tok0 >= (unsigned)rq.rows)) return;
+    const int behind = rq.len - rq.rows;
+    auto token_of = [&](int r) { return SELECTED ? tok0 : r / A.group; };
+    auto pos_of = [&](int r) { return A.mask == PG_MASK_NONE ? rq.len - 1 : behind + token_of(r); };
+    const int low_pos = pos_of(0), high_pos = pos_of(rows - 1);
+    const bool windowed = A.mask == PG_MASK_CAUSAL_SLIDING_WINDOW;
+    const int window = windowed ? A.window : -1;
+
+    int near = 0, sink_tiles = 0, tiles;
+    const int *picked = nullptr;
+    if (SELECTED) {
+        picked = A.selected + ((size_t)unit * A.c.heads + head) * A.top;
+        const int blocks = high_pos < 0 ? 0 : min(A.top, (high_pos >> shift) + 1);
+        tiles = (int)((((long)blocks << shift) + 63) >> 6);
+    } else {
+        const int to = max(high_pos + 1, 0);
+        const int from = windowed ? max((long)low_pos - A.window, 0l) : 0;
+        near = from >> 6;
+        sink_tiles = windowed ? min((int)(((long)A.sinks + 63) >> 6), near) : 0;
+        tiles = to > 0 ? sink_tiles + ((to + 63) >> 6) - near : 0;
+    }
+    const int per = (tiles + A.splits - 1) / A.splits, begin = split * per, end = min(begin + per, tiles);
+
+    const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
+    auto fetch = [&](int tile, kv_tile64<D> &t) {
+        const uint8_t *rec[4];
+        int at[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            int phys = -1, pos = 0x7fffff00;
+            if (SELECTED) {
+                const int v = 64 * tile + 16 * u, e = v >> shift;
+                if (e < A.top) {
+                    const int block = picked[e], before = e ? picked[e - 1] : -1;
+                    if (block > before && block >= 0 && block <= high_pos >> shift) {
+                        pos = (block << shift) + (v & (bs - 1));
+                        phys = table[block];
+                    }
+                }
+            } else {
+                const int p = 64 * (tile < sink_tiles ? tile : tile - sink_tiles + near) + 16 * u;
+                if (p <= high_pos) {
+                    pos = p;
+                    phys = table[p >> shift];
+                }
+            }
+            phys = __builtin_amdgcn_readfirstlane(phys);
+            pos = __builtin_amdgcn_readfirstlane(pos);
+            if ((unsigned)phys >= (unsigned)A.c.num_blocks) phys = 0, pos = 0x7fffff00;
+            t.pos[u] = pos;
+            at[u] = pos == 0x7fffff00 ? 0 : pos & (bs - 1);
+            rec[u] = A.c.data + ((size_t)phys * A.c.heads + head) * R::bytes(shift);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint8_t *kp = rec[u] + (size_t)at[u] * R::ROW, *vp = kp + R::v(shift);
+            const uint32_t ko = c * R::ROW + g * (D == 64 ? 8 : 16);
+#pragma unroll
+            for (int cc = 0; cc < kv_tile64<D>::NC; ++cc) {
+                if (D == 64) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(kp + ko);
+                    t.k[u][cc][0] = x.x, t.k[u][cc][1] = x.y;
+                } else {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(kp + ko + 64 * cc);
+                    t.k[u][cc][0] = x.x, t.k[u][cc][1] = x.y, t.k[u][cc][kv_tile64<D>::KW - 2] = x.z, t.k[u][cc][kv_tile64<D>::KW - 1] = x.w;
+                }
+            }
+            const uint32_t vo = 4 * g * R::ROW + (D == 64 ? c >> 1 : c) * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int cc = 0; cc < kv_tile64<D>::NC; ++cc) t.v[u][i][cc] = *reinterpret_cast<const uint32_t *>(vp + vo + i * R::ROW + 64 * cc);
+        }
+#pragma unroll
+        for (int p = 0; p < HB / 4; ++p) {
+            // this lane's token: HB = 4 of run g, HB = 8 of run 2 p + (g >> 1)
+            const uint8_t *r0 = HB == 4 ? (g < 2 ? (g == 0 ? rec[0] : rec[1]) : (g == 2 ? rec[2] : rec[3])) : (g < 2 ? rec[2 * p] : rec[2 * p + 1]);
+            const int a0 = HB == 4 ? (g < 2 ? (g == 0 ? at[0] : at[1]) : (g == 2 ? at[2] : at[3])) : (g < 2 ? at[2 * p] : at[2 * p + 1]);
+            const uint32_t *mp = reinterpret_cast<const uint32_t *>(r0 + R::k_meta(shift)) + a0 + c;
+            t.km[p] = mp[0];
+            t.vm[p] = mp[(size_t)1 << shift];
+        }
+    };
+    kv_tile64<D> t;
+    int tile = begin + wave;
+    if (tile < end) fetch(tile, t);  // on its way while the queries are made ready
+    q_few<D, HB> q;
+    float c1[4], sq[4];
+    int row_pos[4];
+    {
+        const int r = HB == 4 ? c & 3 : c & 7;
+        load_q_few<D, HB>(r < rows ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr,
+                          A.c.head_dim, lane, q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int mine = HB == 4 ? i : 4 * (g & 1) + i;
+            c1[i] = q.unit[i] * A.scale * (CAP ? 1.f : LOG2E);
+            sq[i] = q.sum[i] * c1[i];
+            row_pos[i] = mine < rows ? pos_of(mine) : -1;
+        }
+    }
+    const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
+
+    softmax_few<D> a;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) a.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a.m[i] = a.l[i] = a.zsum[i] = 0.f, a.set[i] = false;
+    a.step = a.norm = 0.f;
+    _Float16 *pbuf = reinterpret_cast<_Float16 *>(lds) + wave * 2 * HB * P_ROW;
+
+    auto take = [&] {
+        const int far = max(max(t.pos[0], t.pos[1]), max(t.pos[2], t.pos[3])), close = min(min(t.pos[0], t.pos[1]), min(t.pos[2], t.pos[3]));
+        const bool whole = far + 15 <= low_pos && (!windowed || high_pos - close <= A.window);
+        if (whole) take_tile64<D, HB, CAP, false>(t, q, a, row_pos, window, A.sinks, c1, sq, cap_log2e, inv_cap, lane, pbuf);
+        else take_tile64<D, HB, CAP, true>(t, q, a, row_pos, window, A.sinks, c1, sq, cap_log2e, inv_cap, lane, pbuf);
+    };
+    while (tile < end) {
+        take();
+        tile += 4;
+        if (tile < end) fetch(tile, t);
+    }
+
+    // Four wavefronts' sums, and each column's two halves, into one.
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a.l[i] = sum_heads<HB>(a.l[i]);
+        a.zsum[i] = sum_heads<HB>(a.zsum[i]);
+    }
+    __syncthreads();  // (the probabilities' memory is the sums')
+    constexpr int RUN = D / 4;
+    if (c < 2 * HB)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                const int d = D == 256 ? 128 * (n >> 3) + 32 * g + 8 * i + (n & 7) : RUN * g + (D / 16) * i + n;
+                so[wave][c][d] = a.o[n][i];
+            }
+    if (c == 0 && g < HB / 4)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int h = 4 * g + i;
+            sm[wave][h] = a.set[i] ? a.m[i] : a.l[i] == 0.f ? -INFINITY : 0.f;
+            sl[wave][h] = a.l[i];
+            sz[wave][h] = a.zsum[i];
+        }
+    if (lane == 0) sback[wave] = a.step * (1.f / (P_TOP * CODE));
+    __syncthreads();
+    constexpr int TPR = 256 / HB;
+    const int row = threadIdx.x / TPR, part = threadIdx.x % TPR;
+    if (row >= rows) return;
+    float m = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row])), w[4], l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = sm[i][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][row] - m);
+        l += w[i] == 0.f ? 0.f : w[i] * sl[i][row];
+    }
+    float *out;
+    float by = 1.f;
+    if (A.splits > 1) {
+        float *base = A.part + (size_t)blockIdx.x * (HB * D + 32);
+        out = base + row * D;
+        if (part == 0) base[HB * D + row] = m, base[HB * D + 16 + row] = l;
+    } else {
+        out = A.out + ((size_t)(rq.first + token_of(row)) * A.q_heads + head * A.group + (SELECTED ? row : row % A.group)) * A.c.head_dim;
+        by = l == 0.f ? 0.f : 1.f / l;
+    }
+    const int most = A.splits > 1 ? D : A.c.head_dim;
+#pragma unroll
+    for (int d = part; d < D; d += TPR) {
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v += w[j] == 0.f ? 0.f : w[j] * fmaf(so[j][row][d] + so[j][HB + row][d], sback[j], sz[j][row]);
+        if (d < most) out[d] = v * by;
+    }
+}
+
+// The splits of a row into its output, in their order: a wavefront a row, `RT` rows a tile.  The splits' weights first, a lane a
+// split, so that the loop over their rows waits for nothing but its loads.
+template <int D, int RT, bool SELECTED>
 __global__ __launch_bounds__(256) void kv4_join_kernel(kv4_attn A) {
+    constexpr size_t NEXT = RT * D + 32;
     const int lane = threadIdx.x & 63;
     const unsigned id = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = id & 15;
-    unsigned tile = id >> 4;
+    const int row = id % RT;
+    unsigned tile = id / RT;
     const size_t first = (size_t)tile * A.splits;
     const int rt = tile % A.row_tiles;
     tile /= A.row_tiles;
@@ -478,26 +965,35 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(kv4_attn A) {
     const int b = SELECTED ? kv4_request_of(A.ba.starts, A.ba.batch, unit) : unit;
     if (b < 0 || (!SELECTED && b >= A.ba.batch)) return;
     const kv4_request rq = kv4_request_at(A.ba, b, A.c.shift);
-    const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group, r = rt * 16 + row;
+    const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group, r = rt * RT + row;
     if (r >= rows || (SELECTED && (unsigned)(unit - rq.first) >= (unsigned)rq.rows)) return;
     const int token = SELECTED ? unit : rq.first + r / A.group;
-    const float *part = A.part + first * (16 * D + 32);
-    constexpr size_t NEXT = 16 * D + 32;
+    const float *part = A.part + first * NEXT;
     float m = -INFINITY;
-    for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, part[s * NEXT + 16 * D + row]);
+    for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, part[s * NEXT + RT * D + row]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
     float l = 0.f, o[D / 64];
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
-    for (int s = 0; s < A.splits; ++s) {
-        const float ms = part[s * NEXT + 16 * D + row];
-        if (ms == -INFINITY) continue;
-        const float w = __builtin_amdgcn_exp2f(ms - m);
-        if (w == 0.f) continue;
-        l += w * part[s * NEXT + 16 * D + 16 + row];
+    for (int s0 = 0; s0 < A.splits; s0 += 64) {
+        const int s = s0 + lane, n = min(64, A.splits - s0);
+        const float ms = s < A.splits ? part[s * NEXT + RT * D + row] : -INFINITY;
+        const float w = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+        float mine = w == 0.f ? 0.f : w * part[s * NEXT + RT * D + 16 + row];
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) o[i] += w * part[s * NEXT + row * D + 64 * i + lane];
+        for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d);
+        l += mine;
+        const float *rows_at = part + s0 * NEXT + row * D + lane;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+            const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const float x = rows_at[j * NEXT + 64 * i];
+                o[i] += wj == 0.f ? 0.f : wj * x;  // (a run that saw nothing may hold anything)
+            }
+        }
     }
     const float by = l == 0.f ? 0.f : 1.f / l;
     float *out = A.out + ((size_t)token * A.q_heads + head * A.group + (SELECTED ? r : r % A.group)) * A.c.head_dim;
@@ -681,36 +1177,33 @@ pg_status with_width(int D, F f) {
     return f(std::integral_constant<int, 256>{});
 }
 
-size_t part_bytes(int D, size_t tiles, size_t splits) { return splits > 1 ? tiles * splits * (16 * (size_t)D + 32) * sizeof(float) : 0; }
-
-// Runs that a row tile's keys are divided in: as many as fill the chip with workgroups (`per_cu` on each), none shorter
-// than two tiles a wavefront.
-size_t pick_splits(const pg_ctx *ctx, size_t tiles, size_t tokens) {
-    const size_t fill = (size_t)ctx->num_cu * 3;
-    size_t splits = tiles ? (fill + tiles - 1) / tiles : 1;
+// Runs that a row tile's keys are divided in: as many as fill the chip with workgroups, none shorter than a tile of 64
+// tokens a wavefront.
+size_t pick_splits(const pg_ctx *ctx, int D, size_t tiles, size_t tokens) {
+    const size_t fill = (size_t)ctx->num_cu * (D == 256 ? 1 : 2);  // what runs at once
+    size_t splits = tiles ? fill / tiles : 1;
     const size_t most = (tokens + 255) / 256;
     if (splits > most) splits = most;
     return splits < 1 ? 1 : splits;
 }
 
 struct plan {
-    size_t row_tiles, tiles, splits, bytes;
+    size_t rows, row_tiles, tiles, splits, bytes;  // rows a tile (4, 8 or 16)
 };
-plan dense_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t max_query, size_t max_blocks) {
+plan plan_for(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t units, size_t unit_rows, size_t tokens) {
     plan p;
-    p.row_tiles = (max_query * (num_q_heads / c->heads) + 15) / 16;
-    p.tiles = batch * c->heads * p.row_tiles;
-    p.splits = pick_splits(ctx, p.tiles, max_blocks * c->block_size);
-    p.bytes = part_bytes(c->D, p.tiles, p.splits);
+    p.rows = unit_rows <= 4 ? 4 : unit_rows <= 8 ? 8 : 16;
+    p.row_tiles = (unit_rows + p.rows - 1) / p.rows;
+    p.tiles = units * c->heads * p.row_tiles;
+    p.splits = pick_splits(ctx, c->D, p.tiles, tokens);
+    p.bytes = p.splits > 1 ? p.tiles * p.splits * (p.rows * (size_t)c->D + 32) * sizeof(float) : 0;
     return p;
 }
+plan dense_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t max_query, size_t max_blocks) {
+    return plan_for(ctx, c, batch, max_query * (num_q_heads / c->heads), max_blocks * c->block_size);
+}
 plan selected_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t tokens, size_t top) {
-    plan p;
-    p.row_tiles = (num_q_heads / c->heads + 15) / 16;
-    p.tiles = tokens * c->heads * p.row_tiles;
-    p.splits = pick_splits(ctx, p.tiles, top * c->block_size);
-    p.bytes = part_bytes(c->D, p.tiles, p.splits);
-    return p;
+    return plan_for(ctx, c, tokens, num_q_heads / c->heads, top * c->block_size);
 }
 
 template <bool SELECTED>
@@ -718,12 +1211,16 @@ pg_status launch_rows(pg_ctx *ctx, const char *fn, const pg_paged_kv4 *c, kv4_at
     if (p.tiles * p.splits >= (1u << 24)) return pg_fail(PG_EUNSUPPORTED, "%s: %zu row tiles in %zu runs are more than a launch takes", fn, p.tiles, p.splits);
     A.splits = (int)p.splits;
     A.row_tiles = (int)p.row_tiles;
+    const dim3 grid((unsigned)(p.tiles * p.splits)), join((unsigned)(p.tiles * p.rows / 4)), block(256);
     return with_width(c->D, [&](auto w) -> pg_status {
         constexpr int D = decltype(w)::value;
-        PG_TRY(pg_launch(ctx, SELECTED ? "kv4_selected_kernel" : "kv4_rows_kernel", A.cap > 0.f ? kv4_rows_kernel<D, true, SELECTED> : kv4_rows_kernel<D, false, SELECTED>,
-                         dim3((unsigned)(p.tiles * p.splits)), dim3(256), 0, A));
-        if (p.splits == 1) return PG_OK;
-        return pg_launch(ctx, "kv4_join_kernel", kv4_join_kernel<D, SELECTED>, dim3((unsigned)(p.tiles * 4)), dim3(256), 0, A);
+        auto go = [&](const char *name, auto plain, auto capped, auto joined) -> pg_status {
+            PG_TRY(pg_launch(ctx, name, A.cap > 0.f ? capped : plain, grid, block, 0, A));
+            return p.splits == 1 ? PG_OK : pg_launch(ctx, "kv4_join_kernel", joined, join, block, 0, A);
+        };
+        if (p.rows == 4) return go(SELECTED ? "kv4_few_selected_kernel" : "kv4_few_kernel", kv4_few_kernel<D, 4, false, SELECTED>, kv4_few_kernel<D, 4, true, SELECTED>, kv4_join_kernel<D, 4, SELECTED>);
+        if (p.rows == 8) return go(SELECTED ? "kv4_few_selected_kernel" : "kv4_few_kernel", kv4_few_kernel<D, 8, false, SELECTED>, kv4_few_kernel<D, 8, true, SELECTED>, kv4_join_kernel<D, 8, SELECTED>);
+        return go(SELECTED ? "kv4_rows_selected_kernel" : "kv4_rows_kernel", kv4_rows_kernel<D, false, SELECTED>, kv4_rows_kernel<D, true, SELECTED>, kv4_join_kernel<D, 16, SELECTED>);
     });
 }
 
