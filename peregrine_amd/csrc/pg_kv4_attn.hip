@@ -172,6 +172,15 @@ __device__ __forceinline__ void load_tile(const uint8_t *const (&rec)[2], const 
     }
 }
 
+// Lets products of the matrix cores end before anything reads them.  Straight code needs none of it, but where a branch stands between
+// a product and its first reader the compiler counts the wait along one of the two ways only, and the hardware does not count.
+__device__ __forceinline__ void settle(i32x4 &a, i32x4 &b) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void settle_all() {  // ahead of accumulators that are read behind a loop
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // The running softmax of a wavefront's 16 rows: O^T in the accumulators (this lane's row, channels of D / 4 in a run).
 template <int D>
 struct softmax_rows {
@@ -215,6 +224,7 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
         for (int i = 0; i < 4; ++i) hi[i] = (hi[i] << 8) + q.sum_hi1;  // |hi| < 2^26: 256 channels of 15 x 128 x 256 at most
 #pragma unroll
         for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[1][j], hi, 0, 0, 0);
+        if (MASKED) settle(hi, lo);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float x = fmaf((float)hi[i], 256.f, (float)lo[i]);
@@ -226,7 +236,7 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
             float z = kv4_z(vm), e = kv4_d(vm);
             if (MASKED) {
                 const int key = t.pos[r] + 4 * g + i, far = rv.pos - key;
-                const bool seen = far >= 0 && (rv.window < 0 || far <= rv.window || key < rv.sinks);
+                const bool seen = (far >= 0) & ((rv.window < 0) | (far <= rv.window) | (key < rv.sinks));  // (no branch)
                 y = seen ? y : -INFINITY;
                 z = seen ? z : 0.f;  // what is masked may be anything
                 e = seen ? e : 0.f;
@@ -437,6 +447,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_rows_kernel(kv4_att
         if (tile < end) fetch(tile, t);
     }
 
+    settle_all();
     // Four wavefronts' sums into one.
     a.l = over_groups(a.l);
     a.zsum = over_groups(a.zsum);
@@ -594,6 +605,10 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
             for (int s = 0; s < SETS; ++s) acc[s][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.digit[s][j], k8, acc[s][u], 0, 0, 0);
         }
     }
+    if (MASKED) {
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) settle(acc[s][0], acc[s][1]), settle(acc[s][2], acc[s][3]);
+    }
     float s[NT][4], dv[NT], zv[NT];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -628,7 +643,7 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
             if (MASKED) {
                 const int run = HB == 4 ? (g == 0 ? t.pos[0] : g == 1 ? t.pos[1] : g == 2 ? t.pos[2] : t.pos[3]) : (g < 2 ? t.pos[2 * p] : t.pos[2 * p + 1]);
                 const int key = run + c, far = row_pos[i] - key;
-                const bool seen = far >= 0 && (window < 0 || far <= window || key < sinks);
+                const bool seen = (far >= 0) & ((window < 0) | (far <= window) | (key < sinks));  // (no branch)
                 y = seen ? y : -INFINITY;
                 any |= seen;
             }
@@ -894,6 +909,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_few_kernel(kv4_attn
         if (tile < end) fetch(tile, t);
     }
 
+    settle_all();
     // Four wavefronts' sums, and each column's two halves, into one.
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -941,11 +957,369 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_few_kernel(kv4_attn
     }
     const int most = A.splits > 1 ? D : A.c.head_dim;
 #pragma unroll
-    for (int d = part; d < D; d += TPR) {
+    for (int i = 0; i < D / TPR; ++i) {
+        const int d = part + TPR * i;
         float v = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v += w[j] == 0.f ? 0.f : w[j] * fmaf(so[j][row][d] + so[j][HB + row][d], sback[j], sz[j][row]);
         if (d < most) out[d] = v * by;
+    }
+}
+
+// ---- prompts --------------------------------------------------------------------------------
+// With many rows the keys' and values' way from codes to operands is what 16 rows at a time would pay for again and again.
+// Here a workgroup has NW wavefronts of RT tiles of 16 rows and makes the operands of 64 tokens once, in LDS, in the order in
+// which the lanes take them; the next 64 tokens' codes are on their way meanwhile, and the two buffers take turns, one
+// barrier a tile.  Scores and probabilities as in kv4_rows_kernel.  What bounds it is the arithmetic on scores: about 17
+// instructions for each of 16 x 64 beside 56 products of the matrix cores.
+template <int D>
+struct prompt_lds {
+    static constexpr int K = 64 * D, V = 128 * D;  // bytes of a tile's operands
+    alignas(16) uint8_t k[2][K];
+    alignas(16) uint8_t v[2][V];
+    alignas(16) float meta[2][4][64];  // key step, key z + d / 2, value step, value z
+};
+
+template <int D, int RT, int NW, bool CAP>
+__global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
+    static_assert(NW == 4 || NW == 8, "keys are staged by four wavefronts, values by the same or the other four");
+    using R = kv4_rec<D>;
+    constexpr int NJ = D / 64, NV = D / 16, NC = D == 256 ? 2 : 1, KW = D == 64 ? 2 : 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+    auto &lds = *reinterpret_cast<prompt_lds<D> *>(lds_raw);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    // The heads next to each other: workgroups go to the XCDs in turn, and a head's rows share its keys in one L2.  The last rows,
+    // which see the most keys, first.
+    unsigned id = blockIdx.x;
+    const int head = id % A.c.heads;
+    id /= A.c.heads;
+    const int split = id % A.splits;
+    id /= A.splits;
+    const int groups = (A.row_tiles + NW * RT - 1) / (NW * RT);
+    const int group = groups - 1 - id % groups;
+    const int b = id / groups;
+    const int shift = A.c.shift, bs = 1 << shift;
+    const kv4_request rq = kv4_request_at(A.ba, b, shift);
+    const int rows = min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group;
+    const int r0 = group * 16 * NW * RT;
+    if (r0 >= rows) return;
+    const int behind = rq.len - rq.rows;
+    auto pos_of = [&](int r) { return A.mask == PG_MASK_NONE ? rq.len - 1 : behind + r / A.group; };
+    const int mine = r0 + wave * 16 * RT;  // this wavefront's first row
+    const int last_row = min(r0 + 16 * NW * RT, rows) - 1, my_last = min(mine + 16 * RT, rows) - 1;
+    const int group_low = pos_of(r0), group_high = pos_of(last_row);
+    const int low_pos = pos_of(min(mine, last_row)), high_pos = mine < rows ? pos_of(my_last) : -1;
+    const bool windowed = A.mask == PG_MASK_CAUSAL_SLIDING_WINDOW;
+    const int window = windowed ? A.window : -1;
+    const int to = max(group_high + 1, 0), from = windowed ? (int)max((long)group_low - A.window, 0l) : 0;
+    const int near = from >> 6, sink_tiles = windowed ? min((int)(((long)A.sinks + 63) >> 6), near) : 0;
+    const int tiles = to > 0 ? sink_tiles + ((to + 63) >> 6) - near : 0;
+    const int per = (tiles + A.splits - 1) / A.splits, begin = split * per, end = min(begin + per, tiles);
+
+    // A tile's codes on their way to LDS: a thread has one token's chunk of keys (4 threads a token), and words of values
+    // for one half of the tile and one half of each word's channels.
+    struct {
+        uint32_t k[NC][KW], v[8][NC], km, vm;
+    } st;
+    const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
+    auto first_of = [&](int tile) { return 64 * (tile < sink_tiles ? tile : tile - sink_tiles + near); };
+    auto rec_of = [&](int run, int tile, int &at) {  // record and place of a run of 16 tokens (some block where there is none)
+        const int p = first_of(tile) + 16 * run;
+        int phys = p <= group_high ? table[p >> shift] : -1;
+        at = p & (bs - 1);
+        if ((unsigned)phys >= (unsigned)A.c.num_blocks) phys = 0;
+        return A.c.data + ((size_t)phys * A.c.heads + head) * R::bytes(shift);
+    };
+    const int k_token = tid >> 2, k_chunk = tid & 3, v_half = wave & 1, v_part = wave >> 1 & 1;
+    const bool does_k = NW == 4 || wave < 4, does_v = NW == 4 || wave >= 4;
+    auto fetch = [&](int tile) {
+        if (does_k) {
+        int at;
+        // (the wavefront's keys are one run: tokens 16 wave .. 16 wave + 15)
+        const uint8_t *rec = rec_of(wave, tile, at);
+        const uint8_t *kp = rec + (size_t)(at + (k_token & 15)) * R::ROW + k_chunk * (D == 64 ? 8 : 16);
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc) {
+            if (D == 64) {
+                const uint2 x = *reinterpret_cast<const uint2 *>(kp);
+                st.k[cc][0] = x.x, st.k[cc][1] = x.y;
+            } else {
+                const uint4 x = *reinterpret_cast<const uint4 *>(kp + 64 * cc);
+                st.k[cc][0] = x.x, st.k[cc][1] = x.y, st.k[cc][KW - 2] = x.z, st.k[cc][KW - 1] = x.w;
+            }
+        }
+        if (lane < 16) {
+            st.km = reinterpret_cast<const uint32_t *>(rec + R::k_meta(shift))[at + lane];
+            st.vm = reinterpret_cast<const uint32_t *>(rec + R::v_meta(shift))[at + lane];
+        }
+        }
+        if (does_v)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            int va;
+            const uint8_t *vp = rec_of(2 * v_half + r, tile, va);
+            vp += R::v(shift) + (size_t)(va + 4 * g) * R::ROW + (D == 64 ? c >> 1 : c) * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int cc = 0; cc < NC; ++cc) st.v[4 * r + i][cc] = *reinterpret_cast<const uint32_t *>(vp + i * R::ROW + 64 * cc);
+        }
+    };
+    auto store = [&](int buf) {
+        // keys: product j of a run, lanes (chunk, token) in the order of the operand
+        if (does_k) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const uint32_t x = st.k[j >> 1][2 * (j & 1)], y = st.k[j >> 1][2 * (j & 1) + 1];
+            *reinterpret_cast<i32x4 *>(&lds.k[buf][((wave * NJ + j) * 64 + 16 * k_chunk + (k_token & 15)) * 16]) =
+                i32x4{(int)(x & 0x0f0f0f0fu), (int)(x >> 4 & 0x0f0f0f0fu), (int)(y & 0x0f0f0f0fu), (int)(y >> 4 & 0x0f0f0f0fu)};
+        }
+        if (lane < 16) {
+            const float d = kv4_d(st.km);
+            lds.meta[buf][0][16 * wave + lane] = d;
+            lds.meta[buf][1][16 * wave + lane] = fmaf(0.5f, d, kv4_z(st.km));
+            lds.meta[buf][2][16 * wave + lane] = kv4_d(st.vm);
+            lds.meta[buf][3][16 * wave + lane] = kv4_z(st.vm);
+        }
+        }
+        if (!does_v) return;
+        const f16x2 low_by = {(_Float16)32768.f, (_Float16)32768.f}, high_by = {(_Float16)2048.f, (_Float16)2048.f};
+        const f16x2 centre = {(_Float16)(-7.5f * CODE), (_Float16)(-7.5f * CODE)};
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc)
+#pragma unroll
+            for (int q = 0; q < (D == 64 ? 1 : 2); ++q) {
+                const int b2 = (D == 64 ? 1 : 2) * v_part + q;
+                uint32_t sel = 0x0c040c00u + 0x00010001u * b2;
+                if (D == 64) sel += (lane & 1) ? 0x00020002u : 0u;
+                f16x8 even, odd;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const uint32_t x = __builtin_amdgcn_perm(st.v[2 * h + 1][cc], st.v[2 * h][cc], sel);
+                    const f16x2 e = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x000f000fu), low_by, centre);
+                    const f16x2 o = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x00f000f0u), high_by, centre);
+                    even[2 * h] = e[0], even[2 * h + 1] = e[1];
+                    odd[2 * h] = o[0], odd[2 * h + 1] = o[1];
+                }
+                const int n = (D == 64 ? 0 : 8 * cc) + 2 * b2;
+                *reinterpret_cast<f16x8 *>(&lds.v[buf][((v_half * NV + n) * 64 + lane) * 16]) = even;
+                *reinterpret_cast<f16x8 *>(&lds.v[buf][((v_half * NV + n + 1) * 64 + lane) * 16]) = odd;
+            }
+    };
+    if (begin < end) fetch(begin);
+
+    q_rows<D> q[RT];
+    float c1[RT], sq[RT];
+    int row_pos[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int r = mine + 16 * t + c;
+        const bool live = r < rows;
+        load_q<D>(live ? A.q + (size_t)(rq.first + r / A.group) * A.q_token + (size_t)(head * A.group + r % A.group) * A.q_head : nullptr, A.c.head_dim, g, q[t]);
+        c1[t] = q[t].unit * A.scale * (CAP ? 1.f : LOG2E);
+        sq[t] = q[t].sum * c1[t];
+        row_pos[t] = live ? pos_of(r) : -1;
+    }
+    const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
+    f32x4 o[RT][NV];
+    float m[RT], l[RT], zsum[RT], step = 0.f, norm = 0.f;
+    bool set[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m[t] = l[t] = zsum[t] = 0.f;
+        set[t] = false;
+    }
+
+    auto take = [&](auto masked_, const int (&run_pos)[4], int buf) {
+        constexpr bool MASKED = decltype(masked_)::value;
+#pragma unroll 1
+        for (int w = 0; w < 2; ++w) {
+            float s[RT][8], dv[8], zv[8];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int run = 2 * w + r;
+                const int key0 = run_pos[run] + 4 * g;
+                i32x4 k8[NJ];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) k8[j] = *reinterpret_cast<const i32x4 *>(&lds.k[buf][((run * NJ + j) * 64 + lane) * 16]);
+                const f32x4 kd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][0][16 * run + 4 * g]), kw = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][1][16 * run + 4 * g]);
+                const f32x4 vd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][2][16 * run + 4 * g]), vz = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][3][16 * run + 4 * g]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    i32x4 hi = {q[t].sum_hi2, q[t].sum_hi2, q[t].sum_hi2, q[t].sum_hi2}, lo = {q[t].sum_lo, q[t].sum_lo, q[t].sum_lo, q[t].sum_lo};
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q[t].digit[2][j], hi, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q[t].digit[0][j], lo, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) hi[i] = (hi[i] << 8) + q[t].sum_hi1;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q[t].digit[1][j], hi, 0, 0, 0);
+                    if (MASKED) settle(hi, lo);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = fmaf((float)hi[i], 256.f, (float)lo[i]);
+                        float y;
+                        if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(kd[i] * c1[t], x, kw[i] * sq[t]) * inv_cap), -m[t]);
+                        else y = fmaf(kd[i] * c1[t], x, fmaf(kw[i], sq[t], -m[t]));
+                        if (MASKED) {
+                            const int key = key0 + i, far = row_pos[t] - key;
+                            y = (far >= 0) & ((window < 0) | (far <= window) | (key < A.sinks)) ? y : -INFINITY;  // (no branch)
+                        }
+                        s[t][4 * r + i] = y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dv[4 * r + i] = vd[i], zv[4 * r + i] = vz[i];
+            }
+            if (MASKED) {
+                // What lies behind the rows' last position, or in no block, may be anything, and so may masked tokens: their
+                // probabilities are 0 below whatever they are multiplied by.
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    bool any = false;
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) any |= s[t][i] != -INFINITY;
+                    dv[i] = any ? dv[i] : 0.f;
+                    zv[i] = any ? zv[i] : 0.f;
+                }
+            }
+            float p[RT][8], pd[RT][8], sum[RT];
+            uint32_t top;
+            auto weigh = [&] {
+                top = 0;
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    sum[t] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        p[t][i] = __builtin_amdgcn_exp2f(s[t][i]);
+                        sum[t] += p[t][i];
+                        pd[t][i] = p[t][i] * (dv[i] * norm);
+                        if (MASKED) pd[t][i] = s[t][i] == -INFINITY ? 0.f : pd[t][i];
+                        top = max(top, __builtin_bit_cast(uint32_t, pd[t][i]));
+                    }
+                }
+            };
+            weigh();
+            uint32_t steps = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) steps = max(steps, __builtin_bit_cast(uint32_t, dv[i]));
+            bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || steps > __builtin_bit_cast(uint32_t, step);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) off |= !set[t] || !(sum[t] < 1.2676506e30f);
+            if (__ballot(off)) {
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = fmaxf(most, dv[i]);
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+                float fs = 1.f;
+                if (most > step) {
+                    const float next = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+                    fs = step / next;
+                    step = next;
+                    norm = P_TOP / next;
+                }
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    float at = s[t][0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) at = fmaxf(at, s[t][i]);
+                    at = max_groups(at);
+                    float f = 1.f;
+                    if (at > -INFINITY && (!set[t] || at > 0.f)) {
+                        f = set[t] ? __builtin_amdgcn_exp2f(-at) : 1.f;
+                        m[t] += at;
+                        set[t] = true;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) s[t][i] -= at;
+                    }
+                    l[t] *= f;
+                    zsum[t] *= f;
+                    f *= fs;
+#pragma unroll
+                    for (int n = 0; n < NV; ++n) o[t][n] *= f;
+                }
+                weigh();
+            }
+            f16x8 ph[RT], pl[RT];
+            float minus = -1.f;
+            asm("" : "+s"(minus));  // (not a subtraction, so that one instruction takes the f16 as it is)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                l[t] += sum[t];
+                float zs = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    zs = MASKED && s[t][i] == -INFINITY ? zs : fmaf(p[t][i], zv[i], zs);
+                    ph[t][i] = (_Float16)pd[t][i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pl[t][i] = (_Float16)fmaf((float)ph[t][i], minus, pd[t][i]);
+                zsum[t] += zs;
+            }
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const f16x8 v = *reinterpret_cast<const f16x8 *>(&lds.v[buf][((w * NV + n) * 64 + lane) * 16]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o[t][n], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[t], o[t][n], 0, 0, 0);
+            }
+        }
+    };
+    if (begin < end) store(0);
+    __syncthreads();
+    for (int tile = begin; tile < end; ++tile) {
+        const int buf = (tile - begin) & 1, first = first_of(tile);
+        if (tile + 1 < end) fetch(tile + 1);
+        if (first <= high_pos) {
+            int run_pos[4];  // of each run's first token, beyond every row where the run lies in no block
+            bool there = true;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int p = first + 16 * r;
+                const bool ok = (p <= group_high) & ((unsigned)table[min(p, group_high) >> shift] < (unsigned)A.c.num_blocks);
+                run_pos[r] = ok ? p : 0x7fffff00;
+                there &= ok;
+            }
+            if (there && first + 63 <= low_pos && (!windowed || high_pos - first <= window)) take(std::false_type{}, run_pos, buf);
+            else take(std::true_type{}, run_pos, buf);
+        }
+        if (tile + 1 < end) store(buf ^ 1);
+        __syncthreads();
+    }
+
+    settle_all();
+    const float back = step * (1.f / (P_TOP * CODE));
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int r = mine + 16 * t + c;
+        const float ls = over_groups(l[t]), zs = over_groups(zsum[t]);
+        if (r >= rows) continue;
+        float *out;
+        float by = 1.f;
+        if (A.splits > 1) {
+            const size_t tile = ((size_t)b * A.c.heads + head) * A.row_tiles + r / 16;
+            float *base = A.part + (tile * A.splits + split) * (16 * D + 32);
+            out = base + c * D;
+            if (g == 0) base[16 * D + c] = set[t] ? m[t] : ls == 0.f ? -INFINITY : 0.f, base[16 * D + 16 + c] = ls;
+        } else {
+            out = A.out + ((size_t)(rq.first + r / A.group) * A.q_heads + head * A.group + r % A.group) * A.c.head_dim;
+            by = ls == 0.f ? 0.f : 1.f / ls;
+        }
+        const int most = A.splits > 1 ? D : A.c.head_dim;
+        constexpr int RUN = D / 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const int d = D == 256 ? 128 * (n >> 3) + 32 * g + 8 * i + (n & 7) : RUN * g + (D / 16) * i + n;
+                if (d < most) out[d] = fmaf(o[t][n][i], back, zs) * by;
+            }
     }
 }
 
@@ -985,14 +1359,26 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(kv4_attn A) {
         for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d);
         l += mine;
         const float *rows_at = part + s0 * NEXT + row * D + lane;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) {
+        auto add = [&](int j, const float (&x)[D / 64]) {
             const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) {
-                const float x = rows_at[j * NEXT + 64 * i];
-                o[i] += wj == 0.f ? 0.f : wj * x;  // (a run that saw nothing may hold anything)
-            }
+            for (int i = 0; i < D / 64; ++i) o[i] += wj == 0.f ? 0.f : wj * x[i];  // (a run that saw nothing may hold anything)
+        };
+        int j = 0;
+        for (; j + 8 <= n; j += 8) {  // eight splits' rows on their way at once
+            float x[8][D / 64];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) x[u][i] = rows_at[(j + u) * NEXT + 64 * i];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) add(j + u, x[u]);
+        }
+        for (; j < n; ++j) {
+            float x[D / 64];
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) x[i] = rows_at[j * NEXT + 64 * i];
+            add(j, x);
         }
     }
     const float by = l == 0.f ? 0.f : 1.f / l;
@@ -1189,13 +1575,18 @@ size_t pick_splits(const pg_ctx *ctx, int D, size_t tiles, size_t tokens) {
 
 struct plan {
     size_t rows, row_tiles, tiles, splits, bytes;  // rows a tile (4, 8 or 16)
+    size_t wide;                                   // row tiles a workgroup of kv4_prompt_kernel, or 0: the other kernels
 };
+constexpr int PROMPT_RT = 1, PROMPT_NW = 8;
+constexpr size_t PROMPT_TILES = 4;
 plan plan_for(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t units, size_t unit_rows, size_t tokens) {
     plan p;
     p.rows = unit_rows <= 4 ? 4 : unit_rows <= 8 ? 8 : 16;
     p.row_tiles = (unit_rows + p.rows - 1) / p.rows;
     p.tiles = units * c->heads * p.row_tiles;
-    p.splits = pick_splits(ctx, c->D, p.tiles, tokens);
+    p.wide = p.row_tiles < PROMPT_TILES ? 0 : PROMPT_RT * PROMPT_NW;
+    const size_t workgroups = p.wide ? units * c->heads * ((p.row_tiles + p.wide - 1) / p.wide) : p.tiles;
+    p.splits = pick_splits(ctx, c->D, workgroups, tokens);
     p.bytes = p.splits > 1 ? p.tiles * p.splits * (p.rows * (size_t)c->D + 32) * sizeof(float) : 0;
     return p;
 }
@@ -1218,6 +1609,15 @@ pg_status launch_rows(pg_ctx *ctx, const char *fn, const pg_paged_kv4 *c, kv4_at
             PG_TRY(pg_launch(ctx, name, A.cap > 0.f ? capped : plain, grid, block, 0, A));
             return p.splits == 1 ? PG_OK : pg_launch(ctx, "kv4_join_kernel", joined, join, block, 0, A);
         };
+        if constexpr (!SELECTED)
+            if (p.wide) {
+                auto kernel = A.cap > 0.f ? kv4_prompt_kernel<D, PROMPT_RT, PROMPT_NW, true> : kv4_prompt_kernel<D, PROMPT_RT, PROMPT_NW, false>;
+                constexpr size_t lds = sizeof(prompt_lds<D>);
+                if (lds > (48u << 10)) PG_TRY(pg_allow_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds));
+                const size_t groups = (p.row_tiles + p.wide - 1) / p.wide;
+                PG_TRY(pg_launch(ctx, "kv4_prompt_kernel", kernel, dim3((unsigned)(A.ba.batch * c->heads * groups * p.splits)), dim3(64 * PROMPT_NW), lds, A));
+                return p.splits == 1 ? PG_OK : pg_launch(ctx, "kv4_join_kernel", kv4_join_kernel<D, 16, SELECTED>, join, block, 0, A);
+            }
         if (p.rows == 4) return go(SELECTED ? "kv4_few_selected_kernel" : "kv4_few_kernel", kv4_few_kernel<D, 4, false, SELECTED>, kv4_few_kernel<D, 4, true, SELECTED>, kv4_join_kernel<D, 4, SELECTED>);
         if (p.rows == 8) return go(SELECTED ? "kv4_few_selected_kernel" : "kv4_few_kernel", kv4_few_kernel<D, 8, false, SELECTED>, kv4_few_kernel<D, 8, true, SELECTED>, kv4_join_kernel<D, 8, SELECTED>);
         return go(SELECTED ? "kv4_rows_selected_kernel" : "kv4_rows_kernel", kv4_rows_kernel<D, false, SELECTED>, kv4_rows_kernel<D, true, SELECTED>, kv4_join_kernel<D, 16, SELECTED>);

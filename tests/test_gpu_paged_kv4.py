@@ -659,3 +659,25 @@ def test_a_cache_may_outlive_the_work_of_its_context(ctx):
         k, _ = c.read([0, 3])
         assert (k[0] == 1).all() and (k[1] == 2).all()
         c.free()
+
+
+@pytest.mark.parametrize("hd,heads,group,bs,lens,rows", [(128, 2, 4, 64, [700, 90], [300, 90]), (64, 1, 7, 16, [200, 33, 400], [200, 2, 101]), (256, 2, 1, 32, [500], [257]), (80, 1, 2, 128, [300], [130])])
+def test_prompts_leave_out_what_is_no_block_and_read_nothing_behind(ctx, hd, heads, group, bs, lens, rows):
+    """Pieces of prompts with every mask, with table entries that are no block in the middle of what they see; NaN rows behind
+    the last token and in every block that is not theirs."""
+    w = World(ctx, lens, heads, hd, bs, seed=hd + 1)
+    q = w.q(sum(rows), heads * group)
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    for m in (dict(), dict(mask=0), dict(mask=2, window=33, sinks=70), dict(mask=2, window=5, sinks=0), dict(cap=3.0)):
+        s = Step(ctx, w, q, starts)
+        s.attention(**m)
+        w.check(s.result(), q, rows, hd ** -0.5, what=str(m), **m)
+    table = w.table.copy()
+    gone = [1, 2] if bs < 64 else [1]
+    table[0, gone[0]], table[0, gone[-1]] = -1, w.nb + 3
+    s = Step(ctx, w, q, starts, table=table)
+    s.attention()
+    got = s.result()
+    one = World.__new__(World)
+    one.__dict__.update(w.__dict__, lens=w.lens[:1], table=w.table[:1])
+    one.check(got[: rows[0]], q[: rows[0]], rows[:1], hd ** -0.5, only=lambda t, h: [j for j in range(w.width) if j not in gone], what="no block")
