@@ -8,96 +8,122 @@ namespace {
 
 // ---- block tables ---------------------------------------------------------------------------
 
-// Sum over the threads below this one in a workgroup of 1024, and over all of them; part: 16 words of LDS.
-__device__ __forceinline__ long below_sum(long v, long *part, long *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    long s = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long u = __shfl_up(s, d);
-        if (lane >= d) s += u;
-    }
-    __syncthreads();
-    if (lane == 63) part[wave] = s;
-    __syncthreads();
-    long below = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        const long p = part[w];
-        below += w < wave ? p : 0;
-        all += p;
-    }
-    *total = all;
-    return below + s - v;
-}
-
 __device__ __forceinline__ int blocks_of(long tokens, int shift) { return (int)((tokens + (1l << shift) - 1) >> shift); }
 
-// One workgroup takes the requests in runs of 1024, a thread a request: needs and rows are prefix sums.  The work is some
-// loads and a few dozen instructions a request: a launch's latency bounds it, so it is one launch wherever the slot map
-// is short enough for one workgroup (slots_here), and the map's own launch over the chip where it is not.
+// Sums over the threads below this one in a workgroup of 1024, and over all of them, of two numbers; part: 32 words of LDS.
+__device__ __forceinline__ void below_sums(long &a, long &b, long *part, long *all_a, long *all_b) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    long s = a, t = b;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long u = __shfl_up(s, d), v = __shfl_up(t, d);
+        if (lane >= d) s += u, t += v;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = s, part[16 + wave] = t;
+    __syncthreads();
+    long below_a = 0, below_b = 0, sum_a = 0, sum_b = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const long p = part[w], q = part[16 + w];
+        below_a += w < wave ? p : 0, below_b += w < wave ? q : 0;
+        sum_a += p, sum_b += q;
+    }
+    *all_a = sum_a, *all_b = sum_b;
+    a = below_a + s - a, b = below_b + t - b;
+}
+
+// The last of n ascending numbers that is at most v (the first is).
+__device__ __forceinline__ int last_upto(const int *at, int n, int v) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (at[mid] <= v) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// The requests in runs of 1024, a thread a request: rows and needs are prefix sums.  Needs are counted whether they are met or
+// not, so those that are met come first: a granted request's new blocks begin at the sum of the needs before it, and new entries
+// and slots are flat lists, a thread a place, the request by bisection in LDS.  A slot in a new block comes from the free list like
+// the entry itself, so nothing waits for what this launch writes.  A few loads behind one another bound it: 256 decoding
+// requests 13.4 us with a wavefront a request for entries and slots, one after the other.
+// Workgroup w does the slots of rows 4096 w .. and on; the first does everything else, and may write lengths and count over their
+// inputs if it is the only one (slots = null: no slots, slot_map_kernel does them).
 __global__ __launch_bounds__(1024) void extend_tables_kernel(const int *seq_lens, const int *new_lens, int batch, int shift, const int *free_list, const int *free_count,
                                                              int num_blocks, int *table, int max_blocks, int *lens_out, int *free_out, int *starts, int *granted,
-                                                             int *slots, int max_tokens, int slots_here) {
-    __shared__ long part[16];
-    __shared__ int first_row[1024], base_pos[1024], old_blocks[1024], first_free[1024], taken[1024];
+                                                             int *slots, int max_tokens) {
+    __shared__ long part[32];
+    __shared__ int first_row[1024], base_pos[1024], old_blocks[1024], first_need[1024];
+    __shared__ uint8_t fine[1024];
+    __shared__ int handed;
     const int have_free = min(max(*free_count, 0), num_blocks), tid = threadIdx.x;
+    const bool all_else = blockIdx.x == 0;
+    const long from_row = (long)blockIdx.x * 4096, to_row = min(from_row + 4096, (long)max_tokens);
     const long most = (long)max_blocks << shift;
-    long rows_before = 0;  // of the runs before this one
-    long needs_before = 0;
-    long handed_out = 0;
+    long rows_before = 0, needs_before = 0;  // of the runs before this one
+    if (tid == 0) handed = 0;
     for (int at = 0; at < batch; at += 1024) {
-        const int b = at + tid;
+        const int b = at + tid, run = min(1024, batch - at);
         const int len = b < batch ? max(seq_lens[b], 0) : 0, add = b < batch ? max(new_lens[b], 0) : 0;
         const bool fits = (long)len + add <= most;
         const int have = blocks_of(len, shift);
         const int need = b < batch && fits ? blocks_of((long)len + add, shift) - have : 0;
-        long rows_all, needs_all, taken_all;
-        const long row = below_sum(add, part, &rows_all), before = below_sum(need, part, &needs_all);
-        const long row0 = rows_before + row, need0 = needs_before + before;
-        const bool ok = b < batch && fits && (need == 0 || need0 + need <= have_free);
-        const int mine = ok ? need : 0;
-        below_sum(mine, part, &taken_all);
-        first_row[tid] = (int)min(row0, (long)max_tokens);
+        long row = add, before = need, rows_all, needs_all;
+        below_sums(row, before, part, &rows_all, &needs_all);
+        row += rows_before, before += needs_before;
+        const bool ok = b < batch && fits && (need == 0 || before + need <= have_free);
+        first_row[tid] = (int)min(row, (long)max_tokens);
         base_pos[tid] = len;
         old_blocks[tid] = have;
-        first_free[tid] = ok ? (int)(have_free - 1 - need0) : 0;
-        taken[tid] = mine;
-        if (b < batch) {
-            starts[b] = (int)min(row0, (long)max_tokens);
+        first_need[tid] = (int)min(before, (long)num_blocks);
+        fine[tid] = ok;
+        if (ok && need) atomicMax(&handed, (int)(before + need));
+        if (all_else && b < batch) {
+            starts[b] = (int)min(row, (long)max_tokens);
             granted[b] = ok;
             lens_out[b] = ok ? len + add : len;
         }
         __syncthreads();
-        // The new entries: a wavefront a request.
-        const int run = min(1024, batch - at);
-        for (int i = tid >> 6; i < run; i += 16)
-            for (int j = tid & 63; j < taken[i]; j += 64)
-                table[(size_t)(at + i) * max_blocks + old_blocks[i] + j] = free_list[first_free[i] - j];
-        __syncthreads();
-        if (slots_here) {
-            for (int i = tid >> 6; i < run; i += 16) {
-                const int from = first_row[i];
-                const int to = i + 1 < run ? first_row[i + 1] : (int)min(rows_before + rows_all, (long)max_tokens);
-                const bool yes = granted[at + i];
-                for (int j = from + (tid & 63); j < to; j += 64) {
-                    const int pos = base_pos[i] + j - from;
-                    slots[j] = yes ? (int)(((unsigned)table[(size_t)(at + i) * max_blocks + (pos >> shift)] << shift) | (pos & ((1 << shift) - 1))) : -1;
+        for (int e = (int)min(needs_before, (long)num_blocks) + 1024 * blockIdx.x + tid; e < handed; e += 1024 * gridDim.x) {
+            const int i = last_upto(first_need, run, e);
+            table[(size_t)(at + i) * max_blocks + old_blocks[i] + e - first_need[i]] = free_list[have_free - 1 - e];
+        }
+        if (slots) {
+            const int upto = (int)min(min(rows_before + rows_all, (long)max_tokens), to_row);
+            const int from = (int)max(min(rows_before, (long)max_tokens), from_row);
+            int pos[4], phys[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {  // a thread's four places' loads go out together
+                const int j = from + tid + 1024 * u;
+                pos[u] = -1, phys[u] = 0;
+                if (j < upto) {
+                    const int i = last_upto(first_row, run, j), p = base_pos[i] + j - first_row[i], block = p >> shift;
+                    if (fine[i]) {
+                        const int *from_list = free_list + (have_free - 1 - (first_need[i] + block - old_blocks[i]));
+                        phys[u] = *(block < old_blocks[i] ? table + (size_t)(at + i) * max_blocks + block : from_list);
+                        pos[u] = p;
+                    }
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = from + tid + 1024 * u;
+                if (j < upto) slots[j] = pos[u] < 0 ? -1 : (int)(((unsigned)phys[u] << shift) | (pos[u] & ((1 << shift) - 1)));
             }
         }
         rows_before += rows_all;
         needs_before += needs_all;
-        handed_out += taken_all;
         __syncthreads();
     }
     const int rows = (int)min(rows_before, (long)max_tokens);
-    if (tid == 0) {
+    if (all_else && tid == 0) {
         starts[batch] = rows;
-        *free_out = have_free - (int)handed_out;
+        *free_out = have_free - handed;
     }
-    if (slots_here)
-        for (int j = rows + tid; j < max_tokens; j += 1024) slots[j] = -1;
+    if (slots)
+        for (int j = max(rows, (int)from_row) + tid; j < to_row; j += 1024) slots[j] = -1;
 }
 
 // The slot map over the chip: a thread a row, its request by bisection.
@@ -124,7 +150,7 @@ __global__ __launch_bounds__(256) void slot_map_kernel(const int *__restrict__ s
 // Blocks of flagged requests back to the free list, requests and their blocks in ascending order.
 __global__ __launch_bounds__(1024) void release_tables_kernel(const int *release, int *seq_lens, int batch, int shift, int *table, int max_blocks, int *free_list,
                                                               int *free_count, int num_blocks) {
-    __shared__ long part[16];
+    __shared__ long part[32];
     __shared__ int valid[1024], first[1024];
     const int tid = threadIdx.x, lane = tid & 63;
     int top = min(max(*free_count, 0), num_blocks);
@@ -142,8 +168,9 @@ __global__ __launch_bounds__(1024) void release_tables_kernel(const int *release
             if (lane == 0) valid[i] = n;
         }
         __syncthreads();
-        long all;
-        first[tid] = (int)below_sum(tid < run ? valid[tid] : 0, part, &all);
+        long all, mine = tid < run ? valid[tid] : 0, none = 0, no_sum;
+        below_sums(mine, none, part, &all, &no_sum);
+        first[tid] = (int)mine;
         __syncthreads();
         for (int i = tid >> 6; i < run; i += 16)
             if (release[at + i]) {
@@ -169,77 +196,91 @@ __global__ __launch_bounds__(1024) void release_tables_kernel(const int *release
 
 // ---- rows -----------------------------------------------------------------------------------
 
-// v over the L lanes of a row (L a power of two), in each of them.
+// v over the L lanes of a row (8, 16 or 32), in each of them: DPP moves within 16 lanes, a swap of half rows across.
 template <int L, class F>
-__device__ __forceinline__ float row_all(float v, F f) {
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) v = f(v, __shfl_xor(v, d));
+__device__ __forceinline__ uint32_t row_all(uint32_t v, F f) {
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // quad_perm [1,0,3,2]
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));   // quad_perm [2,3,0,1]
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));  // row_half_mirror
+    if (L >= 16) v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));  // row_mirror
+    if (L >= 32) v = f(v, (uint32_t)__shfl_xor((int)v, 16));
     return v;
 }
+struct row_min {
+    __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return __builtin_bit_cast(uint32_t, fminf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b))); }
+};
+struct row_max {
+    __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b))); }
+};
 
-// Eight channels of a row a lane, D / 8 lanes a row: a wavefront takes 512 / D rows, keys and values of a head in turn.
-// Bound by memory: a row's 4 D bytes in, D / 2 + 4 out.
+// Eight channels of a row a lane, D / 8 lanes a row, TWO rows a lane half the launch apart: both rows' loads are on their way before
+// anything is known of their slots.  Bound by memory: a row's 4 D bytes in, D / 2 + 4 out.
 template <int D, bool WIDE>
 __global__ __launch_bounds__(256) void kv4_append_kernel(const float *__restrict__ k, const float *__restrict__ v, kv4_view c, size_t token_stride, size_t head_stride,
                                                          int tokens, const int *__restrict__ slots) {
     using R = kv4_rec<D>;
-    constexpr int L = D / 8;
-    const int lane = threadIdx.x & (L - 1);
-    const size_t row = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    const int side = row & 1;
-    const size_t th = row >> 1;
-    const int head = (int)(th % c.heads);
-    const size_t token = th / c.heads;
-    const int slot = token < (size_t)tokens ? slots[token] : -1;
-    const bool live = slot >= 0 && (slot >> c.shift) < c.num_blocks;  // (every lane stays for the shuffles)
-    const float *x = (side ? v : k) + (live ? token : 0) * token_stride + head * head_stride;
-    float a[8];
-    const int i0 = lane * 8;
-    if (WIDE) {
+    constexpr int L = D / 8, TWO = 2;
+    const int lane = threadIdx.x & (L - 1), i0 = lane * 8;
+    float a[TWO][8];
+    int slot[TWO], head[TWO], side[TWO];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (live && i0 + 4 * h < c.head_dim) f = *reinterpret_cast<const float4 *>(x + i0 + 4 * h);
-            a[4 * h] = f.x, a[4 * h + 1] = f.y, a[4 * h + 2] = f.z, a[4 * h + 3] = f.w;
+    for (int u = 0; u < TWO; ++u) {
+        const unsigned row = (blockIdx.x * TWO + u) * (256 / L) + threadIdx.x / L;  // (a launch has under 2^31 of them)
+        side[u] = row & 1;
+        const unsigned th = row >> 1, token = th / (unsigned)c.heads;
+        head[u] = (int)(th % (unsigned)c.heads);
+        const bool there = token < (unsigned)tokens;  // (every lane stays for its row's sums)
+        slot[u] = there ? slots[token] : -1;
+        const float *x = (side[u] ? v : k) + (size_t)(there ? token : 0) * token_stride + head[u] * head_stride;
+        if (WIDE) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i0 + 4 * h < c.head_dim) f = *reinterpret_cast<const float4 *>(x + i0 + 4 * h);
+                a[u][4 * h] = f.x, a[u][4 * h + 1] = f.y, a[u][4 * h + 2] = f.z, a[u][4 * h + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[u][i] = i0 + i < c.head_dim ? x[i0 + i] : 0.f;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = live && i0 + i < c.head_dim ? x[i0 + i] : 0.f;
     }
-    float lo = INFINITY, hi = -INFINITY;
-    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i0 + i < c.head_dim) {
-            lo = fminf(lo, a[i]);
-            hi = fmaxf(hi, a[i]);
-            bad |= !(fabsf(a[i]) <= 3.402823466e38f);
+    for (int u = 0; u < TWO; ++u) {
+        float lo = INFINITY, hi = -INFINITY;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i0 + i < c.head_dim) {
+                lo = fminf(lo, a[u][i]);
+                hi = fmaxf(hi, a[u][i]);
+                top = max(top, __builtin_bit_cast(uint32_t, a[u][i]) & 0x7fffffffu);  // (of magnitudes the bits are in order, NaN last)
+            }
+        lo = __builtin_bit_cast(float, row_all<L>(__builtin_bit_cast(uint32_t, lo), row_min{}));
+        hi = __builtin_bit_cast(float, row_all<L>(__builtin_bit_cast(uint32_t, hi), row_max{}));
+        top = row_all<L>(top, [](uint32_t p, uint32_t q) { return max(p, q); });
+        uint32_t zb = __builtin_bit_cast(uint32_t, 0.5f * lo + 0.5f * hi);
+        zb = (zb + 0x7fffu + ((zb >> 16) & 1)) & 0xffff0000u;  // to bfloat16, to nearest even
+        const float z = __builtin_bit_cast(float, zb);
+        const float h = fmaxf(hi - z, z - lo);
+        // up to the next bfloat16, so that 7.5 steps reach both ends; not so small that 1 / d is infinite
+        const uint32_t db = (__builtin_bit_cast(uint32_t, h * (1.0f / 7.5f)) + 0xffffu) & 0xffff0000u;
+        const float d = h == 0.f ? 0.f : fmaxf(__builtin_bit_cast(float, db), 7.52316385e-37f);  // 2^-120
+        const float r = h == 0.f ? 0.f : 1.0f / d;
+        const bool bad = top >= 0x7f800000u || !(h <= 3.402823466e38f);
+        uint32_t codes = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float n = fminf(fmaxf(rintf((a[u][i] - z) * r + 7.5f), 0.f), 15.f);
+            codes |= (i0 + i < c.head_dim && !bad ? (uint32_t)n : 0u) << (4 * i);
         }
-    lo = row_all<L>(lo, [](float p, float q) { return fminf(p, q); });
-    hi = row_all<L>(hi, [](float p, float q) { return fmaxf(p, q); });
-    bad = row_all<L>(bad ? 1.f : 0.f, [](float p, float q) { return fmaxf(p, q); }) != 0.f;
-    uint32_t zb = __builtin_bit_cast(uint32_t, 0.5f * lo + 0.5f * hi);
-    zb = (zb + 0x7fffu + ((zb >> 16) & 1)) & 0xffff0000u;  // to bfloat16, to nearest even
-    const float z = __builtin_bit_cast(float, zb);
-    const float h = fmaxf(hi - z, z - lo);
-    // up to the next bfloat16, so that 7.5 steps reach both ends; not so small that 1 / d is infinite
-    const uint32_t db = (__builtin_bit_cast(uint32_t, h * (1.0f / 7.5f)) + 0xffffu) & 0xffff0000u;
-    const float d = h == 0.f ? 0.f : fmaxf(__builtin_bit_cast(float, db), 7.52316385e-37f);  // 2^-120
-    const float r = h == 0.f ? 0.f : 1.0f / d;
-    bad |= !(h <= 3.402823466e38f);
-    uint32_t codes = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float n = fminf(fmaxf(rintf((a[i] - z) * r + 7.5f), 0.f), 15.f);
-        codes |= (i0 + i < c.head_dim && !bad ? (uint32_t)n : 0u) << (4 * i);
+        if (slot[u] < 0 || (slot[u] >> c.shift) >= c.num_blocks) continue;
+        uint8_t *rec = c.data + ((size_t)(slot[u] >> c.shift) * c.heads + head[u]) * R::bytes(c.shift);
+        const int at = slot[u] & ((1 << c.shift) - 1);
+        *reinterpret_cast<uint32_t *>(rec + (side[u] ? R::v(c.shift) : 0) + (size_t)at * R::ROW + lane * 4) = codes;
+        if (lane == 0)
+            reinterpret_cast<uint32_t *>(rec + (side[u] ? R::v_meta(c.shift) : R::k_meta(c.shift)))[at] =
+                bad ? 0x7fc07fc0u : (zb >> 16) | (__builtin_bit_cast(uint32_t, d) & 0xffff0000u);
     }
-    if (!live) return;
-    uint8_t *rec = c.data + ((size_t)(slot >> c.shift) * c.heads + head) * R::bytes(c.shift);
-    const int at = slot & ((1 << c.shift) - 1);
-    *reinterpret_cast<uint32_t *>(rec + (side ? R::v(c.shift) : 0) + (size_t)at * R::ROW + lane * 4) = codes;
-    if (lane == 0)
-        reinterpret_cast<uint32_t *>(rec + (side ? R::v_meta(c.shift) : R::k_meta(c.shift)))[at] =
-            bad ? 0x7fc07fc0u : (zb >> 16) | (__builtin_bit_cast(uint32_t, d) & 0xffff0000u);
 }
 
 // The rows of the named slots as the values they stand for; rows of a slot that is none are 0.
@@ -248,12 +289,11 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const int *__restrict__ s
     using R = kv4_rec<D>;
     constexpr int L = D / 8;
     const int lane = threadIdx.x & (L - 1);
-    const size_t row = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const unsigned row = blockIdx.x * (256 / L) + threadIdx.x / L;  // (a launch has under 2^31 of them)
     const int side = row & 1;
-    const size_t th = row >> 1;
-    const int head = (int)(th % c.heads);
-    const size_t token = th / c.heads;
-    if (token >= (size_t)n) return;
+    const unsigned th = row >> 1, token = th / (unsigned)c.heads;
+    const int head = (int)(th % (unsigned)c.heads);
+    if (token >= (unsigned)n) return;
     const int slot = slots[token];
     const bool live = slot >= 0 && (slot >> c.shift) < c.num_blocks;
     const uint8_t *rec = c.data + ((size_t)(live ? slot >> c.shift : 0) * c.heads + head) * R::bytes(c.shift);
@@ -276,20 +316,24 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const int *__restrict__ s
     }
 }
 
-// The summaries of the blocks that a step's rows end in or fill: a wavefront a (row, head); rows that neither fill their
-// block nor are their request's last have nothing to do.  A block's least and most are order-independent, so a block that
-// two requests share gets the same bits from both.
+// The summaries of the blocks that a step's rows lie in: a wavefront an (item, head).  Request b has the items from (its first row
+// >> shift) + 2 b on -- its r rows lie in at most (r >> shift) + 2 blocks, so no two requests share one -- and those without a block
+// have nothing to do.  A block's least and most are order-independent, so a block that two requests share gets the same bits from both.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_summarise_kernel(kv4_batch ba, kv4_view c) {
     using R = kv4_rec<D>;
     constexpr int L = D / 8, G = 64 / L;  // lanes a row, rows at a time
-    const int t = blockIdx.x, lane = threadIdx.x & (L - 1), group = (threadIdx.x & 63) / L;
-    const int b = kv4_request_of(ba.starts, ba.batch, t);
+    const int item = blockIdx.x, lane = threadIdx.x & (L - 1), group = (threadIdx.x & 63) / L;
+    int upto = 0;
+    for (int i = threadIdx.x & 63; i - (int)(threadIdx.x & 63) < ba.batch; i += 64)
+        upto += __popcll(__ballot(i < ba.batch && (long)(ba.starts[min(i, ba.batch - 1)] >> c.shift) + 2 * i <= item));
+    const int b = upto - 1;
     if (b < 0) return;
     const kv4_request rq = kv4_request_at(ba, b, c.shift);
-    const int pos = rq.len - rq.rows + (t - rq.first), bs = 1 << c.shift;
-    if ((unsigned)(t - rq.first) >= (unsigned)rq.rows || pos < 0 || pos >= rq.len || ((pos & (bs - 1)) != bs - 1 && t - rq.first != rq.rows - 1)) return;
-    const int phys = ba.table[(size_t)b * ba.max_blocks + (pos >> c.shift)], count = (pos & (bs - 1)) + 1;
+    if (rq.rows == 0) return;
+    const int bs = 1 << c.shift, first = max(rq.len - rq.rows, 0), block = (first >> c.shift) + item - ((rq.first >> c.shift) + 2 * b);
+    if (block < 0 || (long)block << c.shift >= rq.len) return;
+    const int phys = ba.table[(size_t)b * ba.max_blocks + block], count = min(bs, rq.len - (block << c.shift));
     if (phys < 0 || phys >= c.num_blocks) return;
     for (int head = blockIdx.y * 4 + (threadIdx.x >> 6); head < c.heads; head += gridDim.y * 4) {
         const size_t at = (size_t)phys * c.heads + head;
@@ -320,7 +364,8 @@ __global__ __launch_bounds__(256) void kv4_summarise_kernel(kv4_batch ba, kv4_vi
             }
             if (lane * 8 + i < c.head_dim) most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
         }
-        most = row_all<64>(most, [](float p, float q) { return fmaxf(p, q); });
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
         bad = __ballot(bad) != 0;
         const float r = bad || most < 7.88860905e-31f ? 0.f : 1.0f / most * 127.f;  // 2^-100
         uint32_t h4[2] = {0, 0}, l4[2] = {0, 0};
@@ -339,28 +384,28 @@ __global__ __launch_bounds__(256) void kv4_summarise_kernel(kv4_batch ba, kv4_vi
     }
 }
 
-// Least and most of each channel of the named blocks, as their summaries hold them; 0 where the block is none.
+// Least and most of each channel of the named blocks, as their summaries hold them; 0 where the block is none.  A workgroup a block,
+// a wavefront a head at a time.
 template <int D>
-__global__ __launch_bounds__(256) void kv4_read_sums_kernel(const int *__restrict__ blocks, float *__restrict__ lo, kv4_view c, int n, float *__restrict__ hi) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int ch = (int)(i % c.head_dim);
-    const size_t bh = i / c.head_dim, at = bh / c.heads;
-    if (at >= (size_t)n) return;
-    const int phys = blocks[at];
-    float l = 0.f, h = 0.f;
-    if (phys >= 0 && phys < c.num_blocks) {
-        const uint8_t *s = c.sums + ((size_t)phys * c.heads + bh % c.heads) * kv4_rec<D>::SUM;
-        const float scale = *reinterpret_cast<const float *>(s + 2 * D);
-        h = (float)(int8_t)s[ch] * scale;
-        l = (float)(int8_t)s[D + ch] * scale;
+__global__ __launch_bounds__(256) void kv4_read_sums_kernel(const int *__restrict__ blocks, float *__restrict__ lo, kv4_view c, float *__restrict__ hi) {
+    const int phys = blocks[blockIdx.x];
+    const bool there = phys >= 0 && phys < c.num_blocks;
+    for (int head = threadIdx.x >> 6; head < c.heads; head += 4) {
+        const uint8_t *s = c.sums + ((size_t)(there ? phys : 0) * c.heads + head) * kv4_rec<D>::SUM;
+        const float scale = there ? *reinterpret_cast<const float *>(s + 2 * D) : 0.f;
+        const size_t at = ((size_t)blockIdx.x * c.heads + head) * c.head_dim;
+        for (int ch = threadIdx.x & 63; ch < c.head_dim; ch += 64) {
+            lo[at + ch] = there ? (float)(int8_t)s[D + ch] * scale : 0.f;
+            hi[at + ch] = there ? (float)(int8_t)s[ch] * scale : 0.f;
+        }
     }
-    lo[i] = l;
-    hi[i] = h;
 }
 
 __global__ __launch_bounds__(256) void kv4_clear_kernel(uint4 *p, size_t n) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = make_uint4(0, 0, 0, 0);
 }
+
+constexpr size_t ROWS_A_LAUNCH = 1u << 30;  // rows (token, head, side) of an append or a read-back in one launch: 32 bits count them
 
 int log2_of(size_t v) {
     int s = 0;
@@ -406,10 +451,14 @@ PG_API pg_status pg_block_tables_extend_dev(pg_ctx *ctx, const int32_t *seq_lens
                      (batch == 0 || (seq_lens_dev && new_lens_dev && block_table_dev && seq_lens_out_dev && granted_dev)),
                  "pg_block_tables_extend: null pointer");
     const int shift = log2_of(block_size);
-    const bool here = max_tokens <= 4096;
-    PG_TRY(pg_launch(ctx, "extend_tables_kernel", extend_tables_kernel, dim3(1), dim3(1024), 0, seq_lens_dev, new_lens_dev, (int)batch, shift, free_list_dev, free_count_dev,
-                     (int)num_blocks, block_table_dev, (int)max_blocks, seq_lens_out_dev, free_count_out_dev, query_start_dev, granted_dev, slots_dev, (int)max_tokens,
-                     here ? 1 : 0));
+    // One launch, every workgroup with its own sums, unless outputs lie over what the others would still read, or the sums of very
+    // many requests are not worth repeating.
+    const bool in_place = pg_overlap(seq_lens_dev, batch * 4, seq_lens_out_dev, batch * 4) || free_count_dev == free_count_out_dev;
+    const size_t parts = std::max<size_t>(1, (max_tokens + 4095) / 4096);
+    const bool here = parts == 1 || (!in_place && batch <= 4096);
+    PG_TRY(pg_launch(ctx, "extend_tables_kernel", extend_tables_kernel, dim3((unsigned)(here ? parts : 1)), dim3(1024), 0, seq_lens_dev, new_lens_dev, (int)batch, shift,
+                     free_list_dev, free_count_dev, (int)num_blocks, block_table_dev, (int)max_blocks, seq_lens_out_dev, free_count_out_dev, query_start_dev, granted_dev,
+                     here ? slots_dev : nullptr, (int)max_tokens));
     if (here) return PG_OK;
     return pg_launch(ctx, "slot_map_kernel", slot_map_kernel, dim3((unsigned)((max_tokens + 255) / 256)), dim3(256), 0, query_start_dev, seq_lens_out_dev, (int)batch, shift,
                      block_table_dev, (int)max_blocks, granted_dev, slots_dev, (int)max_tokens);
@@ -545,14 +594,16 @@ PG_API pg_status pg_paged_kv4_append_dev(pg_ctx *ctx, pg_paged_kv4 *c, const flo
     PG_CHECK_ARG(k_dev && v_dev && slots_dev, "pg_paged_kv4_append: null pointer");
     PG_CHECK_ARG(tokens < (1ull << 31) && token_stride < (1ull << 40) && head_stride < (1ull << 40), "pg_paged_kv4_append: %zu rows: out of range", tokens);
     c->touch(ctx);
-    const size_t rows = tokens * c->heads * 2;
     const bool wide = c->head_dim % 4 == 0 && token_stride % 4 == 0 && head_stride % 4 == 0 && (((uintptr_t)k_dev | (uintptr_t)v_dev) & 15) == 0;
     return with_width(c->D, [&](auto w) -> pg_status {
-        constexpr int D = decltype(w)::value, PER = 256 / (D / 8);
-        const size_t grid = (rows + PER - 1) / PER;
-        PG_CHECK_ARG(grid < (1ull << 31), "pg_paged_kv4_append: %zu rows of %zu heads: out of range", tokens, c->heads);
-        return pg_launch(ctx, "kv4_append_kernel", wide ? kv4_append_kernel<D, true> : kv4_append_kernel<D, false>, dim3((unsigned)grid), dim3(256), 0, k_dev, v_dev,
-                         kv4_view_of(c), token_stride, head_stride, (int)tokens, slots_dev);
+        constexpr int D = decltype(w)::value, PER = 2 * 256 / (D / 8);
+        const size_t most = ROWS_A_LAUNCH / (2 * c->heads);  // tokens a launch
+        for (size_t at = 0; at < tokens; at += most) {
+            const size_t n = std::min(most, tokens - at);
+            PG_TRY(pg_launch(ctx, "kv4_append_kernel", wide ? kv4_append_kernel<D, true> : kv4_append_kernel<D, false>, dim3((unsigned)((n * c->heads * 2 + PER - 1) / PER)),
+                             dim3(256), 0, k_dev + at * token_stride, v_dev + at * token_stride, kv4_view_of(c), token_stride, head_stride, (int)n, slots_dev + at));
+        }
+        return PG_OK;
     });
 }
 
@@ -565,9 +616,13 @@ PG_API pg_status pg_paged_kv4_read_dev(pg_ctx *ctx, const pg_paged_kv4 *c, const
     c->touch(ctx);
     return with_width(c->D, [&](auto w) -> pg_status {
         constexpr int D = decltype(w)::value, PER = 256 / (D / 8);
-        const size_t grid = (n * c->heads * 2 + PER - 1) / PER;
-        PG_CHECK_ARG(grid < (1ull << 31), "pg_paged_kv4_read: %zu rows of %zu heads: out of range", n, c->heads);
-        return pg_launch(ctx, "kv4_read_kernel", kv4_read_kernel<D>, dim3((unsigned)grid), dim3(256), 0, slots_dev, k_dev, kv4_view_of(c), (int)n, v_dev);
+        const size_t most = ROWS_A_LAUNCH / (2 * c->heads), width = c->heads * c->head_dim;
+        for (size_t at = 0; at < n; at += most) {
+            const size_t m = std::min(most, n - at);
+            PG_TRY(pg_launch(ctx, "kv4_read_kernel", kv4_read_kernel<D>, dim3((unsigned)((m * c->heads * 2 + PER - 1) / PER)), dim3(256), 0, slots_dev + at, k_dev + at * width,
+                             kv4_view_of(c), (int)m, v_dev + at * width));
+        }
+        return PG_OK;
     });
 }
 
@@ -581,7 +636,8 @@ PG_API pg_status pg_paged_kv4_summarise_dev(pg_ctx *ctx, pg_paged_kv4 *c, const 
     c->touch(ctx);
     const kv4_batch ba = {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks};
     return with_width(c->D, [&](auto w) -> pg_status {
-        return pg_launch(ctx, "kv4_summarise_kernel", kv4_summarise_kernel<decltype(w)::value>, dim3((unsigned)tokens, (unsigned)((c->heads + 3) / 4)), dim3(256), 0, ba,
+        return pg_launch(ctx, "kv4_summarise_kernel", kv4_summarise_kernel<decltype(w)::value>, dim3((unsigned)((tokens >> c->shift) + 2 * batch), (unsigned)((c->heads + 3) / 4)),
+                         dim3(256), 0, ba,
                          kv4_view_of(c));
     });
 }
@@ -591,12 +647,10 @@ PG_API pg_status pg_paged_kv4_read_summaries_dev(pg_ctx *ctx, const pg_paged_kv4
     PG_CHECK_ARG(c != nullptr, "pg_paged_kv4_read_summaries: null cache");
     if (n == 0) return PG_OK;
     PG_CHECK_ARG(blocks_dev && lo_dev && hi_dev, "pg_paged_kv4_read_summaries: null pointer");
-    const size_t grid = (n * c->heads * c->head_dim + 255) / 256;
-    PG_CHECK_ARG(n < (1ull << 31) && grid < (1ull << 31), "pg_paged_kv4_read_summaries: %zu blocks: out of range", n);
+    PG_CHECK_ARG(n < (1ull << 24), "pg_paged_kv4_read_summaries: %zu blocks: out of range", n);
     c->touch(ctx);
     return with_width(c->D, [&](auto w) -> pg_status {
-        return pg_launch(ctx, "kv4_read_sums_kernel", kv4_read_sums_kernel<decltype(w)::value>, dim3((unsigned)grid), dim3(256), 0, blocks_dev, lo_dev, kv4_view_of(c), (int)n,
-                         hi_dev);
+        return pg_launch(ctx, "kv4_read_sums_kernel", kv4_read_sums_kernel<decltype(w)::value>, dim3((unsigned)n), dim3(256), 0, blocks_dev, lo_dev, kv4_view_of(c), hi_dev);
     });
 }
 
