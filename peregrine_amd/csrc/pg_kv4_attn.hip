@@ -172,10 +172,10 @@ __device__ __forceinline__ void load_tile(const uint8_t *const (&rec)[2], const 
     }
 }
 
-// Lets products of the matrix cores end before anything reads them.  Straight code needs none of it, but where a branch stands between
-// a product and its first reader the compiler counts the wait along one of the two ways only, and the hardware does not count.
-__device__ __forceinline__ void settle(i32x4 &a, i32x4 &b) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(a), "+v"(b)); }
-__device__ __forceinline__ void settle_all() {  // ahead of accumulators that are read behind a loop
+// Lets products of the matrix cores end before accumulators are read behind a loop.  Straight code needs none of it, but where a
+// branch stands between a product and its first reader the compiler counts the wait along one of the two ways only, and the
+// hardware does not count: so nothing branches between the scores' products and their readers either (masks are without one).
+__device__ __forceinline__ void settle_all() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
     __builtin_amdgcn_sched_barrier(0);
@@ -224,7 +224,6 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
         for (int i = 0; i < 4; ++i) hi[i] = (hi[i] << 8) + q.sum_hi1;  // |hi| < 2^26: 256 channels of 15 x 128 x 256 at most
 #pragma unroll
         for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[1][j], hi, 0, 0, 0);
-        if (MASKED) settle(hi, lo);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float x = fmaf((float)hi[i], 256.f, (float)lo[i]);
@@ -604,10 +603,6 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
 #pragma unroll
             for (int s = 0; s < SETS; ++s) acc[s][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.digit[s][j], k8, acc[s][u], 0, 0, 0);
         }
-    }
-    if (MASKED) {
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) settle(acc[s][0], acc[s][1]), settle(acc[s][2], acc[s][3]);
     }
     float s[NT][4], dv[NT], zv[NT];
 #pragma unroll
@@ -1157,8 +1152,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
                     for (int i = 0; i < 4; ++i) hi[i] = (hi[i] << 8) + q[t].sum_hi1;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q[t].digit[1][j], hi, 0, 0, 0);
-                    if (MASKED) settle(hi, lo);
-#pragma unroll
+            #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float x = fmaf((float)hi[i], 256.f, (float)lo[i]);
                         float y;
