@@ -1317,6 +1317,347 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
     }
 }
 
+// The same for heads up to 128 on 32 x 32 products: a wavefront has 32 rows, so each operand that it takes from LDS serves twice the
+// rows.  Keys go through the f16 matrix cores too, against q as two f16 (scaled by a power of two to 1 .. 2 at the row's
+// largest): two more products a step than with three int8 digits on half the depth, and four instructions a score less, of
+// which there are 16 a lane.  Lanes and operands: A and B of a product hold 8 values of its 16 deep side, row or column lane & 31;
+// a result's registers i are rows (i & 3) + 8 (i >> 2) + 4 (lane >> 5), which makes the probabilities of registers 8 s .. 8 s + 7
+// the B operand of step s once the values' tokens stand in that order.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int D>
+struct prompt32_lds {
+    static constexpr int K = 128 * D, V = 128 * D;  // bytes of 64 tokens' operands
+    alignas(16) uint8_t k[2][K];
+    alignas(16) uint8_t v[2][V];
+    alignas(16) float meta[2][4][64];  // key step, key centre, value step, value centre
+};
+
+template <int D, bool CAP>
+__global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
+    using R = kv4_rec<D>;
+    constexpr int KS = D / 16, DT = D / 32, W = D / 8, KW = D / 32;  // steps of a score, tiles of channels, words of a row, words a lane stages
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+    auto &lds = *reinterpret_cast<prompt32_lds<D> *>(lds_raw);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, c = lane & 31;
+    // The heads next to each other: workgroups go to the XCDs in turn, and a head's rows share its keys in one L2.  The last rows,
+    // which see the most keys, first.
+    unsigned id = blockIdx.x;
+    const int head = id % A.c.heads;
+    id /= A.c.heads;
+    const int split = id % A.splits;
+    id /= A.splits;
+    const int groups = (A.row_tiles + 7) / 8;
+    const int group = groups - 1 - id % groups;
+    const int b = id / groups;
+    const int shift = A.c.shift, bs = 1 << shift;
+    const kv4_request rq = kv4_request_at(A.ba, b, shift);
+    const int rows = min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group;
+    const int r0 = group * 128;
+    if (r0 >= rows) return;
+    const int behind = rq.len - rq.rows;
+    auto pos_of = [&](int r) { return A.mask == PG_MASK_NONE ? rq.len - 1 : behind + r / A.group; };
+    const int mine = r0 + wave * 32, last_row = min(r0 + 128, rows) - 1;
+    const int group_low = pos_of(r0), group_high = pos_of(last_row);
+    const int low_pos = pos_of(min(mine, last_row)), high_pos = mine < rows ? pos_of(min(mine + 32, rows) - 1) : -1;
+    const bool windowed = A.mask == PG_MASK_CAUSAL_SLIDING_WINDOW;
+    const int window = windowed ? A.window : -1;
+    const int to = max(group_high + 1, 0), from = windowed ? (int)max((long)group_low - A.window, 0l) : 0;
+    const int near = from >> 6, sink_tiles = windowed ? min((int)(((long)A.sinks + 63) >> 6), near) : 0;
+    const int tiles = to > 0 ? sink_tiles + ((to + 63) >> 6) - near : 0;
+    const int per = (tiles + A.splits - 1) / A.splits, begin = split * per, end = min(begin + per, tiles);
+
+    const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
+    auto first_of = [&](int tile) { return 64 * (tile < sink_tiles ? tile : tile - sink_tiles + near); };
+    // A tile on its way: the blocks of its four runs first (a tile ahead of the codes), then its codes in registers -- a lane has one
+    // token's chunk of keys, and words of eight tokens' values, those of run `wave` in the order that the products take them.
+    int phys[4], run_pos[4], next_pos[4];
+    auto look = [&](int tile) {
+        const int first = first_of(tile);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int p = first + 16 * r;
+            phys[r] = table[min(p, group_high) >> shift];
+            if (p > group_high) phys[r] = -1;
+        }
+    };
+    uint32_t ck[KW], cv[8], cm = 0;
+    auto fetch = [&](int tile) {
+        const int first = first_of(tile);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool ok = (unsigned)phys[r] < (unsigned)A.c.num_blocks;
+            next_pos[r] = ok ? first + 16 * r : 0x7fffff00;
+            phys[r] = ok ? phys[r] : 0;
+        }
+        const int of_lane = lane < 32 ? (lane < 16 ? phys[0] : phys[1]) : (lane < 48 ? phys[2] : phys[3]);
+        const int at = (first + lane) & (bs - 1);
+        const uint8_t *rec = A.c.data + ((size_t)of_lane * A.c.heads + head) * R::bytes(shift);
+        const uint8_t *kp = rec + (uint32_t)(at * R::ROW) + wave * (4 * KW);
+        if (D == 64) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(kp);
+            ck[0] = x.x, ck[1] = x.y;
+        } else {
+            const uint4 x = *reinterpret_cast<const uint4 *>(kp);
+            ck[0] = x.x, ck[1] = x.y, ck[KW - 2] = x.z, ck[KW - 1] = x.w;
+        }
+        if (wave < 2) cm = reinterpret_cast<const uint32_t *>(rec + (wave ? R::v_meta(shift) : R::k_meta(shift)))[at];
+        const int my_phys = wave < 2 ? (wave == 0 ? phys[0] : phys[1]) : (wave == 2 ? phys[2] : phys[3]);
+        const uint8_t *vp = A.c.data + ((size_t)my_phys * A.c.heads + head) * R::bytes(shift) + R::v(shift) + (size_t)((first + 16 * wave) & (bs - 1)) * R::ROW;
+        const uint32_t vo = 4 * half * R::ROW + (c & (W - 1)) * 4;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cv[e] = *reinterpret_cast<const uint32_t *>(vp + vo + ((e & 3) + 8 * (e >> 2)) * R::ROW);
+    };
+    const f16x2 low_by = {(_Float16)32768.f, (_Float16)32768.f}, high_by = {(_Float16)2048.f, (_Float16)2048.f};
+    const f16x2 centre = {(_Float16)(-7.5f * CODE), (_Float16)(-7.5f * CODE)};
+    const bool upper = c / W & 1;  // which of a byte's channels this lane's rows of values are
+    const uint32_t v_mask = upper ? 0x00f000f0u : 0x000f000fu;
+    const f16x2 v_by = upper ? high_by : low_by;
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+            const int word = KW * wave + i;
+            const uint32_t x = ck[i], y = x >> 8;
+            const f16x2 p0 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x000f000fu), low_by, centre);
+            const f16x2 p1 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, x & 0x00f000f0u), high_by, centre);
+            const f16x2 p2 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, y & 0x000f000fu), low_by, centre);
+            const f16x2 p3 = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, y & 0x00f000f0u), high_by, centre);
+            *reinterpret_cast<f16x8 *>(&lds.k[buf][((half * KS + (word >> 1)) * 64 + c + 32 * (word & 1)) * 16]) = f16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+        }
+        if (wave < 2) {
+            lds.meta[buf][2 * wave][lane] = kv4_d(cm);
+            lds.meta[buf][2 * wave + 1][lane] = kv4_z(cm);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            uint32_t sel = 0x0c040c00u + 0x00010001u * (D == 64 ? 2 * dt : dt);
+            if (D == 64) sel += 0x00010001u * (c >> 4);
+            f16x8 x;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const f16x2 y = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(cv[2 * h + 1], cv[2 * h], sel) & v_mask), v_by, centre);
+                x[2 * h] = y[0], x[2 * h + 1] = y[1];
+            }
+            *reinterpret_cast<f16x8 *>(&lds.v[buf][((wave * DT + dt) * 64 + lane) * 16]) = x;
+        }
+    };
+    if (begin < end) {
+        look(begin);
+        fetch(begin);
+        look(min(begin + 1, end - 1));
+    }
+
+    // The rows: lane (row c, half) has channels 8 (2 step + half) .. + 7 in the keys' order.
+    f16x8 qh[KS], ql[KS];
+    float c1, sq;
+    const int r = mine + c;
+    const bool live = r < rows;
+    {
+        const float *x = live ? A.q + (size_t)(rq.first + r / A.group) * A.q_token + (size_t)(head * A.group + r % A.group) * A.q_head : nullptr;
+        float a[KS][8], sum = 0.f;
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = 8 * (2 * k + half) + (e >> 1) + 4 * (e & 1);
+                a[k][e] = x && d < A.c.head_dim ? x[d] : 0.f;
+                top = max(top, __builtin_bit_cast(uint32_t, a[k][e]) & 0x7fffffffu);
+            }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        const bool bad = top >= 0x7f800000u, none = bad || top < 0x0d800000u;  // 2^-100: scores of 0
+        // to 1 .. 2 by a power of two (of which the inverse is one too: 2^-100 .. 2^127)
+        const uint32_t exponent = none ? 127u << 23 : top & 0x7f800000u;
+        const float by = none ? 0.f : __builtin_bit_cast(float, (254u << 23) - exponent), back = __builtin_bit_cast(float, exponent);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = bad ? 0.f : a[k][e] * by;
+                sum += y;
+                qh[k][e] = (_Float16)y;
+                ql[k][e] = (_Float16)(y - (float)qh[k][e]);
+            }
+        sum += __shfl_xor(sum, 32);
+        const float unit = bad ? __builtin_nanf("") : back * A.scale * (CAP ? 1.f : LOG2E);
+        c1 = unit * (1.f / CODE);
+        sq = sum * unit;
+    }
+    const int row_pos = live ? pos_of(r) : -1;
+    const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    float m = 0.f, l = 0.f, zsum = 0.f, step = 0.f, norm = 0.f;
+    bool set = false;
+
+    auto take = [&](bool masked, int buf) {
+#pragma unroll 1
+        for (int w = 0; w < 2; ++w) {
+            const int pos0 = w ? run_pos[2] : run_pos[0], pos1 = w ? run_pos[3] : run_pos[1];
+            f32x16 x;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const f16x8 key = *reinterpret_cast<const f16x8 *>(&lds.k[buf][((w * KS + k) * 64 + lane) * 16]);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, qh[k], x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, ql[k], x, 0, 0, 0);
+            }
+            float s[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 kd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][0][32 * w + 8 * j + 4 * half]), kz = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][1][32 * w + 8 * j + 4 * half]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float y;
+                    if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(kd[i] * c1, x[4 * j + i], kz[i] * sq) * inv_cap), -m);
+                    else y = fmaf(kd[i] * c1, x[4 * j + i], fmaf(kz[i], sq, -m));
+                    s[4 * j + i] = y;
+                }
+            }
+            if (masked)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = (i < 8 ? pos0 : pos1) + 8 * (i >> 2 & 1) + 4 * half + (i & 3), far = row_pos - key;
+                    s[i] = (far >= 0) & ((window < 0) | (far <= window) | (key < A.sinks)) ? s[i] : -INFINITY;
+                }
+            float pd[16], sum, zs;
+            uint32_t top, steps;
+            auto weigh_as = [&](auto masked_) {
+                constexpr bool MASKED = decltype(masked_)::value;
+                sum = zs = 0.f;
+                top = steps = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 vd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][2][32 * w + 8 * j + 4 * half]), vz = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][3][32 * w + 8 * j + 4 * half]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float y = s[4 * j + i], p = __builtin_amdgcn_exp2f(y);
+                        const bool none = MASKED && y == -INFINITY;  // (what is masked may be anything)
+                        const float d = none ? 0.f : vd[i], z = none ? 0.f : vz[i];
+                        sum += p;
+                        zs = fmaf(p, z, zs);
+                        pd[4 * j + i] = p * (d * norm);
+                        top = max(top, __builtin_bit_cast(uint32_t, pd[4 * j + i]));
+                        steps = max(steps, __builtin_bit_cast(uint32_t, d));
+                    }
+                }
+            };
+            auto weigh = [&] {
+                if (masked) weigh_as(std::true_type{});
+                else weigh_as(std::false_type{});
+            };
+            weigh();
+            if (__ballot(!set || top > __builtin_bit_cast(uint32_t, P_MOST) || steps > __builtin_bit_cast(uint32_t, step) || !(sum < 1.2676506e30f))) {
+                float most = steps < 0x7f800000u ? __builtin_bit_cast(float, steps) : 0.f;  // (a step of NaN reaches what it may and is no scale)
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+                float at = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) at = fmaxf(at, s[i]);
+                at = fmaxf(at, __shfl_xor(at, 32));
+                float f = 1.f;
+                if (at > -INFINITY && (!set || at > 0.f)) {
+                    f = set ? __builtin_amdgcn_exp2f(-at) : 1.f;
+                    m += at;
+                    set = true;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] -= at;
+                }
+                l *= f;
+                zsum *= f;
+                if (most > step) {
+                    const float next = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+                    f *= step / next;
+                    step = next;
+                    norm = P_TOP / next;
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+                weigh();
+            }
+            l += sum;
+            zsum += zs;
+            float minus = -1.f;
+            asm("" : "+s"(minus));  // (not a subtraction, so that one instruction takes the f16 as it is)
+            f16x8 ph[2], pl[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ph[i >> 3][i & 7] = (_Float16)pd[i];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pl[i >> 3][i & 7] = (_Float16)fmaf((float)ph[i >> 3][i & 7], minus, pd[i]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const f16x8 v = *reinterpret_cast<const f16x8 *>(&lds.v[buf][(((2 * w + t) * DT + dt) * 64 + lane) * 16]);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[t], o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[t], o[dt], 0, 0, 0);
+                }
+        }
+    };
+    if (begin < end) store(0);
+    __syncthreads();
+    for (int tile = begin; tile < end; ++tile) {
+        const int buf = (tile - begin) & 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) run_pos[i] = next_pos[i];
+        if (tile + 1 < end) {
+            fetch(tile + 1);
+            look(min(tile + 2, end - 1));
+        }
+        const int far = max(max(run_pos[0], run_pos[1]), max(run_pos[2], run_pos[3])), close = min(min(run_pos[0], run_pos[1]), min(run_pos[2], run_pos[3]));
+        if (close <= high_pos) take(far + 15 > low_pos || (windowed && high_pos - close > window), buf);
+        if (tile + 1 < end) store(buf ^ 1);
+        __syncthreads();
+    }
+
+    settle_all();
+    l += __shfl_xor(l, 32);
+    zsum += __shfl_xor(zsum, 32);
+    if (!live) return;
+    const float back = step * (1.f / (P_TOP * CODE));
+    float *out;
+    float by = 1.f;
+    if (A.splits > 1) {
+        const size_t tile = ((size_t)b * A.c.heads + head) * A.row_tiles + r / 16;
+        float *base = A.part + (tile * A.splits + split) * (16 * D + 32);
+        out = base + (r & 15) * D;
+        if (half == 0) base[16 * D + (r & 15)] = set ? m : l == 0.f ? -INFINITY : 0.f, base[16 * D + 16 + (r & 15)] = l;
+    } else {
+        out = A.out + ((size_t)(rq.first + r / A.group) * A.q_heads + head * A.group + r % A.group) * A.c.head_dim;
+        by = l == 0.f ? 0.f : 1.f / l;
+    }
+    const int most = A.splits > 1 ? D : A.c.head_dim;
+    const bool wide = (most & 3) == 0 && ((uintptr_t)out & 15) == 0;
+    auto put = [&](int d, float x0, float x1, float x2, float x3) {
+        const float4 y = make_float4(fmaf(x0, back, zsum) * by, fmaf(x1, back, zsum) * by, fmaf(x2, back, zsum) * by, fmaf(x3, back, zsum) * by);
+        if (wide) {
+            if (d < most) *reinterpret_cast<float4 *>(out + d) = y;
+        } else {
+            if (d < most) out[d] = y.x;
+            if (d + 1 < most) out[d + 1] = y.y;
+            if (d + 2 < most) out[d + 2] = y.z;
+            if (d + 3 < most) out[d + 3] = y.w;
+        }
+    };
+    // Row rho = a + 8 j + 4 half of a tile is word rho % W of a row of values, and of the word's channels the one that `store` chose.
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        if constexpr (D == 64) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) put(8 * (a + 4 * half) + 4 * dt, o[dt][a], o[dt][4 + a], o[dt][8 + a], o[dt][12 + a]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int dt = 0; dt < DT; dt += 2) put(8 * (a + 8 * j + 4 * half) + 2 * dt, o[dt][4 * j + a], o[dt][4 * (j + 2) + a], o[dt + 1][4 * j + a], o[dt + 1][4 * (j + 2) + a]);
+        }
+    }
+}
+
 // The splits of a row into its output, in their order: a wavefront a row, `RT` rows a tile.  The splits' weights first, a lane a
 // split, so that the loop over their rows waits for nothing but its loads.
 template <int D, int RT, bool SELECTED>
@@ -1569,16 +1910,15 @@ size_t pick_splits(const pg_ctx *ctx, int D, size_t tiles, size_t tokens) {
 
 struct plan {
     size_t rows, row_tiles, tiles, splits, bytes;  // rows a tile (4, 8 or 16)
-    size_t wide;                                   // row tiles a workgroup of kv4_prompt_kernel, or 0: the other kernels
+    size_t wide;                                   // row tiles a workgroup of the prompts' kernels, or 0: the others
 };
-constexpr int PROMPT_RT = 1, PROMPT_NW = 8;
 constexpr size_t PROMPT_TILES = 4;
 plan plan_for(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t units, size_t unit_rows, size_t tokens) {
     plan p;
     p.rows = unit_rows <= 4 ? 4 : unit_rows <= 8 ? 8 : 16;
     p.row_tiles = (unit_rows + p.rows - 1) / p.rows;
     p.tiles = units * c->heads * p.row_tiles;
-    p.wide = p.row_tiles < PROMPT_TILES ? 0 : PROMPT_RT * PROMPT_NW;
+    p.wide = p.row_tiles < PROMPT_TILES ? 0 : 8;
     const size_t workgroups = p.wide ? units * c->heads * ((p.row_tiles + p.wide - 1) / p.wide) : p.tiles;
     p.splits = pick_splits(ctx, c->D, workgroups, tokens);
     p.bytes = p.splits > 1 ? p.tiles * p.splits * (p.rows * (size_t)c->D + 32) * sizeof(float) : 0;
@@ -1605,11 +1945,15 @@ pg_status launch_rows(pg_ctx *ctx, const char *fn, const pg_paged_kv4 *c, kv4_at
         };
         if constexpr (!SELECTED)
             if (p.wide) {
-                auto kernel = A.cap > 0.f ? kv4_prompt_kernel<D, PROMPT_RT, PROMPT_NW, true> : kv4_prompt_kernel<D, PROMPT_RT, PROMPT_NW, false>;
-                constexpr size_t lds = sizeof(prompt_lds<D>);
-                if (lds > (48u << 10)) PG_TRY(pg_allow_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds));
-                const size_t groups = (p.row_tiles + p.wide - 1) / p.wide;
-                PG_TRY(pg_launch(ctx, "kv4_prompt_kernel", kernel, dim3((unsigned)(A.ba.batch * c->heads * groups * p.splits)), dim3(64 * PROMPT_NW), lds, A));
+                const dim3 workgroups((unsigned)(A.ba.batch * c->heads * ((p.row_tiles + p.wide - 1) / p.wide) * p.splits));
+                auto prompt = [&](const char *name, auto kernel, size_t lds, unsigned threads) -> pg_status {
+                    PG_TRY(pg_allow_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds));
+                    return pg_launch(ctx, name, kernel, workgroups, dim3(threads), lds, A);
+                };
+                if constexpr (D == 256)
+                    PG_TRY(prompt("kv4_prompt_kernel", A.cap > 0.f ? kv4_prompt_kernel<D, 1, 8, true> : kv4_prompt_kernel<D, 1, 8, false>, sizeof(prompt_lds<D>), 512));
+                else
+                    PG_TRY(prompt("kv4_prompt32_kernel", A.cap > 0.f ? kv4_prompt32_kernel<D, true> : kv4_prompt32_kernel<D, false>, sizeof(prompt32_lds<D>), 256));
                 return p.splits == 1 ? PG_OK : pg_launch(ctx, "kv4_join_kernel", kv4_join_kernel<D, 16, SELECTED>, join, block, 0, A);
             }
         if (p.rows == 4) return go(SELECTED ? "kv4_few_selected_kernel" : "kv4_few_kernel", kv4_few_kernel<D, 4, false, SELECTED>, kv4_few_kernel<D, 4, true, SELECTED>, kv4_join_kernel<D, 4, SELECTED>);
