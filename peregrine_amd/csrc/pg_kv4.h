@@ -48,26 +48,58 @@ struct kv4_rec {
 __device__ __forceinline__ float kv4_z(uint32_t meta) { return __builtin_bit_cast(float, meta << 16); }
 __device__ __forceinline__ float kv4_d(uint32_t meta) { return __builtin_bit_cast(float, meta & 0xffff0000u); }
 
-// The request that packed row t belongs to (starts ascending, batch + 1 of them), or -1; the whole wavefront asks.
-__device__ __forceinline__ int kv4_request_of(const int *__restrict__ starts, int batch, int t) {
-    int below = 0;
-    for (int i = threadIdx.x & 63; i - (int)(threadIdx.x & 63) <= batch; i += 64)
-        below += __popcll(__ballot(i <= batch && starts[min(i, batch)] <= t));
-    return below >= 1 && below <= batch ? below - 1 : -1;
-}
-
 // What a request of the batch asks of a step, made safe: rows outside the packed array and lengths outside the table are cut.
 struct kv4_request {
     int first, rows, len;  // first packed row, rows, tokens in the cache (the rows among them: they are the last)
 };
-__device__ __forceinline__ kv4_request kv4_request_at(const kv4_batch &ba, int b, int shift) {
-    kv4_request r;
-    r.first = ba.starts[b];
-    r.rows = ba.starts[b + 1] - r.first;
-    const long most = (long)ba.max_blocks << shift;
-    r.len = (int)min((long)max(ba.lens[b], 0), most);
-    if (r.first < 0 || r.rows < 0 || r.first > ba.tokens) r.rows = 0;
+__device__ __forceinline__ kv4_request kv4_request_of(const kv4_batch &ba, int from, int to, int len, int shift) {
+    kv4_request r = {from, to - from, (int)min((long)max(len, 0), (long)ba.max_blocks << shift)};
+    if (from < 0 || to < from || from > ba.tokens) r.rows = 0;
     return r;
 }
+__device__ __forceinline__ kv4_request kv4_request_at(const kv4_batch &ba, int b, int shift) { return kv4_request_of(ba, ba.starts[b], ba.starts[b + 1], ba.lens[b], shift); }
+
+// The request that packed row t belongs to and what it asks, or -1: a lane looks at a request, so that up to 64 of them cost one
+// memory latency.  The whole wavefront asks.
+__device__ __forceinline__ int kv4_find(const kv4_batch &ba, int t, int shift, kv4_request &r) {
+    const int lane = threadIdx.x & 63;
+    for (int at = 0; at < ba.batch; at += 64) {
+        const int i = min(at + lane, ba.batch - 1);
+        const int from = ba.starts[i], to = ba.starts[i + 1], len = ba.lens[i];
+        const uint64_t mine = __ballot(at + lane < ba.batch && from <= t && t < to);
+        if (mine) {
+            const int who = __builtin_ctzll(mine);
+            r = kv4_request_of(ba, __builtin_amdgcn_readlane(from, who), __builtin_amdgcn_readlane(to, who), __builtin_amdgcn_readlane(len, who), shift);
+            return r.rows > 0 ? at + who : -1;
+        }
+    }
+    return -1;
+}
+
+// Sums and maxima across lanes without LDS: DPP moves within 16, swaps of rows and halves beyond.
+struct kv4_add { __device__ float operator()(float a, float b) const { return a + b; } };
+struct kv4_max { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct kv4_umax { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; } };
+struct kv4_iadd { __device__ int operator()(int a, int b) const { return a + b; } };
+template <class T, class F>
+__device__ __forceinline__ T over_16(T v, F f) {  // lanes of a row of 16
+    const auto move = [](T x, auto ctrl) { return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, false)); };
+    v = f(v, move(v, std::integral_constant<int, 0xB1>{}));   // quad_perm [1,0,3,2]
+    v = f(v, move(v, std::integral_constant<int, 0x4E>{}));   // quad_perm [2,3,0,1]
+    v = f(v, move(v, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+    return f(v, move(v, std::integral_constant<int, 0x140>{}));  // row_mirror
+}
+template <class T, class F>
+__device__ __forceinline__ T over_rows(T v, F f) {  // lane and lane ^ 16
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    return f(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
+}
+template <class T, class F>
+__device__ __forceinline__ T over_halves(T v, F f) {  // lane and lane ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    return f(__builtin_bit_cast(T, (unsigned)r[0]), __builtin_bit_cast(T, (unsigned)r[1]));
+}
+template <class T, class F>
+__device__ __forceinline__ T over_wave(T v, F f) { return over_halves(over_rows(over_16(v, f), f), f); }
 
 pg_status pg_kv4_check_step(const char *fn, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t tokens, size_t max_blocks);

@@ -49,18 +49,10 @@ struct q_rows {
     float unit, sum;               // value of a unit, sum of the row in units
 };
 
-__device__ __forceinline__ float over_groups(float v) {  // sum over the four lanes of a row
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
-}
-__device__ __forceinline__ int over_groups(int v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
-}
-__device__ __forceinline__ float max_groups(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
+// Over the four lanes of a row (lane & 15).
+__device__ __forceinline__ float over_groups(float v) { return over_halves(over_rows(v, kv4_add{}), kv4_add{}); }
+__device__ __forceinline__ int over_groups(int v) { return over_halves(over_rows(v, kv4_iadd{}), kv4_iadd{}); }
+__device__ __forceinline__ float max_groups(float v) { return over_halves(over_rows(v, kv4_max{}), kv4_max{}); }
 
 // First channel of the 16 that lane group g holds for the j-th product.
 template <int D>
@@ -90,8 +82,7 @@ __device__ __forceinline__ void fix_q(const float *x, int head_dim, int g, q_fix
             a[j][e] = x && d < head_dim ? x[d] : 0.f;
             top = max(top, __builtin_bit_cast(uint32_t, a[j][e]) & 0x7fffffffu);  // (of magnitudes the bits are in order, NaN last)
         }
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    top = over_halves(over_rows(top, kv4_umax{}), kv4_umax{});
     const bool bad = top >= 0x7f800000u;
     const float most = __builtin_bit_cast(float, top);
     const float inv = bad || most < 7.88860905e-31f ? 0.f : Q_UNITS / most;  // under 2^-100: scores of 0
@@ -199,8 +190,8 @@ struct row_view {
     int window, sinks;    // and, where window >= 0, from window behind it or below sinks
 };
 
-template <int D, bool CAP, bool MASKED>
-__device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &q, softmax_rows<D> &a, const row_view &rv, float c1, float sq, float cap_log2e, float inv_cap,
+template <int D, bool CAP>
+__device__ __forceinline__ void take_tile(bool masked, const kv_tile<D> &t, const q_rows<D> &q, softmax_rows<D> &a, const row_view &rv, float c1, float sq, float cap_log2e, float inv_cap,
                                           int lane) {
     constexpr int NJ = D / 64, NV = D / 16, NC = kv_tile<D>::NC;
     const int g = lane >> 4;
@@ -232,19 +223,20 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
             float y;
             if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(d * c1, x, w * sq) * inv_cap), -a.m);
             else y = fmaf(d * c1, x, fmaf(w, sq, -a.m));
-            float z = kv4_z(vm), e = kv4_d(vm);
-            if (MASKED) {
-                const int key = t.pos[r] + 4 * g + i, far = rv.pos - key;
-                const bool seen = (far >= 0) & ((rv.window < 0) | (far <= rv.window) | (key < rv.sinks));  // (no branch)
-                y = seen ? y : -INFINITY;
-                z = seen ? z : 0.f;  // what is masked may be anything
-                e = seen ? e : 0.f;
-            }
             s[4 * r + i] = y;
-            zv[4 * r + i] = z;
-            dv[4 * r + i] = e;
+            zv[4 * r + i] = kv4_z(vm);
+            dv[4 * r + i] = kv4_d(vm);
         }
     }
+    if (masked)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = t.pos[i >> 2] + 4 * g + (i & 3), far = rv.pos - key;
+            const bool seen = (far >= 0) & ((rv.window < 0) | (far <= rv.window) | (key < rv.sinks));
+            s[i] = seen ? s[i] : -INFINITY;
+            zv[i] = seen ? zv[i] : 0.f;  // what is masked may be anything
+            dv[i] = seen ? dv[i] : 0.f;
+        }
     float p[8], pd[8], sum;
     uint32_t top;
     auto weigh = [&] {
@@ -282,8 +274,7 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
                 a.m += at;
                 a.set = true;
             }
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+            most = over_wave(most, kv4_max{});
             float fo = f;
             if (most > a.step) {
                 const float step = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
@@ -342,7 +333,7 @@ __device__ __forceinline__ void take_tile(const kv_tile<D> &t, const q_rows<D> &
 // with SELECTED the group's rows of one token) over one of `splits` runs of their keys, its four wavefronts every fourth
 // tile of 32 tokens.
 template <int D, bool CAP, bool SELECTED>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_rows_kernel(kv4_attn A) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_rows_kernel(kv4_attn A) {
     using R = kv4_rec<D>;
     constexpr int STRIDE = D + 4;
     __shared__ float so[4][16][STRIDE];
@@ -357,9 +348,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_rows_kernel(kv4_att
     const int unit = id / A.c.heads;
     const int shift = A.c.shift, bs = 1 << shift;
 
-    const int b = SELECTED ? kv4_request_of(A.ba.starts, A.ba.batch, unit) : unit;
+    kv4_request rq;
+    const int b = SELECTED ? kv4_find(A.ba, unit, shift, rq) : unit;
     if (SELECTED && b < 0) return;
-    const kv4_request rq = kv4_request_at(A.ba, b, shift);
+    if (!SELECTED) rq = kv4_request_at(A.ba, b, shift);
     const int tok0 = SELECTED ? unit - rq.first : 0;
     const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group;
     const int r0 = rt * 16;
@@ -437,8 +429,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_rows_kernel(kv4_att
 
     auto take = [&] {
         const bool whole = max(t.pos[0], t.pos[1]) + 15 <= low_pos && (!windowed || high_pos - min(t.pos[0], t.pos[1]) <= A.window);
-        if (whole) take_tile<D, CAP, false>(t, q, a, rv, c1, sq, cap_log2e, inv_cap, lane);
-        else take_tile<D, CAP, true>(t, q, a, rv, c1, sq, cap_log2e, inv_cap, lane);
+        take_tile<D, CAP>(!whole, t, q, a, rv, c1, sq, cap_log2e, inv_cap, lane);
     };
     while (tile < end) {
         take();
@@ -571,23 +562,15 @@ struct softmax_few {
 
 constexpr int P_ROW = 72;  // f16 from one row of probabilities to the next: 64 and a shift of four banks
 
-template <int HB>
-__device__ __forceinline__ float max_heads(float v) {  // over the lanes that have this lane's heads
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-    if (HB == 4) v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
-template <int HB>
-__device__ __forceinline__ float sum_heads(float v) {
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
-    if (HB == 4) v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+template <int HB, class F>
+__device__ __forceinline__ float over_heads(float v, F f) {  // over the lanes that have this lane's heads
+    v = over_16(v, f);
+    if (HB == 4) v = over_rows(v, f);
+    return over_halves(v, f);
 }
 
-template <int D, int HB, bool CAP, bool MASKED>
-__device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D, HB> &q, softmax_few<D> &a, const int (&row_pos)[4], int window, int sinks,
+template <int D, int HB, bool CAP>
+__device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, const q_few<D, HB> &q, softmax_few<D> &a, const int (&row_pos)[4], int window, int sinks,
                                             const float (&c1)[4], const float (&sq)[4], float cap_log2e, float inv_cap, int lane, _Float16 *pbuf) {
     constexpr int NJ = D / 64, NC = kv_tile64<D>::NC, SETS = HB == 4 ? 1 : 2, NT = HB / 4;  // NT: tokens a lane
     const int g = lane >> 4, c = lane & 15;
@@ -629,44 +612,51 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
         const float d = kv4_d(t.km[p]), w = fmaf(0.5f, d, kv4_z(t.km[p]));
         zv[p] = kv4_z(t.vm[p]);
         dv[p] = kv4_d(t.vm[p]);
-        bool any = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float y;
-            if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(d * c1[i], s[p][i], w * sq[i]) * inv_cap), -a.m[i]);
-            else y = fmaf(d * c1[i], s[p][i], fmaf(w, sq[i], -a.m[i]));
-            if (MASKED) {
-                const int run = HB == 4 ? (g == 0 ? t.pos[0] : g == 1 ? t.pos[1] : g == 2 ? t.pos[2] : t.pos[3]) : (g < 2 ? t.pos[2 * p] : t.pos[2 * p + 1]);
-                const int key = run + c, far = row_pos[i] - key;
-                const bool seen = (far >= 0) & ((window < 0) | (far <= window) | (key < sinks));  // (no branch)
-                y = seen ? y : -INFINITY;
-                any |= seen;
-            }
-            s[p][i] = y;
-        }
-        if (MASKED) {  // what no row sees may be anything; a row's own mask is on its probability below
-            zv[p] = any ? zv[p] : 0.f;
-            dv[p] = any ? dv[p] : 0.f;
+            if (CAP) s[p][i] = fmaf(cap_log2e, tanhf(fmaf(d * c1[i], s[p][i], w * sq[i]) * inv_cap), -a.m[i]);
+            else s[p][i] = fmaf(d * c1[i], s[p][i], fmaf(w, sq[i], -a.m[i]));
         }
     }
-    float pr[NT][4], pd[NT][4], sum[4], total;
+    if (masked)
+#pragma unroll
+        for (int p = 0; p < NT; ++p) {
+            const int run = HB == 4 ? (g == 0 ? t.pos[0] : g == 1 ? t.pos[1] : g == 2 ? t.pos[2] : t.pos[3]) : (g < 2 ? t.pos[2 * p] : t.pos[2 * p + 1]);
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = run + c, far = row_pos[i] - key;
+                const bool seen = (far >= 0) & ((window < 0) | (far <= window) | (key < sinks));
+                s[p][i] = seen ? s[p][i] : -INFINITY;
+                any |= seen;
+            }
+            zv[p] = any ? zv[p] : 0.f;  // what no row sees may be anything; a row's own mask is on its probability below
+            dv[p] = any ? dv[p] : 0.f;
+        }
+    float pd[NT][4], sum[4], zs[4], total;
     uint32_t top;
-    auto weigh = [&] {
+    auto weigh_as = [&](auto masked_) {
+        constexpr bool MASKED = decltype(masked_)::value;
         total = 0.f;
         top = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            sum[i] = 0.f;
+            sum[i] = zs[i] = 0.f;
 #pragma unroll
             for (int p = 0; p < NT; ++p) {
-                pr[p][i] = __builtin_amdgcn_exp2f(s[p][i]);
-                sum[i] += pr[p][i];
-                pd[p][i] = pr[p][i] * (dv[p] * a.norm);
-                if (MASKED) pd[p][i] = s[p][i] == -INFINITY ? 0.f : pd[p][i];  // (a step of NaN is not this row's where it is masked)
+                const float pr = __builtin_amdgcn_exp2f(s[p][i]);
+                const bool none = MASKED && s[p][i] == -INFINITY;  // (a token that another row sees may be NaN)
+                sum[i] += pr;
+                zs[i] = fmaf(pr, none ? 0.f : zv[p], zs[i]);
+                pd[p][i] = pr * ((none ? 0.f : dv[p]) * a.norm);
                 top = max(top, __builtin_bit_cast(uint32_t, pd[p][i]));  // (none is negative: the bits are in order, NaN last)
             }
             total += sum[i];
         }
+    };
+    auto weigh = [&] {
+        if (masked) weigh_as(std::true_type{});
+        else weigh_as(std::false_type{});
     };
     weigh();
     bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(total < 1.2676506e30f);  // 2^100; a NaN is off too
@@ -680,7 +670,7 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
         for (int i = 0; i < 4; ++i) {
             float at = s[0][i];
             if (NT == 2) at = fmaxf(at, s[NT - 1][i]);
-            at = max_heads<HB>(at);
+            at = over_heads<HB>(at, kv4_max{});
             f[i] = 1.f;
             if (at > -INFINITY && (!a.set[i] || at > 0.f)) {
                 f[i] = a.set[i] ? __builtin_amdgcn_exp2f(-at) : 1.f;
@@ -692,8 +682,7 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
             a.l[i] *= f[i];
             a.zsum[i] *= f[i];
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+        most = over_wave(most, kv4_max{});
         // the column's head: its factor from a lane that has it
         float fo = 1.f;
 #pragma unroll
@@ -724,11 +713,10 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
             const _Float16 hi = (_Float16)pd[p][i];
             pbuf[head * P_ROW + at] = hi;
             pbuf[(HB + head) * P_ROW + at] = (_Float16)fmaf((float)hi, minus, pd[p][i]);
-            a.zsum[i] = MASKED ? a.zsum[i] + (s[p][i] == -INFINITY ? 0.f : pr[p][i] * zv[p]) : fmaf(pr[p][i], zv[p], a.zsum[i]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a.l[i] += sum[i];
+    for (int i = 0; i < 4; ++i) a.l[i] += sum[i], a.zsum[i] += zs[i];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -762,7 +750,7 @@ __device__ __forceinline__ void take_tile64(const kv_tile64<D> &t, const q_few<D
 
 // As kv4_rows_kernel, for up to HB rows of a unit: one row tile, wavefronts every fourth tile of 64 tokens.
 template <int D, int HB, bool CAP, bool SELECTED>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_few_kernel(kv4_attn A) {
+__global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void kv4_few_kernel(kv4_attn A) {
     using R = kv4_rec<D>;
     constexpr int STRIDE = D + 4;
     __shared__ __attribute__((aligned(16))) char lds[4 * 2 * HB * STRIDE * 4 > 4 * 2 * HB * P_ROW * 2 ? 4 * 2 * HB * STRIDE * 4 : 4 * 2 * HB * P_ROW * 2];
@@ -776,9 +764,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_few_kernel(kv4_attn
     const int unit = id / A.c.heads;
     const int shift = A.c.shift, bs = 1 << shift;
 
-    const int b = SELECTED ? kv4_request_of(A.ba.starts, A.ba.batch, unit) : unit;
+    kv4_request rq;
+    const int b = SELECTED ? kv4_find(A.ba, unit, shift, rq) : unit;
     if (SELECTED && b < 0) return;
-    const kv4_request rq = kv4_request_at(A.ba, b, shift);
+    if (!SELECTED) rq = kv4_request_at(A.ba, b, shift);
     const int tok0 = SELECTED ? unit - rq.first : 0;
     const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group;
     if (rows <= 0 || (SELECTED && (unsigned)tok0 >= (unsigned)rq.rows)) return;
@@ -895,8 +884,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_few_kernel(kv4_attn
     auto take = [&] {
         const int far = max(max(t.pos[0], t.pos[1]), max(t.pos[2], t.pos[3])), close = min(min(t.pos[0], t.pos[1]), min(t.pos[2], t.pos[3]));
         const bool whole = far + 15 <= low_pos && (!windowed || high_pos - close <= A.window);
-        if (whole) take_tile64<D, HB, CAP, false>(t, q, a, row_pos, window, A.sinks, c1, sq, cap_log2e, inv_cap, lane, pbuf);
-        else take_tile64<D, HB, CAP, true>(t, q, a, row_pos, window, A.sinks, c1, sq, cap_log2e, inv_cap, lane, pbuf);
+        take_tile64<D, HB, CAP>(!whole, t, q, a, row_pos, window, A.sinks, c1, sq, cap_log2e, inv_cap, lane, pbuf);
     };
     while (tile < end) {
         take();
@@ -908,8 +896,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_few_kernel(kv4_attn
     // Four wavefronts' sums, and each column's two halves, into one.
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        a.l[i] = sum_heads<HB>(a.l[i]);
-        a.zsum[i] = sum_heads<HB>(a.zsum[i]);
+        a.l[i] = over_heads<HB>(a.l[i], kv4_add{});
+        a.zsum[i] = over_heads<HB>(a.zsum[i], kv4_add{});
     }
     __syncthreads();  // (the probabilities' memory is the sums')
     constexpr int RUN = D / 4;
@@ -1208,8 +1196,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
                 float most = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) most = fmaxf(most, dv[i]);
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+                most = over_wave(most, kv4_max{});
                 float fs = 1.f;
                 if (most > step) {
                     const float next = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
@@ -1464,7 +1451,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                 a[k][e] = x && d < A.c.head_dim ? x[d] : 0.f;
                 top = max(top, __builtin_bit_cast(uint32_t, a[k][e]) & 0x7fffffffu);
             }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        top = over_halves(top, kv4_umax{});
         const bool bad = top >= 0x7f800000u, none = bad || top < 0x0d800000u;  // 2^-100: scores of 0
         // to 1 .. 2 by a power of two (of which the inverse is one too: 2^-100 .. 2^127)
         const uint32_t exponent = none ? 127u << 23 : top & 0x7f800000u;
@@ -1478,7 +1465,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                 qh[k][e] = (_Float16)y;
                 ql[k][e] = (_Float16)(y - (float)qh[k][e]);
             }
-        sum += __shfl_xor(sum, 32);
+        sum = over_halves(sum, kv4_add{});
         const float unit = bad ? __builtin_nanf("") : back * A.scale * (CAP ? 1.f : LOG2E);
         c1 = unit * (1.f / CODE);
         sq = sum * unit;
@@ -1553,12 +1540,11 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
             weigh();
             if (__ballot(!set || top > __builtin_bit_cast(uint32_t, P_MOST) || steps > __builtin_bit_cast(uint32_t, step) || !(sum < 1.2676506e30f))) {
                 float most = steps < 0x7f800000u ? __builtin_bit_cast(float, steps) : 0.f;  // (a step of NaN reaches what it may and is no scale)
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+                most = over_wave(most, kv4_max{});
                 float at = s[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) at = fmaxf(at, s[i]);
-                at = fmaxf(at, __shfl_xor(at, 32));
+                at = over_halves(at, kv4_max{});
                 float f = 1.f;
                 if (at > -INFINITY && (!set || at > 0.f)) {
                     f = set ? __builtin_amdgcn_exp2f(-at) : 1.f;
@@ -1615,8 +1601,8 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
     }
 
     settle_all();
-    l += __shfl_xor(l, 32);
-    zsum += __shfl_xor(zsum, 32);
+    l = over_halves(l, kv4_add{});
+    zsum = over_halves(zsum, kv4_add{});
     if (!live) return;
     const float back = step * (1.f / (P_TOP * CODE));
     float *out;
@@ -1671,17 +1657,17 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(kv4_attn A) {
     const int rt = tile % A.row_tiles;
     tile /= A.row_tiles;
     const int head = tile % A.c.heads, unit = tile / A.c.heads;
-    const int b = SELECTED ? kv4_request_of(A.ba.starts, A.ba.batch, unit) : unit;
-    if (b < 0 || (!SELECTED && b >= A.ba.batch)) return;
-    const kv4_request rq = kv4_request_at(A.ba, b, A.c.shift);
+    kv4_request rq;
+    const int b = SELECTED ? kv4_find(A.ba, unit, A.c.shift, rq) : unit;
+    if (b < 0 || b >= A.ba.batch) return;
+    if (!SELECTED) rq = kv4_request_at(A.ba, b, A.c.shift);
     const int rows = SELECTED ? A.group : min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group, r = rt * RT + row;
     if (r >= rows || (SELECTED && (unsigned)(unit - rq.first) >= (unsigned)rq.rows)) return;
     const int token = SELECTED ? unit : rq.first + r / A.group;
     const float *part = A.part + first * NEXT;
     float m = -INFINITY;
     for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, part[s * NEXT + RT * D + row]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    m = over_wave(m, kv4_max{});
     float l = 0.f, o[D / 64];
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
@@ -1690,8 +1676,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(kv4_attn A) {
         const float ms = s < A.splits ? part[s * NEXT + RT * D + row] : -INFINITY;
         const float w = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
         float mine = w == 0.f ? 0.f : w * part[s * NEXT + RT * D + 16 + row];
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d);
+        mine = over_wave(mine, kv4_add{});
         l += mine;
         const float *rows_at = part + s0 * NEXT + row * D + lane;
         auto add = [&](int j, const float (&x)[D / 64]) {
@@ -1742,22 +1727,37 @@ __device__ __forceinline__ uint32_t score_key(float s) {
 
 // One workgroup: one query token and key head.  Scores of 16 blocks a wavefront at a time -- rows of the product are the
 // group's query rows (x where positive, x where negative), columns the blocks (hi, lo), whole numbers throughout, and two
-// f32 products a score -- then the key that exactly `top` blocks reach by four passes of 8 bits over a histogram in LDS,
-// then the blocks over it, and of those at it the first, in ascending order.
+// f32 products a score.  Then the key that exactly as many blocks reach as are wanted: passes of 8 bits over a histogram in LDS,
+// from the highest bit in which the keys differ, every wavefront with its own sums over the bins, so a pass is one barrier.  Then
+// the blocks over that key, and of those at it the first, in ascending order.  It is a chain of latencies (request, table,
+// summaries, passes): several tiles' loads go out together, queries ahead of everything.
 template <int D, int T>
 __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
     using R = kv4_rec<D>;
-    constexpr int NJ = D / 64, W = T / 64;
+    constexpr int NJ = D / 64, W = T / 64, U = T == 256 || D == 256 ? 1 : 4;  // U: tiles of 16 blocks whose loads go out together (few wavefronts: all that they have; many: registers count)
     extern __shared__ uint32_t keys[];  // [blocks]
-    __shared__ uint32_t hist[256];
-    __shared__ int above[W], at_key[W], found[2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4, tid = threadIdx.x;
-    const int token = blockIdx.x / A.c.heads, head = blockIdx.x % A.c.heads, shift = A.c.shift;
+    __shared__ uint32_t hist[4][256], least, most_key;
+    __shared__ int above[W], at_key[W];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, g = lane >> 4, tid = threadIdx.x;
+    const int token = blockIdx.x / (unsigned)A.c.heads, head = blockIdx.x % (unsigned)A.c.heads, shift = A.c.shift;
+    for (int i = tid; i < 1024; i += T) hist[i >> 8][i & 255] = 0;
+    if (tid == 0) least = 0xffffffffu, most_key = 0;
+    float a[NJ][16];
+    auto load_rows = [&](int r0) {
+        const float *x = r0 + row < A.group ? A.q + (size_t)token * A.q_token + (size_t)(head * A.group + r0 + row) * A.q_head : nullptr;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int d = 64 * j + 16 * g + e;
+                a[j][e] = x && d < A.c.head_dim ? x[d] : 0.f;
+            }
+    };
+    load_rows(0);
     int *out = A.selected + ((size_t)token * A.c.heads + head) * A.top;
-    const int b = kv4_request_of(A.ba.starts, A.ba.batch, token);
+    kv4_request rq;
+    const int b = kv4_find(A.ba, token, shift, rq);
     if (b < 0) return;
-    const kv4_request rq = kv4_request_at(A.ba, b, shift);
-    if ((unsigned)(token - rq.first) >= (unsigned)rq.rows) return;
     const int pos = rq.len - rq.rows + (token - rq.first);
     const int blocks = pos < 0 ? 0 : (pos >> shift) + 1;
     if (blocks <= A.top) {
@@ -1765,23 +1765,21 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
         return;
     }
     const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
+    const int free_from = A.first, free_to = blocks - A.recent;  // the blocks that are chosen by score
+    __syncthreads();
+    uint32_t low = 0xffffffffu, high = 0;
     for (int r0 = 0; r0 < A.group; r0 += 16) {
-        const float *x = r0 + row < A.group ? A.q + (size_t)token * A.q_token + (size_t)(head * A.group + r0 + row) * A.q_head : nullptr;
+        if (r0) load_rows(r0);
         i32x4 pos8[NJ], neg8[NJ];
-        float a[NJ][16], most = 0.f;
-        bool bad = false;
+        uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int d = 64 * j + 16 * g + e;
-                a[j][e] = x && d < A.c.head_dim ? x[d] : 0.f;
-                most = fmaxf(most, fabsf(a[j][e]));
-                bad |= !(fabsf(a[j][e]) <= 3.402823466e38f);
-            }
-        most = max_groups(most);
-        bad = max_groups(bad ? 1.f : 0.f) != 0.f;
-        const float r = bad || most < 7.88860905e-31f ? 0.f : 1.0f / most * 127.f;
+            for (int e = 0; e < 16; ++e) top = max(top, __builtin_bit_cast(uint32_t, a[j][e]) & 0x7fffffffu);  // (of magnitudes the bits are in order, NaN last)
+        top = over_halves(over_rows(top, kv4_umax{}), kv4_umax{});
+        const bool bad = top >= 0x7f800000u;
+        const float most = __builtin_bit_cast(float, top);
+        const float r = bad || most < 7.88860905e-31f ? 0.f : 1.0f / most * 127.f;  // 2^-100
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -1800,51 +1798,77 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
         float unit[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) unit[i] = __shfl(bad ? 0.f : most * (1.0f / 127.f), 4 * g + i);
-        for (int j0 = 16 * wave; j0 < blocks; j0 += 16 * W) {
-            const int block = j0 + row;
-            const int phys = block < blocks ? table[block] : -1;
-            const bool there = phys >= 0 && phys < A.c.num_blocks;
-            const uint8_t *s = A.c.sums + ((size_t)(there ? phys : 0) * A.c.heads + head) * R::SUM;
-            i32x4 acc = {0, 0, 0, 0};
+        for (int j0 = 16 * wave; j0 < blocks; j0 += 16 * W * U) {
+            int phys[U];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos8[j], *reinterpret_cast<const i32x4 *>(s + 64 * j + 16 * g), acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg8[j], *reinterpret_cast<const i32x4 *>(s + D + 64 * j + 16 * g), acc, 0, 0, 0);
+            for (int u = 0; u < U; ++u) {
+                const int block = j0 + 16 * W * u + row;
+                phys[u] = table[min(block, blocks - 1)];
             }
-            const float scale = *reinterpret_cast<const float *>(s + 2 * D);
-            float score = -INFINITY;
+            i32x4 hi[U][NJ], lo[U][NJ];
+            float scale[U];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (r0 + 4 * g + i < A.group) score = fmaxf(score, ((float)acc[i] * unit[i]) * scale);
-            if (scale == INFINITY) score = INFINITY;  // the block holds a key that is not finite: it is not to be missed
-            if (!there) score = -INFINITY;
-            score = max_groups(score);
-            if (g == 0 && block < blocks) {
+            for (int u = 0; u < U; ++u) {
+                const bool there = (unsigned)phys[u] < (unsigned)A.c.num_blocks;
+                const uint8_t *s = A.c.sums + ((size_t)(there ? phys[u] : 0) * A.c.heads + head) * R::SUM;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    hi[u][j] = *reinterpret_cast<const i32x4 *>(s + 64 * j + 16 * g);
+                    lo[u][j] = *reinterpret_cast<const i32x4 *>(s + D + 64 * j + 16 * g);
+                }
+                scale[u] = *reinterpret_cast<const float *>(s + 2 * D);
+                if (!there) scale[u] = -1.f;  // (a mark: no scale is negative)
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int block = j0 + 16 * W * u + row;
+                i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos8[j], hi[u][j], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg8[j], lo[u][j], acc, 0, 0, 0);
+                }
+                float score = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float mine = ((float)acc[i] * unit[i]) * scale[u];
+                    score = fmaxf(score, r0 + 4 * g + i < A.group ? mine : -INFINITY);
+                }
+                score = scale[u] == INFINITY ? INFINITY : scale[u] < 0.f ? -INFINITY : score;  // a key that is not finite is not to be missed; no block
+                score = max_groups(score);
                 uint32_t key = score_key(score);
-                if (r0) key = max(key, keys[block]);
-                if (block < A.first || block >= blocks - A.recent) key = 0xffffffffu;
-                keys[block] = key;
+                if (g == 0 && block < blocks) {
+                    if (r0) key = max(key, keys[block]);
+                    keys[block] = key;
+                    if (r0 + 16 >= A.group && block >= free_from && block < free_to) low = min(low, key), high = max(high, key);
+                }
             }
         }
     }
+    if (g == 0 && low <= high) {
+        atomicMin(&least, low);
+        atomicMax(&most_key, high);
+    }
     __syncthreads();
-    // The key of the block that is the top-th, and how many blocks at that key are wanted.
+    // The key of the last block that is wanted, as its difference from the least, and how many at that key are.
+    const uint32_t base = least;
+    int want = A.top - A.first - A.recent;
     uint32_t prefix = 0, mask = 0;
-    int want = A.top;
+    if (want > 0) {
+        const uint32_t range = most_key - base;
+        int at = range ? max(24 - __builtin_clz(range), 0) : 0;
 #pragma unroll 1
-    for (int at = 24; at >= 0; at -= 8) {
-        for (int i = tid; i < 256; i += T) hist[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < blocks; j += T) {
-            const uint32_t key = keys[j];
-            if ((key & mask) == prefix) atomicAdd(&hist[key >> at & 255], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {  // the bins from the top, four a lane
-            uint32_t h[4], mine = 0;
+        for (int pass = 0; pass < 4; ++pass) {
+            uint32_t *bins = hist[pass];
+            for (int j = free_from + tid; j < free_to; j += T) {
+                const uint32_t key = keys[j] - base;
+                if ((key & mask) == prefix) atomicAdd(&bins[key >> at & 255], 1u);
+            }
+            __syncthreads();
+            uint32_t h[4], mine = 0;  // the bins from the top, four a lane
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                h[i] = hist[255 - 4 * lane - i];
+                h[i] = bins[255 - 4 * lane - i];
                 mine += h[i];
             }
             uint32_t upto = mine;
@@ -1853,24 +1877,30 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
                 const uint32_t u = __shfl_up(upto, d);
                 if (lane >= d) upto += u;
             }
-            uint32_t over = upto - mine;
+            uint32_t over = upto - mine, bin = 0, left = 0;
+            bool here = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (over < (uint32_t)want && over + h[i] >= (uint32_t)want) found[0] = 255 - 4 * lane - i, found[1] = want - (int)over;
+                if (over < (uint32_t)want && over + h[i] >= (uint32_t)want) here = true, bin = 255 - 4 * lane - i, left = (uint32_t)want - over;
                 over += h[i];
             }
+            const int who = __builtin_ctzll(__ballot(here));
+            prefix |= (uint32_t)__builtin_amdgcn_readlane((int)bin, who) << at;
+            want = __builtin_amdgcn_readlane((int)left, who);
+            mask |= 255u << at;
+            if (at == 0) break;
+            at = max(at - 8, 0);  // (the last pass may look at bits that are settled: they are the same in all that are left)
         }
-        __syncthreads();
-        prefix |= (uint32_t)found[0] << at;
-        mask |= 255u << at;
-        want = found[1];
     }
-    // A thread's run of blocks: how many it has over the key and at it, then where its own go.
+    // A thread's run of blocks: how many of them are in, or at the key, then where its own go.
+    const int wanted = A.top - A.first - A.recent;
+    auto kind = [&](int j) { return j < free_from || j >= free_to ? 2 : wanted == 0 ? 0 : keys[j] - base > prefix ? 2 : keys[j] - base == prefix ? 1 : 0; };
     const int per = (blocks + T - 1) / T, from = min(tid * per, blocks), to = min(from + per, blocks);
     int over = 0, equal = 0;
     for (int j = from; j < to; ++j) {
-        over += keys[j] > prefix;
-        equal += keys[j] == prefix;
+        const int k = kind(j);
+        over += k == 2;
+        equal += k == 1;
     }
     int over_upto = over, equal_upto = equal;
 #pragma unroll
@@ -1883,11 +1913,10 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
     int o = over_upto - over, q = equal_upto - equal;
     for (int w = 0; w < wave; ++w) o += above[w], q += at_key[w];
     for (int j = from; j < to; ++j) {
-        const uint32_t key = keys[j];
-        const bool eq = key == prefix;
-        if (key > prefix || (eq && q < want)) out[o + min(q, want)] = j;
-        o += key > prefix;
-        q += eq;
+        const int k = kind(j);
+        if (k == 2 || (k == 1 && q < want)) out[o + min(q, want)] = j;
+        o += k == 2;
+        q += k == 1;
     }
 }
 
@@ -1900,8 +1929,8 @@ pg_status with_width(int D, F f) {
 
 // Runs that a row tile's keys are divided in: as many as fill the chip with workgroups, none shorter than a tile of 64
 // tokens a wavefront.
-size_t pick_splits(const pg_ctx *ctx, int D, size_t tiles, size_t tokens) {
-    const size_t fill = (size_t)ctx->num_cu * (D == 256 ? 1 : 2);  // what runs at once
+size_t pick_splits(const pg_ctx *ctx, size_t tiles, size_t tokens) {
+    const size_t fill = (size_t)ctx->num_cu * 2;  // what runs at once
     size_t splits = tiles ? fill / tiles : 1;
     const size_t most = (tokens + 255) / 256;
     if (splits > most) splits = most;
@@ -1920,7 +1949,7 @@ plan plan_for(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t units, size_t uni
     p.tiles = units * c->heads * p.row_tiles;
     p.wide = p.row_tiles < PROMPT_TILES ? 0 : 8;
     const size_t workgroups = p.wide ? units * c->heads * ((p.row_tiles + p.wide - 1) / p.wide) : p.tiles;
-    p.splits = pick_splits(ctx, c->D, workgroups, tokens);
+    p.splits = pick_splits(ctx, workgroups, tokens);
     p.bytes = p.splits > 1 ? p.tiles * p.splits * (p.rows * (size_t)c->D + 32) * sizeof(float) : 0;
     return p;
 }

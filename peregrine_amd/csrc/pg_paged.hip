@@ -364,8 +364,7 @@ __global__ __launch_bounds__(256) void kv4_summarise_kernel(kv4_batch ba, kv4_vi
             }
             if (lane * 8 + i < c.head_dim) most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+        most = over_wave(most, kv4_max{});
         bad = __ballot(bad) != 0;
         const float r = bad || most < 7.88860905e-31f ? 0.f : 1.0f / most * 127.f;  // 2^-100
         uint32_t h4[2] = {0, 0}, l4[2] = {0, 0};
