@@ -343,15 +343,24 @@ __global__ __launch_bounds__(256) void kv4_summarise_kernel(kv4_batch ba, kv4_vi
 #pragma unroll
         for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
         bool bad = false;
-        for (int j = group; j < count; j += G) {
-            const uint32_t codes = *reinterpret_cast<const uint32_t *>(rec + (size_t)j * R::ROW + lane * 4), m = meta[j];
-            const float z = kv4_z(m), d = kv4_d(m);
-            bad |= !(d == d);
+        for (int j0 = group; j0 < count; j0 += 8 * G) {  // eight tokens' loads go out together
+            uint32_t codes[8], m[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = d * ((float)((codes >> (4 * i)) & 15) - 7.5f) + z;
-                lo[i] = fminf(lo[i], x);
-                hi[i] = fmaxf(hi[i], x);
+            for (int u = 0; u < 8; ++u) {
+                const int j = min(j0 + u * G, count - 1);  // (the last again does no harm)
+                codes[u] = *reinterpret_cast<const uint32_t *>(rec + (size_t)j * R::ROW + lane * 4);
+                m[u] = meta[j];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float z = kv4_z(m[u]), d = kv4_d(m[u]);
+                bad |= !(d == d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = d * ((float)((codes[u] >> (4 * i)) & 15) - 7.5f) + z;
+                    lo[i] = fminf(lo[i], x);
+                    hi[i] = fmaxf(hi[i], x);
+                }
             }
         }
         float most = 0.f;
