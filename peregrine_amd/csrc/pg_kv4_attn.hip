@@ -2027,7 +2027,8 @@ PG_API pg_status pg_paged_kv4_attention_dev(pg_ctx *ctx, const pg_paged_kv4 *c, 
     if (tokens == 0 || batch == 0 || max_query == 0) return PG_OK;
     PG_CHECK_ARG(q_dev && query_start_dev && seq_lens_dev && block_table_dev && out_dev, "%s: null pointer", fn);
     PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
-    if (max_query > tokens) max_query = tokens;
+    PG_CHECK_ARG(max_query < (1ull << 31), "%s: %zu rows a request: out of range", fn, max_query);
+    // (Planned by max_query even where there are fewer rows than that: the scratch was asked for without their number.)
     const plan p = dense_plan(ctx, c, num_q_heads, batch, max_query, max_blocks);
     PG_CHECK_ARG(p.bytes == 0 || (scratch_dev && scratch_bytes >= p.bytes && ((uintptr_t)scratch_dev & 15) == 0),
                  "%s: scratch of %zu bytes, %zu are needed (16-byte aligned)", fn, scratch_bytes, p.bytes);

@@ -169,6 +169,19 @@ def test_device_forms_refuse_small_scratch_and_large_launches(host):
     host.lib.pg_paged_kv4_free(host.ctx, c)
 
 
+def test_scratch_does_not_depend_on_the_rows_there_are(host):
+    """max_query is a bound: a step of fewer rows in all takes the scratch that was reported for the bound."""
+    c = new_cache(host, 4096, 64, 2, 128)
+    buf = host.alloc(1 << 16)
+    for batch, most in ((100, 12), (100, 3), (1, 64), (30, 200)):
+        n = C.c_size_t()
+        host.ok("pg_paged_kv4_attention_scratch", host.ctx, c, 8, batch, most, 64, C.byref(n))
+        for tokens in (1, 4, 8, 64):
+            host.ok("pg_paged_kv4_attention_dev", host.ctx, c, buf, 1024, 128, 8, buf, buf, batch, tokens, most, buf, 64, 0.1, 1, 0, 0, 0.0, buf, n.value, buf)
+    assert status(host, "pg_paged_kv4_attention_dev", host.ctx, c, buf, 1024, 128, 8, buf, buf, 1, 1, 1 << 31, buf, 64, 0.1, 1, 0, 0, 0.0, buf, 1 << 40, buf) == EINVAL
+    host.lib.pg_paged_kv4_free(host.ctx, c)
+
+
 def test_a_step_is_captured_as_launches_alone(host):
     """Nothing of a step's device forms allocates, waits or copies."""
     c = new_cache(host, 4096, 64, 2, 128)
