@@ -172,6 +172,12 @@ __device__ __forceinline__ void settle_all() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// The power of two over a value step, 2^-117 at least, so that P_TOP over it is finite (steps are 2^-120 and more: such a one is
+// still taken as 2^7).
+__device__ __forceinline__ float step_over(float most) {
+    return __builtin_bit_cast(float, max((__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u, 10u << 23));
+}
+
 // The running softmax of a wavefront's 16 rows: O^T in the accumulators (this lane's row, channels of D / 4 in a run).
 template <int D>
 struct softmax_rows {
@@ -277,7 +283,7 @@ __device__ __forceinline__ void take_tile(bool masked, const kv_tile<D> &t, cons
             most = over_wave(most, kv4_max{});
             float fo = f;
             if (most > a.step) {
-                const float step = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+                const float step = step_over(most);
                 fo *= a.step / step;
                 a.step = step;
                 a.norm = P_TOP / step;
@@ -691,7 +697,7 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
             fo = (c & 3) == i ? fi : fo;
         }
         if (most > a.step) {
-            const float step = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+            const float step = step_over(most);
             fo *= a.step / step;
             a.step = step;
             a.norm = P_TOP / step;
@@ -1199,7 +1205,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
                 most = over_wave(most, kv4_max{});
                 float fs = 1.f;
                 if (most > step) {
-                    const float next = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+                    const float next = step_over(most);
                     fs = step / next;
                     step = next;
                     norm = P_TOP / next;
@@ -1556,7 +1562,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                 l *= f;
                 zsum *= f;
                 if (most > step) {
-                    const float next = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u);
+                    const float next = step_over(most);
                     f *= step / next;
                     step = next;
                     norm = P_TOP / next;

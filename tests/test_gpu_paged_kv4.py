@@ -310,6 +310,19 @@ def test_one_key_among_many_and_values_of_very_different_sizes(ctx):
         w.check(w.cache.attention(q, [0, 1], w.lens, w.table, hd ** -0.5), q, [1], hd ** -0.5, what="values")
 
 
+@pytest.mark.parametrize("hd,group,rows", [(64, 1, 1), (128, 4, 1), (128, 8, 1), (128, 16, 1), (64, 16, 1), (256, 4, 1), (256, 8, 1), (256, 16, 1), (64, 4, 20), (128, 4, 20), (256, 4, 20)])
+def test_values_near_the_smallest(ctx, hd, group, rows):
+    """Rows' steps at and just over the smallest there is (2^-120), zeros before and between them."""
+    n = 150
+    w = World(ctx, [n], 1, hd, 16, seed=hd + group + rows, poison=False)
+    for top in (1e-35, 2e-34):
+        v = (w.rng.standard_normal((n, 1, hd)) * np.exp(w.rng.uniform(-3, 0, (n, 1, 1))) * top / 3).astype(F)
+        v[:70], v[100] = 0, 0
+        w.put(w.keys(n), v, w.slots(0, np.arange(n)))
+        q = w.q(rows, group)
+        w.check(w.cache.attention(q, [0, rows], w.lens, w.table, hd ** -0.5), q, [rows], hd ** -0.5, what=f"values of {top}")
+
+
 class Step:
     """Device arrays of a step, for the `_dev` forms."""
 
