@@ -339,7 +339,7 @@ __device__ __forceinline__ void take_tile(bool masked, const kv_tile<D> &t, cons
 // with SELECTED the group's rows of one token) over one of `splits` runs of their keys, its four wavefronts every fourth
 // tile of 32 tokens.
 template <int D, bool CAP, bool SELECTED>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_rows_kernel(kv4_attn A) {
+__global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv4_rows_kernel(kv4_attn A) {
     using R = kv4_rec<D>;
     constexpr int STRIDE = D + 4;
     __shared__ float so[4][16][STRIDE];
