@@ -969,11 +969,10 @@ struct prompt_lds {
     alignas(16) float meta[2][4][64];  // key step, key z + d / 2, value step, value z
 };
 
-template <int D, int RT, int NW, bool CAP>
-__global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
-    static_assert(NW == 4 || NW == 8, "keys are staged by four wavefronts, values by the same or the other four");
+template <bool CAP>
+__global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
+    constexpr int D = 256, NW = 8, NJ = D / 64, NV = D / 16, NC = 2;
     using R = kv4_rec<D>;
-    constexpr int NJ = D / 64, NV = D / 16, NC = D == 256 ? 2 : 1, KW = D == 64 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     auto &lds = *reinterpret_cast<prompt_lds<D> *>(lds_raw);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
@@ -984,18 +983,18 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
     id /= A.c.heads;
     const int split = id % A.splits;
     id /= A.splits;
-    const int groups = (A.row_tiles + NW * RT - 1) / (NW * RT);
+    const int groups = (A.row_tiles + NW - 1) / NW;
     const int group = groups - 1 - id % groups;
     const int b = id / groups;
     const int shift = A.c.shift, bs = 1 << shift;
     const kv4_request rq = kv4_request_at(A.ba, b, shift);
     const int rows = min(min(rq.rows, A.max_query), A.ba.tokens - rq.first) * A.group;
-    const int r0 = group * 16 * NW * RT;
+    const int r0 = group * 16 * NW;
     if (r0 >= rows) return;
     const int behind = rq.len - rq.rows;
     auto pos_of = [&](int r) { return A.mask == PG_MASK_NONE ? rq.len - 1 : behind + r / A.group; };
-    const int mine = r0 + wave * 16 * RT;  // this wavefront's first row
-    const int last_row = min(r0 + 16 * NW * RT, rows) - 1, my_last = min(mine + 16 * RT, rows) - 1;
+    const int mine = r0 + wave * 16;  // this wavefront's first row
+    const int last_row = min(r0 + 16 * NW, rows) - 1, my_last = min(mine + 16, rows) - 1;
     const int group_low = pos_of(r0), group_high = pos_of(last_row);
     const int low_pos = pos_of(min(mine, last_row)), high_pos = mine < rows ? pos_of(my_last) : -1;
     const bool windowed = A.mask == PG_MASK_CAUSAL_SLIDING_WINDOW;
@@ -1008,7 +1007,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
     // A tile's codes on their way to LDS: a thread has one token's chunk of keys (4 threads a token), and words of values
     // for one half of the tile and one half of each word's channels.
     struct {
-        uint32_t k[NC][KW], v[8][NC], km, vm;
+        uint4 k[NC];
+        uint32_t v[8][NC], km, vm;
     } st;
     const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
     auto first_of = [&](int tile) { return 64 * (tile < sink_tiles ? tile : tile - sink_tiles + near); };
@@ -1020,34 +1020,26 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
         return A.c.data + ((size_t)phys * A.c.heads + head) * R::bytes(shift);
     };
     const int k_token = tid >> 2, k_chunk = tid & 3, v_half = wave & 1, v_part = wave >> 1 & 1;
-    const bool does_k = NW == 4 || wave < 4, does_v = NW == 4 || wave >= 4;
+    const bool does_k = wave < 4;
     auto fetch = [&](int tile) {
         if (does_k) {
-        int at;
-        // (the wavefront's keys are one run: tokens 16 wave .. 16 wave + 15)
-        const uint8_t *rec = rec_of(wave, tile, at);
-        const uint8_t *kp = rec + (size_t)(at + (k_token & 15)) * R::ROW + k_chunk * (D == 64 ? 8 : 16);
+            int at;
+            // (the wavefront's keys are one run: tokens 16 wave .. 16 wave + 15)
+            const uint8_t *rec = rec_of(wave, tile, at);
+            const uint8_t *kp = rec + (size_t)(at + (k_token & 15)) * R::ROW + k_chunk * 16;
 #pragma unroll
-        for (int cc = 0; cc < NC; ++cc) {
-            if (D == 64) {
-                const uint2 x = *reinterpret_cast<const uint2 *>(kp);
-                st.k[cc][0] = x.x, st.k[cc][1] = x.y;
-            } else {
-                const uint4 x = *reinterpret_cast<const uint4 *>(kp + 64 * cc);
-                st.k[cc][0] = x.x, st.k[cc][1] = x.y, st.k[cc][KW - 2] = x.z, st.k[cc][KW - 1] = x.w;
+            for (int cc = 0; cc < NC; ++cc) st.k[cc] = *reinterpret_cast<const uint4 *>(kp + 64 * cc);
+            if (lane < 16) {
+                st.km = reinterpret_cast<const uint32_t *>(rec + R::k_meta(shift))[at + lane];
+                st.vm = reinterpret_cast<const uint32_t *>(rec + R::v_meta(shift))[at + lane];
             }
+            return;
         }
-        if (lane < 16) {
-            st.km = reinterpret_cast<const uint32_t *>(rec + R::k_meta(shift))[at + lane];
-            st.vm = reinterpret_cast<const uint32_t *>(rec + R::v_meta(shift))[at + lane];
-        }
-        }
-        if (does_v)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             int va;
             const uint8_t *vp = rec_of(2 * v_half + r, tile, va);
-            vp += R::v(shift) + (size_t)(va + 4 * g) * R::ROW + (D == 64 ? c >> 1 : c) * 4;
+            vp += R::v(shift) + (size_t)(va + 4 * g) * R::ROW + c * 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1055,32 +1047,31 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
         }
     };
     auto store = [&](int buf) {
-        // keys: product j of a run, lanes (chunk, token) in the order of the operand
         if (does_k) {
+            // keys: product j of a run, lanes (chunk, token) in the order of the operand
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const uint32_t x = st.k[j >> 1][2 * (j & 1)], y = st.k[j >> 1][2 * (j & 1) + 1];
-            *reinterpret_cast<i32x4 *>(&lds.k[buf][((wave * NJ + j) * 64 + 16 * k_chunk + (k_token & 15)) * 16]) =
-                i32x4{(int)(x & 0x0f0f0f0fu), (int)(x >> 4 & 0x0f0f0f0fu), (int)(y & 0x0f0f0f0fu), (int)(y >> 4 & 0x0f0f0f0fu)};
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t x = j & 1 ? st.k[j >> 1].z : st.k[j >> 1].x, y = j & 1 ? st.k[j >> 1].w : st.k[j >> 1].y;
+                *reinterpret_cast<i32x4 *>(&lds.k[buf][((wave * NJ + j) * 64 + 16 * k_chunk + (k_token & 15)) * 16]) =
+                    i32x4{(int)(x & 0x0f0f0f0fu), (int)(x >> 4 & 0x0f0f0f0fu), (int)(y & 0x0f0f0f0fu), (int)(y >> 4 & 0x0f0f0f0fu)};
+            }
+            if (lane < 16) {
+                const float d = kv4_d(st.km);
+                lds.meta[buf][0][16 * wave + lane] = d;
+                lds.meta[buf][1][16 * wave + lane] = fmaf(0.5f, d, kv4_z(st.km));
+                lds.meta[buf][2][16 * wave + lane] = kv4_d(st.vm);
+                lds.meta[buf][3][16 * wave + lane] = kv4_z(st.vm);
+            }
+            return;
         }
-        if (lane < 16) {
-            const float d = kv4_d(st.km);
-            lds.meta[buf][0][16 * wave + lane] = d;
-            lds.meta[buf][1][16 * wave + lane] = fmaf(0.5f, d, kv4_z(st.km));
-            lds.meta[buf][2][16 * wave + lane] = kv4_d(st.vm);
-            lds.meta[buf][3][16 * wave + lane] = kv4_z(st.vm);
-        }
-        }
-        if (!does_v) return;
         const f16x2 low_by = {(_Float16)32768.f, (_Float16)32768.f}, high_by = {(_Float16)2048.f, (_Float16)2048.f};
         const f16x2 centre = {(_Float16)(-7.5f * CODE), (_Float16)(-7.5f * CODE)};
 #pragma unroll
         for (int cc = 0; cc < NC; ++cc)
 #pragma unroll
-            for (int q = 0; q < (D == 64 ? 1 : 2); ++q) {
-                const int b2 = (D == 64 ? 1 : 2) * v_part + q;
-                uint32_t sel = 0x0c040c00u + 0x00010001u * b2;
-                if (D == 64) sel += (lane & 1) ? 0x00020002u : 0u;
+            for (int q = 0; q < 2; ++q) {
+                const int b2 = 2 * v_part + q;
+                const uint32_t sel = 0x0c040c00u + 0x00010001u * b2;
                 f16x8 even, odd;
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
@@ -1090,105 +1081,82 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
                     even[2 * h] = e[0], even[2 * h + 1] = e[1];
                     odd[2 * h] = o[0], odd[2 * h + 1] = o[1];
                 }
-                const int n = (D == 64 ? 0 : 8 * cc) + 2 * b2;
+                const int n = 8 * cc + 2 * b2;
                 *reinterpret_cast<f16x8 *>(&lds.v[buf][((v_half * NV + n) * 64 + lane) * 16]) = even;
                 *reinterpret_cast<f16x8 *>(&lds.v[buf][((v_half * NV + n + 1) * 64 + lane) * 16]) = odd;
             }
     };
     if (begin < end) fetch(begin);
 
-    q_rows<D> q[RT];
-    float c1[RT], sq[RT];
-    int row_pos[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int r = mine + 16 * t + c;
-        const bool live = r < rows;
-        load_q<D>(live ? A.q + (size_t)(rq.first + r / A.group) * A.q_token + (size_t)(head * A.group + r % A.group) * A.q_head : nullptr, A.c.head_dim, g, q[t]);
-        c1[t] = q[t].unit * A.scale * (CAP ? 1.f : LOG2E);
-        sq[t] = q[t].sum * c1[t];
-        row_pos[t] = live ? pos_of(r) : -1;
-    }
+    q_rows<D> q;
+    const int r = mine + c;
+    const bool live = r < rows;
+    load_q<D>(live ? A.q + (size_t)(rq.first + r / A.group) * A.q_token + (size_t)(head * A.group + r % A.group) * A.q_head : nullptr, A.c.head_dim, g, q);
+    const float c1 = q.unit * A.scale * (CAP ? 1.f : LOG2E);
+    const float sq = q.sum * c1;
+    const int row_pos = live ? pos_of(r) : -1;
     const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
-    f32x4 o[RT][NV];
-    float m[RT], l[RT], zsum[RT], step = 0.f, norm = 0.f;
-    bool set[RT];
+    f32x4 o[NV];
+    float m = 0.f, l = 0.f, zsum = 0.f, step = 0.f, norm = 0.f;
+    bool set = false;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-#pragma unroll
-        for (int n = 0; n < NV; ++n) o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        m[t] = l[t] = zsum[t] = 0.f;
-        set[t] = false;
-    }
+    for (int n = 0; n < NV; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    auto take = [&](auto masked_, const int (&run_pos)[4], int buf) {
-        constexpr bool MASKED = decltype(masked_)::value;
+    auto take = [&](bool masked, const int (&run_pos)[4], int buf) {
 #pragma unroll 1
         for (int w = 0; w < 2; ++w) {
-            float s[RT][8], dv[8], zv[8];
+            const int pos0 = w ? run_pos[2] : run_pos[0], pos1 = w ? run_pos[3] : run_pos[1];
+            float s[8], dv[8], zv[8];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int run = 2 * w + r;
-                const int key0 = run_pos[run] + 4 * g;
                 i32x4 k8[NJ];
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) k8[j] = *reinterpret_cast<const i32x4 *>(&lds.k[buf][((run * NJ + j) * 64 + lane) * 16]);
                 const f32x4 kd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][0][16 * run + 4 * g]), kw = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][1][16 * run + 4 * g]);
                 const f32x4 vd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][2][16 * run + 4 * g]), vz = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][3][16 * run + 4 * g]);
+                i32x4 hi = {q.sum_hi2, q.sum_hi2, q.sum_hi2, q.sum_hi2}, lo = {q.sum_lo, q.sum_lo, q.sum_lo, q.sum_lo};
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    i32x4 hi = {q[t].sum_hi2, q[t].sum_hi2, q[t].sum_hi2, q[t].sum_hi2}, lo = {q[t].sum_lo, q[t].sum_lo, q[t].sum_lo, q[t].sum_lo};
+                for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[2][j], hi, 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q[t].digit[2][j], hi, 0, 0, 0);
+                for (int j = 0; j < NJ; ++j) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[0][j], lo, 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) lo = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q[t].digit[0][j], lo, 0, 0, 0);
+                for (int i = 0; i < 4; ++i) hi[i] = (hi[i] << 8) + q.sum_hi1;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) hi[i] = (hi[i] << 8) + q[t].sum_hi1;
+                for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q.digit[1][j], hi, 0, 0, 0);
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) hi = __builtin_amdgcn_mfma_i32_16x16x64_i8(k8[j], q[t].digit[1][j], hi, 0, 0, 0);
-            #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = fmaf((float)hi[i], 256.f, (float)lo[i]);
-                        float y;
-                        if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(kd[i] * c1[t], x, kw[i] * sq[t]) * inv_cap), -m[t]);
-                        else y = fmaf(kd[i] * c1[t], x, fmaf(kw[i], sq[t], -m[t]));
-                        if (MASKED) {
-                            const int key = key0 + i, far = row_pos[t] - key;
-                            y = (far >= 0) & ((window < 0) | (far <= window) | (key < A.sinks)) ? y : -INFINITY;  // (no branch)
-                        }
-                        s[t][4 * r + i] = y;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const float x = fmaf((float)hi[i], 256.f, (float)lo[i]);
+                    float y;
+                    if (CAP) y = fmaf(cap_log2e, tanhf(fmaf(kd[i] * c1, x, kw[i] * sq) * inv_cap), -m);
+                    else y = fmaf(kd[i] * c1, x, fmaf(kw[i], sq, -m));
+                    s[4 * r + i] = y;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dv[4 * r + i] = vd[i], zv[4 * r + i] = vz[i];
             }
-            if (MASKED) {
-                // What lies behind the rows' last position, or in no block, may be anything, and so may masked tokens: their
-                // probabilities are 0 below whatever they are multiplied by.
+            if (masked) {
+                // What lies behind the rows' last position, or in no block, may be anything, and so may masked tokens.
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    bool any = false;
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) any |= s[t][i] != -INFINITY;
-                    dv[i] = any ? dv[i] : 0.f;
-                    zv[i] = any ? zv[i] : 0.f;
+                    const int key = (i < 4 ? pos0 : pos1) + 4 * g + (i & 3), far = row_pos - key;
+                    const bool seen = (far >= 0) & ((window < 0) | (far <= window) | (key < A.sinks));
+                    s[i] = seen ? s[i] : -INFINITY;
+                    dv[i] = seen ? dv[i] : 0.f;
+                    zv[i] = seen ? zv[i] : 0.f;
                 }
             }
-            float p[RT][8], pd[RT][8], sum[RT];
+            float p[8], pd[8], sum;
             uint32_t top;
             auto weigh = [&] {
                 top = 0;
+                sum = 0.f;
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    sum[t] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        p[t][i] = __builtin_amdgcn_exp2f(s[t][i]);
-                        sum[t] += p[t][i];
-                        pd[t][i] = p[t][i] * (dv[i] * norm);
-                        if (MASKED) pd[t][i] = s[t][i] == -INFINITY ? 0.f : pd[t][i];
-                        top = max(top, __builtin_bit_cast(uint32_t, pd[t][i]));
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(s[i]);
+                    sum += p[i];
+                    pd[i] = p[i] * (dv[i] * norm);
+                    top = max(top, __builtin_bit_cast(uint32_t, pd[i]));
                 }
             };
             weigh();
@@ -1196,8 +1164,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) steps = max(steps, __builtin_bit_cast(uint32_t, dv[i]));
             bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || steps > __builtin_bit_cast(uint32_t, step);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) off |= !set[t] || !(sum[t] < 1.2676506e30f);
+            off |= !set || !(sum < 1.2676506e30f);
             if (__ballot(off)) {
                 float most = 0.f;
 #pragma unroll
@@ -1210,51 +1177,43 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
                     step = next;
                     norm = P_TOP / next;
                 }
+                float at = s[0];
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    float at = s[t][0];
+                for (int i = 1; i < 8; ++i) at = fmaxf(at, s[i]);
+                at = max_groups(at);
+                float f = 1.f;
+                if (at > -INFINITY && (!set || at > 0.f)) {
+                    f = set ? __builtin_amdgcn_exp2f(-at) : 1.f;
+                    m += at;
+                    set = true;
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) at = fmaxf(at, s[t][i]);
-                    at = max_groups(at);
-                    float f = 1.f;
-                    if (at > -INFINITY && (!set[t] || at > 0.f)) {
-                        f = set[t] ? __builtin_amdgcn_exp2f(-at) : 1.f;
-                        m[t] += at;
-                        set[t] = true;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) s[t][i] -= at;
-                    }
-                    l[t] *= f;
-                    zsum[t] *= f;
-                    f *= fs;
-#pragma unroll
-                    for (int n = 0; n < NV; ++n) o[t][n] *= f;
+                    for (int i = 0; i < 8; ++i) s[i] -= at;
                 }
+                l *= f;
+                zsum *= f;
+                f *= fs;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) o[n] *= f;
                 weigh();
             }
-            f16x8 ph[RT], pl[RT];
+            f16x8 ph, pl;
             float minus = -1.f;
             asm("" : "+s"(minus));  // (not a subtraction, so that one instruction takes the f16 as it is)
+            l += sum;
+            float zs = 0.f;
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                l[t] += sum[t];
-                float zs = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    zs = MASKED && s[t][i] == -INFINITY ? zs : fmaf(p[t][i], zv[i], zs);
-                    ph[t][i] = (_Float16)pd[t][i];
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) pl[t][i] = (_Float16)fmaf((float)ph[t][i], minus, pd[t][i]);
-                zsum[t] += zs;
+            for (int i = 0; i < 8; ++i) {
+                zs = fmaf(p[i], zv[i], zs);
+                ph[i] = (_Float16)pd[i];
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pl[i] = (_Float16)fmaf((float)ph[i], minus, pd[i]);
+            zsum += zs;
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
                 const f16x8 v = *reinterpret_cast<const f16x8 *>(&lds.v[buf][((w * NV + n) * 64 + lane) * 16]);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[t], o[t][n], 0, 0, 0);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[t], o[t][n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[n], 0, 0, 0);
             }
         }
     };
@@ -1273,8 +1232,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
                 run_pos[r] = ok ? p : 0x7fffff00;
                 there &= ok;
             }
-            if (there && first + 63 <= low_pos && (!windowed || high_pos - first <= window)) take(std::false_type{}, run_pos, buf);
-            else take(std::true_type{}, run_pos, buf);
+            take(!there || first + 63 > low_pos || (windowed && high_pos - first > window), run_pos, buf);
         }
         if (tile + 1 < end) store(buf ^ 1);
         __syncthreads();
@@ -1282,32 +1240,36 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_prompt_kernel(kv4_attn A) {
 
     settle_all();
     const float back = step * (1.f / (P_TOP * CODE));
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int r = mine + 16 * t + c;
-        const float ls = over_groups(l[t]), zs = over_groups(zsum[t]);
-        if (r >= rows) continue;
-        float *out;
-        float by = 1.f;
-        if (A.splits > 1) {
-            const size_t tile = ((size_t)b * A.c.heads + head) * A.row_tiles + r / 16;
-            float *base = A.part + (tile * A.splits + split) * (16 * D + 32);
-            out = base + c * D;
-            if (g == 0) base[16 * D + c] = set[t] ? m[t] : ls == 0.f ? -INFINITY : 0.f, base[16 * D + 16 + c] = ls;
-        } else {
-            out = A.out + ((size_t)(rq.first + r / A.group) * A.q_heads + head * A.group + r % A.group) * A.c.head_dim;
-            by = ls == 0.f ? 0.f : 1.f / ls;
-        }
-        const int most = A.splits > 1 ? D : A.c.head_dim;
-        constexpr int RUN = D / 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                const int d = D == 256 ? 128 * (n >> 3) + 32 * g + 8 * i + (n & 7) : RUN * g + (D / 16) * i + n;
-                if (d < most) out[d] = fmaf(o[t][n][i], back, zs) * by;
-            }
+    const float ls = over_groups(l), zs = over_groups(zsum);
+    if (r >= rows) return;
+    float *out;
+    float by = 1.f;
+    if (A.splits > 1) {
+        const size_t tile = ((size_t)b * A.c.heads + head) * A.row_tiles + r / 16;
+        float *base = A.part + (tile * A.splits + split) * (16 * D + 32);
+        out = base + c * D;
+        if (g == 0) base[16 * D + c] = set ? m : ls == 0.f ? -INFINITY : 0.f, base[16 * D + 16 + c] = ls;
+    } else {
+        out = A.out + ((size_t)(rq.first + r / A.group) * A.q_heads + head * A.group + r % A.group) * A.c.head_dim;
+        by = ls == 0.f ? 0.f : 1.f / ls;
     }
+    const int most = A.splits > 1 ? D : A.c.head_dim;
+    const bool wide = (most & 3) == 0 && ((uintptr_t)out & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < NV; n += 4) {
+            const int d = 128 * (n >> 3) + 32 * g + 8 * i + (n & 7);
+            const float4 y = make_float4(fmaf(o[n][i], back, zs) * by, fmaf(o[n + 1][i], back, zs) * by, fmaf(o[n + 2][i], back, zs) * by, fmaf(o[n + 3][i], back, zs) * by);
+            if (wide) {
+                if (d < most) *reinterpret_cast<float4 *>(out + d) = y;
+            } else {
+                if (d < most) out[d] = y.x;
+                if (d + 1 < most) out[d + 1] = y.y;
+                if (d + 2 < most) out[d + 2] = y.z;
+                if (d + 3 < most) out[d + 3] = y.w;
+            }
+        }
 }
 
 // The same for heads up to 128 on 32 x 32 products: a wavefront has 32 rows, so each operand that it takes from LDS serves twice the
@@ -1986,7 +1948,7 @@ pg_status launch_rows(pg_ctx *ctx, const char *fn, const pg_paged_kv4 *c, kv4_at
                     return pg_launch(ctx, name, kernel, workgroups, dim3(threads), lds, A);
                 };
                 if constexpr (D == 256)
-                    PG_TRY(prompt("kv4_prompt_kernel", A.cap > 0.f ? kv4_prompt_kernel<D, 1, 8, true> : kv4_prompt_kernel<D, 1, 8, false>, sizeof(prompt_lds<D>), 512));
+                    PG_TRY(prompt("kv4_prompt_kernel", A.cap > 0.f ? kv4_prompt_kernel<true> : kv4_prompt_kernel<false>, sizeof(prompt_lds<D>), 512));
                 else
                     PG_TRY(prompt("kv4_prompt32_kernel", A.cap > 0.f ? kv4_prompt32_kernel<D, true> : kv4_prompt32_kernel<D, false>, sizeof(prompt32_lds<D>), 256));
                 return p.splits == 1 ? PG_OK : pg_launch(ctx, "kv4_join_kernel", kv4_join_kernel<D, 16, SELECTED>, join, block, 0, A);
