@@ -323,6 +323,18 @@ def test_values_near_the_smallest(ctx, hd, group, rows):
         w.check(w.cache.attention(q, [0, rows], w.lens, w.table, hd ** -0.5), q, [rows], hd ** -0.5, what=f"values of {top}")
 
 
+@pytest.mark.parametrize("batch,heads,group", [(140, 4, 4), (256, 3, 2), (257, 2, 8), (256, 3, 16), (65, 8, 20)])
+def test_more_requests_than_run_at_once(ctx, batch, heads, group):
+    """Requests are taken the longest first then; lengths that are equal, and none."""
+    hd = 64
+    lens = np.random.default_rng(batch + group).integers(0, 40, batch) * np.where(np.arange(batch) % 5 == 0, 4, 1)
+    lens[-1], lens[batch // 2] = 0, 150
+    w = World(ctx, [int(x) for x in lens], heads, hd, 16, seed=batch, poison=False)
+    rows = [int(min(x, 1)) for x in lens]
+    q = w.q(sum(rows), heads * group)
+    w.check(w.cache.attention(q, np.concatenate([[0], np.cumsum(rows)]), w.lens, w.table, hd ** -0.5), q, rows, hd ** -0.5)
+
+
 class Step:
     """Device arrays of a step, for the `_dev` forms."""
 
