@@ -54,6 +54,37 @@ __device__ __forceinline__ float over_groups(float v) { return over_halves(over_
 __device__ __forceinline__ int over_groups(int v) { return over_halves(over_rows(v, kv4_iadd{}), kv4_iadd{}); }
 __device__ __forceinline__ float max_groups(float v) { return over_halves(over_rows(v, kv4_max{}), kv4_max{}); }
 
+// N channels of a query row from channel d on, zeros where there is no row (x null) or channel.  wide: by 16 bytes, for rows that
+// are aligned and end at such a word -- every lane has a row or a part of one of its own, so that a load costs by the lines that it
+// touches and four times the bytes are nearly free (a wavefront of 32 rows of 128: 64 loads of 4 bytes took 20 us where a CU had
+// eight of them).  `some` is read where nothing is, so that no load stands behind a branch.
+struct query_rows {
+    const float *some;
+    int head_dim;
+    bool wide;
+};
+template <int N>
+__device__ __forceinline__ void take_channels(const query_rows &qr, const float *x, int d, float *a) {
+    if (qr.wide) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const bool there = x && d + i < qr.head_dim;
+            const float4 v = *reinterpret_cast<const float4 *>(there ? x + d + i : qr.some);
+            a[i] = there ? v.x : 0.f, a[i + 1] = there ? v.y : 0.f, a[i + 2] = there ? v.z : 0.f, a[i + 3] = there ? v.w : 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool there = x && d + i < qr.head_dim;
+            const float v = *(there ? x + d + i : qr.some);
+            a[i] = there ? v : 0.f;
+        }
+    }
+}
+__device__ __forceinline__ query_rows rows_of(const float *q, size_t q_token, size_t q_head, int head_dim) {
+    return {q, head_dim, (((uintptr_t)q | q_token * 4 | q_head * 4 | (size_t)head_dim * 4) & 15) == 0};
+}
+
 // First channel of the 16 that lane group g holds for the j-th product.
 template <int D>
 __device__ __forceinline__ constexpr int q_base(int j, int g) {
@@ -70,16 +101,17 @@ struct q_fixed {
 };
 // x: the row, or null (zeros).
 template <int D>
-__device__ __forceinline__ void fix_q(const float *x, int head_dim, int g, q_fixed<D> &r) {
+__device__ __forceinline__ void fix_q(const query_rows &qr, const float *x, int g, q_fixed<D> &r) {
     constexpr int NJ = D / 64;
-    float a[NJ][16];
+    float in[NJ][16], a[NJ][16];
     uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) take_channels<16>(qr, x, q_base<D>(j, g), in[j]);
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int d = q_base<D>(j, g) + 8 * (e >> 3) + 2 * (e & 3) + (e >> 2 & 1);
-            a[j][e] = x && d < head_dim ? x[d] : 0.f;
+            a[j][e] = in[j][8 * (e >> 3) + 2 * (e & 3) + (e >> 2 & 1)];
             top = max(top, __builtin_bit_cast(uint32_t, a[j][e]) & 0x7fffffffu);  // (of magnitudes the bits are in order, NaN last)
         }
     top = over_halves(over_rows(top, kv4_umax{}), kv4_umax{});
@@ -106,9 +138,9 @@ __device__ __forceinline__ int pick_digit(const int *y, uint32_t sel) {  // sel 
 __device__ __forceinline__ int sum_bytes(int x, int s) { return __builtin_amdgcn_sdot4(x, 0x01010101, s, false); }
 
 template <int D>
-__device__ __forceinline__ void load_q(const float *x, int head_dim, int g, q_rows<D> &r) {
+__device__ __forceinline__ void load_q(const query_rows &qr, const float *x, int g, q_rows<D> &r) {
     q_fixed<D> f;
-    fix_q<D>(x, head_dim, g, f);
+    fix_q<D>(qr, x, g, f);
     int s[3] = {0, 0, 0};
 #pragma unroll
     for (int j = 0; j < D / 64; ++j)
@@ -446,7 +478,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
     int tile = begin + wave;
     if (tile < end) fetch(tile, t);  // on its way while the queries are made ready
     q_rows<D> q;
-    load_q<D>(live ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr, A.c.head_dim, g, q);
+    load_q<D>(rows_of(A.q, A.q_token, A.q_head, A.c.head_dim), live ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr, g, q);
     const float c1 = q.unit * A.scale * (CAP ? 1.f : LOG2E), sq = q.sum * c1;
     const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
 
@@ -541,11 +573,11 @@ struct q_few {
 };
 
 template <int D, int HB>
-__device__ __forceinline__ void load_q_few(const float *x, int head_dim, int lane, q_few<D, HB> &r) {
+__device__ __forceinline__ void load_q_few(const query_rows &qr, const float *x, int lane, q_few<D, HB> &r) {
     constexpr int NJ = D / 64, SETS = HB == 4 ? 1 : 2;
     const int g = lane >> 4, row = lane & 15;
     q_fixed<D> f;
-    fix_q<D>(x, head_dim, g, f);
+    fix_q<D>(qr, x, g, f);
     // HB = 4: rows 0-3 the high digit, 4-7 the middle one, 8-11 the low one, 12-15 nothing
     // HB = 8: rows 0-7 high, 8-15 middle; second set: rows 0-7 low, 8-15 nothing
     const int digit0 = HB == 4 ? 2 - (row >> 2) : 2 - (row >> 3);
@@ -889,8 +921,8 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
     int row_pos[4];
     {
         const int r = HB == 4 ? c & 3 : c & 7;
-        load_q_few<D, HB>(r < rows ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr,
-                          A.c.head_dim, lane, q);
+        load_q_few<D, HB>(rows_of(A.q, A.q_token, A.q_head, A.c.head_dim), r < rows ? A.q + (size_t)(rq.first + token_of(r)) * A.q_token + (size_t)(head * A.group + (SELECTED ? r : r % A.group)) * A.q_head : nullptr,
+                          lane, q);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int mine = HB == 4 ? i : 4 * (g & 1) + i;
@@ -1113,7 +1145,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
     q_rows<D> q;
     const int r = mine + c;
     const bool live = r < rows;
-    load_q<D>(live ? A.q + (size_t)(rq.first + r / A.group) * A.q_token + (size_t)(head * A.group + r % A.group) * A.q_head : nullptr, A.c.head_dim, g, q);
+    load_q<D>(rows_of(A.q, A.q_token, A.q_head, A.c.head_dim), live ? A.q + (size_t)(rq.first + r / A.group) * A.q_token + (size_t)(head * A.group + r % A.group) * A.q_head : nullptr, g, q);
     const float c1 = q.unit * A.scale * (CAP ? 1.f : LOG2E);
     const float sq = q.sum * c1;
     const int row_pos = live ? pos_of(r) : -1;
@@ -1431,14 +1463,16 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
     const bool live = r < rows;
     {
         const float *x = live ? A.q + (size_t)(rq.first + r / A.group) * A.q_token + (size_t)(head * A.group + r % A.group) * A.q_head : nullptr;
-        float a[KS][8], sum = 0.f;
+        const query_rows qr = rows_of(A.q, A.q_token, A.q_head, A.c.head_dim);
+        float in[KS][8], a[KS][8], sum = 0.f;
         uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) take_channels<8>(qr, x, 8 * (2 * k + half), in[k]);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int d = 8 * (2 * k + half) + (e >> 1) + 4 * (e & 1);
-                a[k][e] = x && d < A.c.head_dim ? x[d] : 0.f;
+                a[k][e] = in[k][(e >> 1) + 4 * (e & 1)];
                 top = max(top, __builtin_bit_cast(uint32_t, a[k][e]) & 0x7fffffffu);
             }
         top = over_halves(top, kv4_umax{});
@@ -1733,17 +1767,13 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
     for (int i = tid; i < 1024; i += T) hist[i >> 8][i & 255] = 0;
     if (tid == 0) least = 0xffffffffu, most_key = 0;
     float a[NJ][16];
+    const query_rows qr = rows_of(A.q, A.q_token, A.q_head, A.c.head_dim);
     auto load_rows = [&](int r0) {
         const float *x = r0 + row < A.group ? A.q + (size_t)token * A.q_token + (size_t)(head * A.group + r0 + row) * A.q_head : nullptr;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int d = 64 * j + 16 * g + e;
-                a[j][e] = x && d < A.c.head_dim ? x[d] : 0.f;
-            }
+        for (int j = 0; j < NJ; ++j) take_channels<16>(qr, x, 64 * j + 16 * g, a[j]);
     };
-    load_rows(0);
+    if (A.ba.max_blocks > A.top) load_rows(0);  // (or no request has more blocks than are wanted)
     int *out = A.selected + ((size_t)token * A.c.heads + head) * A.top;
     kv4_request rq;
     const int b = kv4_find(A.ba, token, shift, rq);
@@ -1918,10 +1948,13 @@ pg_status with_width(int D, F f) {
 }
 
 // Runs that a row tile's keys are divided in: as many as fill the chip with workgroups, none shorter than a tile of 64
-// tokens a wavefront.
-size_t pick_splits(const pg_ctx *ctx, size_t tiles, size_t tokens) {
+// tokens a wavefront.  Not at all where a workgroup alone takes less longer than the joining launch does: one row of two key heads
+// of 128 at 512 / 1024 / 1536 / 2048 tokens takes 9.0 / 11.3 / 14.4 / 17.1 us alone and 13.4 to 13.9 divided (heads of 256 at
+// 1024: 19.6 and 17.9).  Prompts, with more work a token: 23 x 16 rows at 512 / 1024 tokens 36 / 61 alone, 30 / 33 divided.
+size_t pick_splits(const pg_ctx *ctx, size_t tiles, size_t tokens, bool prompts, size_t D) {
     const size_t fill = (size_t)ctx->num_cu * 2;  // what runs at once
     size_t splits = tiles ? fill / tiles : 1;
+    if (!prompts && tokens * std::max<size_t>(D, 128) <= 1024 * 128) return 1;
     const size_t most = (tokens + 255) / 256;
     if (splits > most) splits = most;
     return splits < 1 ? 1 : splits;
@@ -1939,12 +1972,13 @@ plan plan_for(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t units, size_t uni
     p.tiles = units * c->heads * p.row_tiles;
     p.wide = p.row_tiles < PROMPT_TILES ? 0 : 8;
     const size_t workgroups = p.wide ? units * c->heads * ((p.row_tiles + p.wide - 1) / p.wide) : p.tiles;
-    p.splits = pick_splits(ctx, workgroups, tokens);
+    p.splits = pick_splits(ctx, workgroups, tokens, p.wide, (size_t)c->D);
     p.bytes = p.splits > 1 ? p.tiles * p.splits * (p.rows * (size_t)c->D + 32) * sizeof(float) : 0;
     return p;
 }
-plan dense_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t max_query, size_t max_blocks) {
-    return plan_for(ctx, c, batch, max_query * (num_q_heads / c->heads), max_blocks * c->block_size);
+// (seen: tokens that any row sees, where a window says so.  Fewer runs need no more scratch than was reported without it.)
+plan dense_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t max_query, size_t max_blocks, size_t seen = SIZE_MAX) {
+    return plan_for(ctx, c, batch, max_query * (num_q_heads / c->heads), std::min(max_blocks * c->block_size, seen));
 }
 plan selected_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t tokens, size_t top) {
     return plan_for(ctx, c, tokens, num_q_heads / c->heads, top * c->block_size);
@@ -2020,7 +2054,9 @@ PG_API pg_status pg_paged_kv4_attention_dev(pg_ctx *ctx, const pg_paged_kv4 *c, 
     PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
     PG_CHECK_ARG(max_query < (1ull << 31), "%s: %zu rows a request: out of range", fn, max_query);
     // (Planned by max_query even where there are fewer rows than that: the scratch was asked for without their number.)
-    const plan p = dense_plan(ctx, c, num_q_heads, batch, max_query, max_blocks);
+    // What a tile of rows sees behind its window and of the sinks, in whole tiles of keys.
+    const size_t seen = mask_kind == PG_MASK_CAUSAL_SLIDING_WINDOW && window < (1u << 30) && sink_tokens < (1u << 30) ? window + max_query + sink_tokens + 128 : SIZE_MAX;
+    const plan p = dense_plan(ctx, c, num_q_heads, batch, max_query, max_blocks, seen);
     PG_CHECK_ARG(p.bytes == 0 || (scratch_dev && scratch_bytes >= p.bytes && ((uintptr_t)scratch_dev & 15) == 0),
                  "%s: scratch of %zu bytes, %zu are needed (16-byte aligned)", fn, scratch_bytes, p.bytes);
     c->touch(ctx);
@@ -2074,7 +2110,7 @@ PG_API pg_status pg_paged_kv4_attention_selected_dev(pg_ctx *ctx, const pg_paged
     if (tokens == 0 || batch == 0) return PG_OK;
     PG_CHECK_ARG(q_dev && query_start_dev && seq_lens_dev && block_table_dev && selected_dev && out_dev, "%s: null pointer", fn);
     PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
-    const plan p = selected_plan(ctx, c, num_q_heads, tokens, top_k);
+    const plan p = selected_plan(ctx, c, num_q_heads, tokens, std::min(top_k, max_blocks));  // (no more scratch than was reported without the table)
     PG_CHECK_ARG(p.bytes == 0 || (scratch_dev && scratch_bytes >= p.bytes && ((uintptr_t)scratch_dev & 15) == 0),
                  "%s: scratch of %zu bytes, %zu are needed (16-byte aligned)", fn, scratch_bytes, p.bytes);
     c->touch(ctx);
