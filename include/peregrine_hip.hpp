@@ -731,5 +731,123 @@ private:
 };
 
 }  // namespace huffman
+
+namespace paged {
+
+using llama::AttentionMask;
+
+// Lengths and block tables of `batch` requests over a pool of blocks (pg_block_tables_*; no counterpart in the reference).
+class BlockTables {
+public:
+    struct Step {
+        std::vector<int32_t> query_start, granted, slots;
+    };
+    BlockTables(const GpuContext &gpu, size_t batch, size_t num_blocks, size_t block_size, size_t max_blocks)
+        : seq_lens(batch, 0), table(batch * max_blocks, -1), free_list(num_blocks), free_count((int32_t)num_blocks), gpu_(&gpu), block_size_(block_size), max_blocks_(max_blocks) {
+        for (size_t i = 0; i < num_blocks; ++i) free_list[i] = (int32_t)(num_blocks - 1 - i);  // block 0 is handed out first
+    }
+    // Room for new_lens[b] more tokens of request b.
+    Step extend(const std::vector<int32_t> &new_lens) {
+        if (new_lens.size() != seq_lens.size()) throw Panic(PG_EINVAL, "BlockTables::extend: new_lens.len() != batch");
+        size_t tokens = 0;
+        for (int32_t n : new_lens) tokens += n > 0 ? (size_t)n : 0;
+        Step s{std::vector<int32_t>(seq_lens.size() + 1), std::vector<int32_t>(seq_lens.size()), std::vector<int32_t>(tokens)};
+        std::vector<int32_t> lens(seq_lens.size());
+        int32_t left = 0;
+        check(pg_block_tables_extend(gpu_->raw(), seq_lens.data(), new_lens.data(), seq_lens.size(), block_size_, free_list.data(), &free_count, free_list.size(), table.data(),
+                                     max_blocks_, lens.data(), &left, s.query_start.data(), s.granted.data(), s.slots.data(), tokens),
+              "BlockTables::extend");
+        seq_lens = std::move(lens);
+        free_count = left;
+        return s;
+    }
+    // The blocks of the requests with done[b] != 0 back to the pool.
+    void release(const std::vector<int32_t> &done) {
+        if (done.size() != seq_lens.size()) throw Panic(PG_EINVAL, "BlockTables::release: done.len() != batch");
+        check(pg_block_tables_release(gpu_->raw(), done.data(), seq_lens.data(), seq_lens.size(), block_size_, table.data(), max_blocks_, free_list.data(), &free_count,
+                                      free_list.size()),
+              "BlockTables::release");
+    }
+    size_t max_blocks() const { return max_blocks_; }
+    std::vector<int32_t> seq_lens, table, free_list;
+    int32_t free_count;
+
+private:
+    const GpuContext *gpu_;
+    size_t block_size_, max_blocks_;
+};
+
+// A key/value cache in 4 bits that many requests share (pg_paged_kv4_*).  query_start, seq_lens and table as a step has them.
+class PagedKV4Cache {
+public:
+    PagedKV4Cache(const GpuContext &gpu, size_t num_blocks, size_t block_size, size_t num_kv_heads, size_t head_dim)
+        : num_kv_heads(num_kv_heads), head_dim(head_dim), gpu_(&gpu) {
+        check(pg_paged_kv4_create(gpu.raw(), num_blocks, block_size, num_kv_heads, head_dim, &h_), "PagedKV4Cache::new");
+    }
+    ~PagedKV4Cache() { pg_paged_kv4_free(gpu_->raw(), h_); }
+    PagedKV4Cache(const PagedKV4Cache &) = delete;
+    PagedKV4Cache &operator=(const PagedKV4Cache &) = delete;
+    void append(const std::vector<float> &k, const std::vector<float> &v, const std::vector<int32_t> &slots) {
+        if (k.size() != slots.size() * row() || v.size() != k.size()) throw Panic(PG_EINVAL, "PagedKV4Cache::append: slice lengths");
+        check(pg_paged_kv4_append(gpu_->raw(), h_, k.data(), v.data(), slots.size(), slots.data()), "PagedKV4Cache::append");
+    }
+    std::pair<std::vector<float>, std::vector<float>> read(const std::vector<int32_t> &slots) const {
+        std::vector<float> k(slots.size() * row()), v(k.size());
+        check(pg_paged_kv4_read(gpu_->raw(), h_, slots.data(), slots.size(), k.data(), v.data()), "PagedKV4Cache::read");
+        return {std::move(k), std::move(v)};
+    }
+    std::vector<float> attention(const std::vector<float> &q, size_t num_q_heads, const std::vector<int32_t> &query_start, const std::vector<int32_t> &seq_lens,
+                                 const std::vector<int32_t> &table, float scale, const AttentionMask &mask, float logit_cap) const {
+        const size_t tokens = rows(q, num_q_heads, query_start, seq_lens, table, "PagedKV4Cache::attention");
+        std::vector<float> out(q.size());
+        check(pg_paged_kv4_attention(gpu_->raw(), h_, q.data(), num_q_heads, query_start.data(), seq_lens.data(), seq_lens.size(), tokens, table.data(), width(seq_lens, table),
+                                     scale, mask.kind, mask.window, mask.sink_tokens, logit_cap, out.data()),
+              "PagedKV4Cache::attention");
+        return out;
+    }
+    void summarise(const std::vector<int32_t> &query_start, const std::vector<int32_t> &seq_lens, const std::vector<int32_t> &table) {
+        check_step(query_start, seq_lens, table, "PagedKV4Cache::summarise");
+        check(pg_paged_kv4_summarise(gpu_->raw(), h_, query_start.data(), seq_lens.data(), seq_lens.size(), table.data(), width(seq_lens, table)), "PagedKV4Cache::summarise");
+    }
+    std::vector<int32_t> select(const std::vector<float> &q, size_t num_q_heads, const std::vector<int32_t> &query_start, const std::vector<int32_t> &seq_lens,
+                                const std::vector<int32_t> &table, size_t top_k, size_t first_blocks, size_t recent_blocks) const {
+        const size_t tokens = rows(q, num_q_heads, query_start, seq_lens, table, "PagedKV4Cache::select");
+        std::vector<int32_t> out(tokens * num_kv_heads * top_k);
+        check(pg_paged_kv4_select(gpu_->raw(), h_, q.data(), num_q_heads, query_start.data(), seq_lens.data(), seq_lens.size(), tokens, table.data(), width(seq_lens, table), top_k,
+                                  first_blocks, recent_blocks, out.data()),
+              "PagedKV4Cache::select");
+        return out;
+    }
+    std::vector<float> attention_selected(const std::vector<float> &q, size_t num_q_heads, const std::vector<int32_t> &query_start, const std::vector<int32_t> &seq_lens,
+                                          const std::vector<int32_t> &table, const std::vector<int32_t> &selected, size_t top_k, float scale, float logit_cap) const {
+        const size_t tokens = rows(q, num_q_heads, query_start, seq_lens, table, "PagedKV4Cache::attention_selected");
+        if (selected.size() != tokens * num_kv_heads * top_k) throw Panic(PG_EINVAL, "PagedKV4Cache::attention_selected: selected.len() != tokens * num_kv_heads * top_k");
+        std::vector<float> out(q.size());
+        check(pg_paged_kv4_attention_selected(gpu_->raw(), h_, q.data(), num_q_heads, query_start.data(), seq_lens.data(), seq_lens.size(), tokens, table.data(),
+                                              width(seq_lens, table), selected.data(), top_k, scale, logit_cap, out.data()),
+              "PagedKV4Cache::attention_selected");
+        return out;
+    }
+    pg_paged_kv4 *handle() const { return h_; }
+    const size_t num_kv_heads, head_dim;
+
+private:
+    size_t row() const { return num_kv_heads * head_dim; }
+    static size_t width(const std::vector<int32_t> &seq_lens, const std::vector<int32_t> &table) { return seq_lens.empty() ? 1 : table.size() / seq_lens.size(); }
+    static void check_step(const std::vector<int32_t> &query_start, const std::vector<int32_t> &seq_lens, const std::vector<int32_t> &table, const char *what) {
+        if (query_start.size() != seq_lens.size() + 1 || (seq_lens.empty() ? !table.empty() : table.empty() || table.size() % seq_lens.size()))
+            throw Panic(PG_EINVAL, std::string(what) + ": query_start / table lengths");
+    }
+    size_t rows(const std::vector<float> &q, size_t num_q_heads, const std::vector<int32_t> &query_start, const std::vector<int32_t> &seq_lens, const std::vector<int32_t> &table,
+                const char *what) const {
+        check_step(query_start, seq_lens, table, what);
+        if (num_q_heads == 0 || q.size() % (num_q_heads * head_dim)) throw Panic(PG_EINVAL, std::string(what) + ": q.len() % (num_q_heads * head_dim) != 0");
+        return q.size() / (num_q_heads * head_dim);
+    }
+    const GpuContext *gpu_;
+    pg_paged_kv4 *h_ = nullptr;
+};
+
+}  // namespace paged
 }  // namespace peregrine
 #endif  // PEREGRINE_HIP_HPP

@@ -706,3 +706,12 @@ def test_prompts_leave_out_what_is_no_block_and_read_nothing_behind(ctx, hd, hea
     one = World.__new__(World)
     one.__dict__.update(w.__dict__, lens=w.lens[:1], table=w.table[:1])
     one.check(got[: rows[0]], q[: rows[0]], rows[:1], hd ** -0.5, only=lambda t, h: [j for j in range(w.width) if j not in gone], what="no block")
+
+
+def test_cpp_host_mirror():
+    """tests/cpp/paged_kv4.cpp over the C++ mirror's namespace paged; built by __graft_entry__.build()."""
+    import os
+    import subprocess
+    binary = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "_build", "paged_kv4")
+    r = subprocess.run([binary], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "OK: all checks passed" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
