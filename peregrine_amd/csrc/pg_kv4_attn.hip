@@ -1749,6 +1749,109 @@ __device__ __forceinline__ uint32_t score_key(float s) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// 16 query rows as the operands of the scores' products (rows of the product are x where positive and x where negative), with the
+// values of the units of this lane's four rows of a result.
+template <int D>
+struct pick_rows {
+    i32x4 pos8[D / 64], neg8[D / 64];
+    float unit[4];
+};
+template <int D>
+__device__ __forceinline__ void round_rows(const float (&a)[D / 64][16], int g, pick_rows<D> &r) {
+    constexpr int NJ = D / 64;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, __builtin_bit_cast(uint32_t, a[j][e]) & 0x7fffffffu);  // (of magnitudes the bits are in order, NaN last)
+    top = over_halves(over_rows(top, kv4_umax{}), kv4_umax{});
+    const bool bad = top >= 0x7f800000u;
+    const float most = __builtin_bit_cast(float, top);
+    const float by = bad || most < 7.88860905e-31f ? 0.f : 1.0f / most * 127.f;  // 2^-100
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint32_t up = 0, down = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = bad ? 0 : (int)rintf(a[j][4 * w + e] * by);
+                up |= (uint32_t)(max(v, 0) & 255) << (8 * e);
+                down |= (uint32_t)(min(v, 0) & 255) << (8 * e);
+            }
+            r.pos8[j][w] = (int)up;
+            r.neg8[j][w] = (int)down;
+        }
+    // a lane's four rows of the result are rows 4 g + i
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.unit[i] = __shfl(bad ? 0.f : most * (1.0f / 127.f), 4 * g + i);
+}
+// This lane's part of a block's summary.
+template <int D>
+struct pick_block {
+    i32x4 hi[D / 64], lo[D / 64];
+    float scale;  // -1 (a mark: no scale is negative) where there is no block
+};
+template <int D>
+__device__ __forceinline__ void load_summary(const kv4_view &c, int phys, int head, int g, pick_block<D> &s) {
+    using R = kv4_rec<D>;
+    const bool there = (unsigned)phys < (unsigned)c.num_blocks;
+    const uint8_t *at = c.sums + ((size_t)(there ? phys : 0) * c.heads + head) * R::SUM;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+        s.hi[j] = *reinterpret_cast<const i32x4 *>(at + 64 * j + 16 * g);
+        s.lo[j] = *reinterpret_cast<const i32x4 *>(at + D + 64 * j + 16 * g);
+    }
+    s.scale = *reinterpret_cast<const float *>(at + 2 * D);
+    if (!there) s.scale = -1.f;
+}
+// Scores of this lane's four rows: whole numbers and two f32 products.
+template <int D>
+__device__ __forceinline__ void score_rows(const pick_rows<D> &r, const pick_block<D> &s, float (&score)[4]) {
+    i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.pos8[j], s.hi[j], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.neg8[j], s.lo[j], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) score[i] = ((float)acc[i] * r.unit[i]) * s.scale;
+}
+// ... of a block that is to be taken by itself: a key that is not finite is not to be missed, no block never taken.
+__device__ __forceinline__ float score_of(float score, float scale) { return scale == INFINITY ? INFINITY : scale < 0.f ? -INFINITY : score; }
+
+// Of 256 bins, from the top: the one in which the want-th entry lies, and its number in that bin.  (Four bins a lane.)
+__device__ __forceinline__ void bin_of(const uint32_t *bins, uint32_t want, int lane, uint32_t &bin, uint32_t &left) {
+    uint32_t h[4], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[i] = bins[255 - 4 * lane - i];
+        mine += h[i];
+    }
+    uint32_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t u = __shfl_up(upto, d);
+        if (lane >= d) upto += u;
+    }
+    uint32_t over = upto - mine, at = 0, rest = 0;
+    bool here = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (over < want && over + h[i] >= want) here = true, at = 255 - 4 * lane - i, rest = want - over;
+        over += h[i];
+    }
+    const int who = __builtin_ctzll(__ballot(here));
+    bin = (uint32_t)__builtin_amdgcn_readlane((int)at, who);
+    left = (uint32_t)__builtin_amdgcn_readlane((int)rest, who);
+}
+// What lanes of a wavefront wrote to LDS is there for its others.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // One workgroup: one query token and key head.  Scores of 16 blocks a wavefront at a time -- rows of the product are the
 // group's query rows (x where positive, x where negative), columns the blocks (hi, lo), whole numbers throughout, and two
 // f32 products a score.  Then the key that exactly as many blocks reach as are wanted: passes of 8 bits over a histogram in LDS,
@@ -1757,7 +1860,6 @@ __device__ __forceinline__ uint32_t score_key(float s) {
 // summaries, passes): several tiles' loads go out together, queries ahead of everything.
 template <int D, int T>
 __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
-    using R = kv4_rec<D>;
     constexpr int NJ = D / 64, W = T / 64, U = T == 256 || D == 256 ? 1 : 4;  // U: tiles of 16 blocks whose loads go out together (few wavefronts: all that they have; many: registers count)
     extern __shared__ uint32_t keys[];  // [blocks]
     __shared__ uint32_t hist[4][256], least, most_key;
@@ -1790,34 +1892,8 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
     uint32_t low = 0xffffffffu, high = 0;
     for (int r0 = 0; r0 < A.group; r0 += 16) {
         if (r0) load_rows(r0);
-        i32x4 pos8[NJ], neg8[NJ];
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = max(top, __builtin_bit_cast(uint32_t, a[j][e]) & 0x7fffffffu);  // (of magnitudes the bits are in order, NaN last)
-        top = over_halves(over_rows(top, kv4_umax{}), kv4_umax{});
-        const bool bad = top >= 0x7f800000u;
-        const float most = __builtin_bit_cast(float, top);
-        const float r = bad || most < 7.88860905e-31f ? 0.f : 1.0f / most * 127.f;  // 2^-100
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t up = 0, down = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int v = bad ? 0 : (int)rintf(a[j][4 * w + e] * r);
-                    up |= (uint32_t)(max(v, 0) & 255) << (8 * e);
-                    down |= (uint32_t)(min(v, 0) & 255) << (8 * e);
-                }
-                pos8[j][w] = (int)up;
-                neg8[j][w] = (int)down;
-            }
-        // a lane's four rows of the result are rows 4 g + i
-        float unit[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) unit[i] = __shfl(bad ? 0.f : most * (1.0f / 127.f), 4 * g + i);
+        pick_rows<D> r;
+        round_rows<D>(a, g, r);
         for (int j0 = 16 * wave; j0 < blocks; j0 += 16 * W * U) {
             int phys[U];
 #pragma unroll
@@ -1825,36 +1901,17 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
                 const int block = j0 + 16 * W * u + row;
                 phys[u] = table[min(block, blocks - 1)];
             }
-            i32x4 hi[U][NJ], lo[U][NJ];
-            float scale[U];
+            pick_block<D> s[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const bool there = (unsigned)phys[u] < (unsigned)A.c.num_blocks;
-                const uint8_t *s = A.c.sums + ((size_t)(there ? phys[u] : 0) * A.c.heads + head) * R::SUM;
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    hi[u][j] = *reinterpret_cast<const i32x4 *>(s + 64 * j + 16 * g);
-                    lo[u][j] = *reinterpret_cast<const i32x4 *>(s + D + 64 * j + 16 * g);
-                }
-                scale[u] = *reinterpret_cast<const float *>(s + 2 * D);
-                if (!there) scale[u] = -1.f;  // (a mark: no scale is negative)
-            }
+            for (int u = 0; u < U; ++u) load_summary<D>(A.c, phys[u], head, g, s[u]);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int block = j0 + 16 * W * u + row;
-                i32x4 acc = {0, 0, 0, 0};
+                float mine[4], score = -INFINITY;
+                score_rows<D>(r, s[u], mine);
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos8[j], hi[u][j], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg8[j], lo[u][j], acc, 0, 0, 0);
-                }
-                float score = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float mine = ((float)acc[i] * unit[i]) * scale[u];
-                    score = fmaxf(score, r0 + 4 * g + i < A.group ? mine : -INFINITY);
-                }
-                score = scale[u] == INFINITY ? INFINITY : scale[u] < 0.f ? -INFINITY : score;  // a key that is not finite is not to be missed; no block
+                for (int i = 0; i < 4; ++i) score = fmaxf(score, r0 + 4 * g + i < A.group ? mine[i] : -INFINITY);
+                score = score_of(score, s[u].scale);
                 score = max_groups(score);
                 uint32_t key = score_key(score);
                 if (g == 0 && block < blocks) {
@@ -1885,28 +1942,10 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
                 if ((key & mask) == prefix) atomicAdd(&bins[key >> at & 255], 1u);
             }
             __syncthreads();
-            uint32_t h[4], mine = 0;  // the bins from the top, four a lane
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                h[i] = bins[255 - 4 * lane - i];
-                mine += h[i];
-            }
-            uint32_t upto = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t u = __shfl_up(upto, d);
-                if (lane >= d) upto += u;
-            }
-            uint32_t over = upto - mine, bin = 0, left = 0;
-            bool here = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (over < (uint32_t)want && over + h[i] >= (uint32_t)want) here = true, bin = 255 - 4 * lane - i, left = (uint32_t)want - over;
-                over += h[i];
-            }
-            const int who = __builtin_ctzll(__ballot(here));
-            prefix |= (uint32_t)__builtin_amdgcn_readlane((int)bin, who) << at;
-            want = __builtin_amdgcn_readlane((int)left, who);
+            uint32_t bin, left;
+            bin_of(bins, (uint32_t)want, lane, bin, left);
+            prefix |= bin << at;
+            want = (int)left;
             mask |= 255u << at;
             if (at == 0) break;
             at = max(at - 8, 0);  // (the last pass may look at bits that are settled: they are the same in all that are left)
@@ -1937,6 +1976,114 @@ __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
         if (k == 2 || (k == 1 && q < want)) out[o + min(q, want)] = j;
         o += k == 2;
         q += k == 1;
+    }
+}
+
+// Several tokens of a prompt share a workgroup where a group's rows leave room among the 16 of a product (SLOTS of them a token, a
+// power of two): the summaries are read once for 16 / SLOTS tokens, their keys wait in LDS, and then a wavefront chooses for a
+// token by itself, without barriers.  300 rows of 4 x 8 heads over 250 blocks: 16.6 us, with a workgroup a token 38.5; 200 rows
+// of 8 x 2 heads of 256 over 500: 18 and 41.
+template <int D, int SLOTS>
+__global__ __launch_bounds__(256) void kv4_select_prompt_kernel(kv4_pick A) {
+    constexpr int NJ = D / 64, TOKENS = 16 / SLOTS;
+    extern __shared__ uint32_t keys[];  // [TOKENS][max_blocks]
+    __shared__ uint32_t hist[4][256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, g = lane >> 4, shift = A.c.shift;
+    const int head = blockIdx.x % (unsigned)A.c.heads, width = A.ba.max_blocks;
+    int t = blockIdx.x / (unsigned)A.c.heads * TOKENS;
+    const int behind = min(t + TOKENS, A.ba.tokens);
+    const query_rows qr = rows_of(A.q, A.q_token, A.q_head, A.c.head_dim);
+    while (t < behind) {
+        kv4_request rq;
+        const int b = kv4_find(A.ba, t, shift, rq);
+        if (b < 0) {
+            ++t;
+            continue;
+        }
+        const int n = min(behind, rq.first + rq.rows) - t, pos0 = rq.len - rq.rows + (t - rq.first);  // tokens t .. t + n - 1, the first one's position
+        const int blocks = pos0 + n - 1 < 0 ? 0 : ((pos0 + n - 1) >> shift) + 1;
+        if (blocks > A.top) {
+            float a[NJ][16];
+            const int token = row / SLOTS, h = row % SLOTS;
+            const float *x = token < n && h < A.group ? A.q + (size_t)(t + token) * A.q_token + (size_t)(head * A.group + h) * A.q_head : nullptr;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) take_channels<16>(qr, x, 64 * j + 16 * g, a[j]);
+            pick_rows<D> r;
+            round_rows<D>(a, g, r);
+            const int *table = A.ba.table + (size_t)b * A.ba.max_blocks;
+            for (int j0 = 16 * wave; j0 < blocks; j0 += 64) {
+                const int block = j0 + row;
+                pick_block<D> s;
+                load_summary<D>(A.c, table[min(block, blocks - 1)], head, g, s);
+                float mine[4];
+                score_rows<D>(r, s, mine);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mine[i] = (4 * g + i) % SLOTS < A.group ? mine[i] : -INFINITY;
+                constexpr int EACH = SLOTS < 4 ? SLOTS : 4;  // rows of a token in a lane
+#pragma unroll
+                for (int i = 0; i < 4; i += EACH) {
+                    float score = mine[i];
+#pragma unroll
+                    for (int e = 1; e < EACH; ++e) score = fmaxf(score, mine[i + e]);
+                    if (SLOTS == 8) score = over_rows(score, kv4_max{});
+                    if (block < blocks) keys[(4 * g + i) / SLOTS * width + block] = score_key(score_of(score, s.scale));
+                }
+            }
+        }
+        __syncthreads();
+        for (int token = wave; token < n; token += 4) {
+            const int pos = pos0 + token, mine = pos < 0 ? 0 : (pos >> shift) + 1;  // this token's blocks
+            int *out = A.selected + ((size_t)(t + token) * A.c.heads + head) * A.top;
+            if (mine <= A.top) {
+                for (int j = lane; j < A.top; j += 64) out[j] = j < mine ? j : -1;
+                continue;
+            }
+            const uint32_t *key = keys + token * width;
+            const int free_from = A.first, free_to = mine - A.recent, wanted = A.top - A.first - A.recent;
+            uint32_t low = 0xffffffffu, high = 0, prefix = 0, mask = 0;
+            int want = wanted;
+            if (wanted > 0) {
+                for (int j = free_from + lane; j < free_to; j += 64) low = min(low, key[j]), high = max(high, key[j]);
+                low = ~over_wave(~low, kv4_umax{});
+                high = over_wave(high, kv4_umax{});
+                const uint32_t range = high - low;
+                int at = range ? max(24 - __builtin_clz(range), 0) : 0;
+#pragma unroll 1
+                for (int pass = 0; pass < 4; ++pass) {
+                    uint32_t *bins = hist[wave];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) bins[64 * i + lane] = 0;
+                    wave_fence();
+                    for (int j = free_from + lane; j < free_to; j += 64) {
+                        const uint32_t v = key[j] - low;
+                        if ((v & mask) == prefix) atomicAdd(&bins[v >> at & 255], 1u);
+                    }
+                    wave_fence();
+                    uint32_t bin, left;
+                    bin_of(bins, (uint32_t)want, lane, bin, left);
+                    wave_fence();
+                    prefix |= bin << at;
+                    want = (int)left;
+                    mask |= 255u << at;
+                    if (at == 0) break;
+                    at = max(at - 8, 0);  // (the last pass may look at bits that are settled: they are the same in all that are left)
+                }
+            }
+            int o = 0, equal = 0;
+            for (int j0 = 0; j0 < mine; j0 += 64) {
+                const int j = j0 + lane;
+                int kind = 0;
+                if (j < mine) kind = j < free_from || j >= free_to ? 2 : wanted == 0 ? 0 : key[j] - low > prefix ? 2 : key[j] - low == prefix ? 1 : 0;
+                const uint64_t before = (1ull << lane) - 1, same = __ballot(kind == 1);
+                const bool in = kind == 2 || (kind == 1 && equal + __popcll(same & before) < want);
+                const uint64_t taken = __ballot(in);
+                if (in) out[o + __popcll(taken & before)] = j;
+                o += __popcll(taken);
+                equal += __popcll(same);
+            }
+        }
+        __syncthreads();
+        t += n;
     }
 }
 
@@ -2094,6 +2241,16 @@ PG_API pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *c, con
             if (lds > (48u << 10)) PG_TRY(pg_allow_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds));
             return pg_launch(ctx, "kv4_select_kernel", kernel, dim3((unsigned)(tokens * c->heads)), dim3(threads), lds, A);
         };
+        // Prompts (four rows a request and more, on the whole) of groups that leave room for other tokens, if the chip has enough of them.
+        size_t slots = 1;
+        while (slots < (size_t)A.group) slots *= 2;
+        const size_t each = 16 / slots, shared_lds = each * lds;
+        if (slots <= 8 && max_blocks > top_k && tokens >= 4 * batch && shared_lds <= (40u << 10) && (tokens + each - 1) / each * c->heads >= (size_t)ctx->num_cu / 2) {
+            const dim3 grid((unsigned)((tokens + each - 1) / each * c->heads));
+            auto prompt = [&](auto kernel) { return pg_launch(ctx, "kv4_select_prompt_kernel", kernel, grid, dim3(256), shared_lds, A); };
+            return slots == 1 ? prompt(kv4_select_prompt_kernel<D, 1>) : slots == 2 ? prompt(kv4_select_prompt_kernel<D, 2>) :
+                   slots == 4 ? prompt(kv4_select_prompt_kernel<D, 4>) : prompt(kv4_select_prompt_kernel<D, 8>);
+        }
         return max_blocks > 256 && tokens * c->heads <= (size_t)ctx->num_cu * 2 ? go(kv4_select_kernel<D, 1024>, 1024) : go(kv4_select_kernel<D, 256>, 256);
     });
 }

@@ -526,6 +526,27 @@ def test_selected_attention_over_long_contexts(ctx, hd, heads, group, bs, n, top
     w.check(full, q, [2], hd ** -0.5, cap=4.0, what="all blocks")
 
 
+@pytest.mark.parametrize("hd,heads,group,bs,rows,lens", [(64, 8, 1, 16, [150, 3, 0, 130], [420, 300, 40, 131]), (128, 4, 4, 16, [70, 1, 61], [500, 9, 61]), (80, 8, 3, 16, [40, 33], [90, 333]),
+                                                       (256, 4, 8, 32, [66], [700]), (128, 8, 6, 16, [21, 0, 12], [220, 100, 500]), (64, 4, 2, 64, [200, 90], [2300, 91])])
+def test_selection_for_prompts_is_exact(ctx, hd, heads, group, bs, rows, lens):
+    """Enough rows a request that several of them share a workgroup; groups of rows across two requests' border."""
+    w = World(ctx, lens, heads, hd, bs, seed=hd + group, spare=1)
+    w.put(np.full((1, heads, hd), np.nan, F), np.ones((1, heads, hd), F), w.slots(0, [3 * bs + 1]))
+    w.put(np.zeros((2 * bs, heads, hd), F), np.ones((2 * bs, heads, hd), F), w.slots(0, np.arange(bs, 3 * bs)))       # equal scores
+    w.cache.summarise(np.concatenate([[0], np.cumsum(lens)]), w.lens, w.table)
+    q = w.q(sum(rows), heads * group)
+    q[5, 0], q[6] = np.nan, 0
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    looked = sorted(set(w.rng.integers(0, sum(rows), 12)) | {0, 5, 6, 7, rows[0] - 1, min(rows[0], sum(rows) - 1), sum(rows) - 1})
+    for top, first, recent in ((4, 1, 1), (9, 0, 3), (2, 0, 1), (3, 2, 1), (60, 2, 2)):
+        got = w.cache.select(q, starts, w.lens, w.table, top, first, recent)
+        for t in looked:
+            b = int(np.searchsorted(starts, t, "right")) - 1
+            w.ref.lens_now = lens[b]
+            want = R.select(q[t].reshape(heads, group, hd), w.ref, w.table[b], lens[b] - rows[b] + t - starts[b], top, first, recent)
+            assert (got[t] == want).all(), f"top {top}: row {t} of request {b}"
+
+
 def test_selected_entries_that_break_the_rules_contribute_nothing(ctx):
     w = World(ctx, [100], 1, 64, 16, seed=8)
     q = w.q(1, 2)
