@@ -483,7 +483,8 @@ pg_status pg_paged_kv4_read_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, const in
  * query_start[batch] are left as they were.  Query head h reads key head h / (num_q_heads / num_kv_heads).  Masks as in
  * pg_gqa_attention without LocalGlobal, a row's position being its token's; a row that sees no key is 0.  logit_cap as there.
  * max_query: no request has more rows (those beyond are not computed).  scratch_dev: 16-byte aligned, at least what
- * pg_paged_kv4_attention_scratch says for these sizes (it may be 0); calls that may run at once have one each. */
+ * pg_paged_kv4_attention_scratch says for these sizes (it may be 0); calls that may run at once have one each.  Steps of more
+ * than 2^24 tiles (a request's key head, 4 to 16 of its rows) are PG_EUNSUPPORTED. */
 pg_status pg_paged_kv4_attention_scratch(pg_ctx *ctx, const pg_paged_kv4 *cache, size_t num_q_heads, size_t batch,
                                          size_t max_query, size_t max_blocks, size_t *bytes);
 pg_status pg_paged_kv4_attention(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q, size_t num_q_heads,
@@ -514,7 +515,7 @@ pg_status pg_paged_kv4_read_summaries_dev(pg_ctx *ctx, const pg_paged_kv4 *cache
  * row's scores in the block but for the roundings).  The first `first_blocks` and the last `recent_blocks` (at least 1: the
  * row's own) are always among them; of equal scores the earlier block.  selected [tokens, num_kv_heads, top_k]: block numbers
  * within the request, ascending, -1 behind them.  A block that holds a key that is not finite scores infinity; a query row
- * that is not finite scores 0.  max_blocks <= 36864 (PG_EUNSUPPORTED). */
+ * that is not finite scores 0.  max_blocks <= 36864, tokens * num_kv_heads < 2^22 (PG_EUNSUPPORTED). */
 pg_status pg_paged_kv4_select(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q, size_t num_q_heads,
                               const int32_t *query_start, const int32_t *seq_lens, size_t batch, size_t tokens,
                               const int32_t *block_table, size_t max_blocks, size_t top_k, size_t first_blocks,

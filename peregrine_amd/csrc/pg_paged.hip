@@ -48,7 +48,7 @@ __device__ __forceinline__ int last_upto(const int *at, int n, int v) {
 // not, so those that are met come first: a granted request's new blocks begin at the sum of the needs before it, and new entries
 // and slots are flat lists, a thread a place, the request by bisection in LDS.  A slot in a new block comes from the free list like
 // the entry itself, so nothing waits for what this launch writes.  A few loads behind one another bound it: 256 decoding
-// requests 13.4 us with a wavefront a request for entries and slots, one after the other.
+// requests 6.0 us, 13.4 with a wavefront a request for entries and slots; 200 prompts with 250 000 slots 10.4 us on 62 workgroups.
 // Workgroup w does the slots of rows 4096 w .. and on; the first does everything else, and may write lengths and count over their
 // inputs if it is the only one (slots = null: no slots, slot_map_kernel does them).
 __global__ __launch_bounds__(1024) void extend_tables_kernel(const int *seq_lens, const int *new_lens, int batch, int shift, const int *free_list, const int *free_count,
@@ -213,8 +213,9 @@ struct row_max {
     __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b))); }
 };
 
-// Eight channels of a row a lane, D / 8 lanes a row, TWO rows a lane half the launch apart: both rows' loads are on their way before
-// anything is known of their slots.  Bound by memory: a row's 4 D bytes in, D / 2 + 4 out.
+// Eight channels of a row a lane, D / 8 lanes a row, TWO rows a lane half a workgroup's apart: both rows' loads are on their way before
+// anything is known of their slots.  Bound by memory: a row's 4 D bytes in, D / 2 + 4 out; 13 600 tokens of 8 heads of 128 in 34 us
+// (3.7 TB/s).
 template <int D, bool WIDE>
 __global__ __launch_bounds__(256) void kv4_append_kernel(const float *__restrict__ k, const float *__restrict__ v, kv4_view c, size_t token_stride, size_t head_stride,
                                                          int tokens, const int *__restrict__ slots) {
@@ -641,6 +642,7 @@ PG_API pg_status pg_paged_kv4_summarise_dev(pg_ctx *ctx, pg_paged_kv4 *c, const 
     PG_TRY(pg_kv4_check_step("pg_paged_kv4_summarise", c, c->heads, batch, tokens, max_blocks));
     if (tokens == 0 || batch == 0) return PG_OK;
     PG_CHECK_ARG(query_start_dev && seq_lens_dev && block_table_dev, "pg_paged_kv4_summarise: null pointer");
+    if ((tokens >> c->shift) + 2 * batch >= (1u << 24)) return pg_fail(PG_EUNSUPPORTED, "pg_paged_kv4_summarise: %zu rows are more than a launch takes", tokens);
     c->touch(ctx);
     const kv4_batch ba = {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks};
     return with_width(c->D, [&](auto w) -> pg_status {

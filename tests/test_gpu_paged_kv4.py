@@ -176,6 +176,36 @@ def test_extend_in_place_cuts_what_does_not_fit(ctx):
         assert (slots[:tokens] == want[5]).all() and (slots[tokens:] == 55).all()
 
 
+@pytest.mark.parametrize("batch,most_new,in_place", [(30, 900, False), (30, 900, True), (700, 40, True), (4097, 6, False), (4097, 6, True), (2000, 12, False)])
+def test_extend_over_many_rows(ctx, batch, most_new, in_place):
+    """More rows than one workgroup maps to slots: by several, or by a second launch where lengths are written over their inputs."""
+    rng = np.random.default_rng(batch + most_new)
+    bs = 16
+    lens, add = rng.integers(0, 200, batch).astype(np.int32), rng.integers(0, most_new + 1, batch).astype(np.int32)
+    width = -(-(200 + most_new) // bs)
+    have = -(-lens // bs)
+    need = int((-(-(lens + add) // bs) - have).sum())
+    nb = int(have.sum()) + need + 3
+    ids = rng.permutation(nb).astype(np.int32)
+    table = np.full((batch, width), -1, np.int32)
+    for b, at in enumerate(np.cumsum(have) - have):
+        table[b, :have[b]] = ids[at: at + have[b]]
+    count = need - 20                                                     # the last requests get none
+    free = np.zeros(nb, np.int32)
+    free[:count] = ids[have.sum(): have.sum() + count]
+    tokens = int(add.sum()) + 5
+    assert tokens > 4096
+    want = extend_ref(lens, add, bs, width, table, free, count, tokens)
+    d = [DevBuf(ctx, host=x) for x in (lens, add, free, ints([count]), table, np.zeros(batch + 1, np.int32), np.zeros(batch, np.int32), np.full(tokens, 77, np.int32))]
+    lens_out, count_out = (d[0], d[3]) if in_place else (DevBuf(ctx, host=np.full(batch, 77, np.int32)), DevBuf(ctx, host=ints([77])))
+    ok(lib().pg_block_tables_extend_dev(ctx.handle, d[0].ptr, d[1].ptr, batch, bs, d[2].ptr, d[3].ptr, nb, d[4].ptr, width, lens_out.ptr, count_out.ptr, d[5].ptr, d[6].ptr,
+                                        d[7].ptr, tokens))
+    got = [d[4].to_host(np.int32).reshape(batch, width), lens_out.to_host(np.int32), count_out.to_host(np.int32)[0], d[5].to_host(np.int32), d[6].to_host(np.int32),
+           d[7].to_host(np.int32)]
+    for g, x in zip(got, want):
+        assert (np.asarray(g) == np.asarray(x)).all()
+
+
 @pytest.mark.parametrize("batch", [1, 70, 1100])
 def test_release_gives_every_block_back_in_order(ctx, batch):
     rng = np.random.default_rng(batch)
@@ -727,6 +757,68 @@ def test_prompts_leave_out_what_is_no_block_and_read_nothing_behind(ctx, hd, hea
     one = World.__new__(World)
     one.__dict__.update(w.__dict__, lens=w.lens[:1], table=w.table[:1])
     one.check(got[: rows[0]], q[: rows[0]], rows[:1], hd ** -0.5, only=lambda t, h: [j for j in range(w.width) if j not in gone], what="no block")
+
+
+@pytest.mark.parametrize("hd,heads,group", [(63, 2, 4), (125, 2, 4), (250, 1, 8), (64, 2, 8), (128, 1, 16), (256, 1, 4)])
+def test_prompts_from_strided_queries_and_rows_before_the_first_token(ctx, hd, heads, group):
+    """Queries that no vector load can take give the bits of packed ones; of a request with more rows than tokens the first see no
+    key; rows beyond max_query, which is a bound on what is computed, and behind the last are left."""
+    lens, rows, n = [90, 30], [80, 50], heads * group
+    w = World(ctx, lens, heads, hd, 16, seed=hd)
+    q = w.q(sum(rows) + 3, n)
+    starts = [0, 80, 130]
+    got = []
+    for pad in (0, 1, 4):
+        x = np.full((q.shape[0], n, hd + pad), np.nan, F)
+        x[..., :hd] = q
+        buf, s = DevBuf(ctx, host=x), Step(ctx, w, q, starts)
+        s.attention(strides=(n * (hd + pad), hd + pad), q=buf.ptr)
+        got.append(s.result())
+    assert (bits(got[0]) == bits(got[1])).all() and (bits(got[0]) == bits(got[2])).all()
+    seen = np.r_[0:80, 100:130]
+    assert (got[0][80:100] == 0).all() and (got[0][130:] == 123).all()
+    w.check(got[0][seen], q[seen], [80, 30], hd ** -0.5)
+    s = Step(ctx, w, q, starts, max_query=60)
+    s.attention()
+    cut = s.result()
+    assert (cut[60:80] == 123).all()
+    w.check(cut[np.r_[100:130]], q[np.r_[100:130]], [0, 30], hd ** -0.5)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompts_replayed_from_a_graph(ctx, hd):
+    """Pieces of prompts, and the choice of blocks for them, captured once; other queries and lengths at each replay."""
+    from test_gpu_graph_replay import Hip
+    hip, heads, group, bs, rows, top = Hip(), 2, 4, 16, [90, 170], 3
+    w = World(ctx, [700, 400], heads, hd, bs, seed=hd, poison=False)
+    w.cache.summarise([0, 700, 1100], w.lens, w.table)
+    q = w.q(sum(rows), heads * group)
+    s, e = (Step(ctx, w, q, [0, 90, 260]) for _ in range(2))
+    sel = [DevBuf(ctx, host=np.zeros((sum(rows), heads, top), np.int32)) for _ in range(2)]
+
+    def step(x, out):
+        x.attention(mask=2, window=300, sinks=4)
+        starts, lens, table, qd = x.d
+        ok(lib().pg_paged_kv4_select_dev(ctx.handle, w.cache._h, qd.ptr, heads * group * hd, hd, heads * group, starts.ptr, lens.ptr, 2, sum(rows), table.ptr, x.width, top, 1, 1,
+                                         out.ptr))
+
+    step(s, sel[0])
+    ctx.sync()
+    graph, ex = hip.capture(ctx.stream, lambda: step(s, sel[0]))
+    try:
+        for i in range(4):
+            lens, x = ints([700 - 100 * i, 400 - 70 * i]), w.q(sum(rows), heads * group)
+            for y in (s, e):
+                for b, a in ((y.d[1], lens), (y.d[3], x)):
+                    ok(lib().pg_memcpy_h2d(ctx.handle, b.ptr, C.c_void_p(a.ctypes.data), a.nbytes))
+            step(e, sel[1])
+            ctx.sync()
+            hip.ok(hip.lib.hipGraphLaunch(ex, ctx.stream), "hipGraphLaunch")
+            ctx.sync()
+            assert (bits(s.result()) == bits(e.result())).all() and (sel[0].to_host(np.int32) == sel[1].to_host(np.int32)).all(), f"replay {i}"
+    finally:
+        hip.lib.hipGraphExecDestroy(ex)
+        hip.lib.hipGraphDestroy(graph)
 
 
 def test_cpp_host_mirror():

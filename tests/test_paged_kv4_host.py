@@ -182,6 +182,14 @@ def test_scratch_does_not_depend_on_the_rows_there_are(host):
     host.lib.pg_paged_kv4_free(host.ctx, c)
 
 
+def test_summaries_refuse_more_blocks_than_a_launch_takes(host):
+    c = new_cache(host, 64, 16, 2, 64)
+    buf = host.alloc(1 << 16)
+    for tokens, want in (((1 << 28) - 64, 0), (1 << 28, EUNSUPPORTED), ((1 << 31) - 1, EUNSUPPORTED)):
+        assert status(host, "pg_paged_kv4_summarise_dev", host.ctx, c, buf, buf, 1, tokens, buf, 64) == want, tokens
+    host.lib.pg_paged_kv4_free(host.ctx, c)
+
+
 def test_a_step_is_captured_as_launches_alone(host):
     """Nothing of a step's device forms allocates, waits or copies."""
     c = new_cache(host, 4096, 64, 2, 128)
