@@ -2111,24 +2111,41 @@ struct plan {
     size_t rows, row_tiles, tiles, splits, bytes;  // rows a tile (4, 8 or 16)
     size_t wide;                                   // row tiles a workgroup of the prompts' kernels, or 0: the others
 };
-constexpr size_t PROMPT_TILES = 4;
-plan plan_for(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t units, size_t unit_rows, size_t tokens) {
+
+// What a unit's many rows take on the prompts' kernels and on kv4_rows_kernel, in us, from 38 timed steps (5 to 2048 rows of a group of
+// 1 to 16, 1 to 32 requests of 60 to 16384 tokens): rounds of workgroups, each a start and its tokens, and the joining launch with its bytes.
+// Eight row tiles in one workgroup take what 5.7 of them take apart, but the workgroup starts later (queries and the first operands
+// through LDS), its tiles are not always eight, nor its workgroups always as many as the chip runs: 320 rows of 8 x 8 heads over
+// 2000 tokens 101 us and 78 apart, 200 of 8 over 1000 30 and 15; 256 of 16 x 8 over 4000 187 and 215, 624 of 12 x 8 over 60 25 and
+// 46, 8192 of 8 over 16384 1130 and 1370.
+double join_us(size_t rows, size_t D, size_t splits) { return splits > 1 ? 4 + (double)rows * D * 4 * (2 * splits + 1) / 4.5e6 : 0; }
+double rounds_of(size_t workgroups, double run) { return workgroups <= run ? 1 : (double)workgroups / run + 0.15; }
+bool prompts_pay(const pg_ctx *ctx, size_t units, size_t row_tiles, size_t tokens, size_t D) {
+    const size_t groups = units * ((row_tiles + 7) / 8), tiles = units * row_tiles, rows = tiles * 16;
+    const double cus = ctx->num_cu, each = tokens * (double)D / 128;
+    const size_t ws = pick_splits(ctx, groups, tokens, true, D), rs = pick_splits(ctx, tiles, tokens, false, D);
+    const double whole = rounds_of(groups * ws, D == 256 ? cus : 2 * cus) * (14 + (D == 256 ? 0.0358 : 0.0716) * each / ws) + join_us(rows, D, ws);
+    const double apart = rounds_of(tiles * rs, D == 256 ? 2 * cus : 3 * cus) * (6 + (D == 256 ? 0.0118 : 0.0188) * each / rs) + join_us(rows, D, rs);
+    return whole < apart;
+}
+// tokens: of the table; seen: of those that any row sees, where a window says so (fewer runs than were reported without it need no
+// more scratch; the kernel is chosen without it, so that it is the same one).
+plan plan_for(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t units, size_t unit_rows, size_t tokens, size_t seen, bool prompts) {
     plan p;
     p.rows = unit_rows <= 4 ? 4 : unit_rows <= 8 ? 8 : 16;
     p.row_tiles = (unit_rows + p.rows - 1) / p.rows;
     p.tiles = units * c->heads * p.row_tiles;
-    p.wide = p.row_tiles < PROMPT_TILES ? 0 : 8;
+    p.wide = prompts && p.row_tiles >= 4 && prompts_pay(ctx, units * c->heads, p.row_tiles, tokens, (size_t)c->D) ? 8 : 0;
     const size_t workgroups = p.wide ? units * c->heads * ((p.row_tiles + p.wide - 1) / p.wide) : p.tiles;
-    p.splits = pick_splits(ctx, workgroups, tokens, p.wide, (size_t)c->D);
+    p.splits = pick_splits(ctx, workgroups, std::min(tokens, seen), p.wide, (size_t)c->D);
     p.bytes = p.splits > 1 ? p.tiles * p.splits * (p.rows * (size_t)c->D + 32) * sizeof(float) : 0;
     return p;
 }
-// (seen: tokens that any row sees, where a window says so.  Fewer runs need no more scratch than was reported without it.)
 plan dense_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t max_query, size_t max_blocks, size_t seen = SIZE_MAX) {
-    return plan_for(ctx, c, batch, max_query * (num_q_heads / c->heads), std::min(max_blocks * c->block_size, seen));
+    return plan_for(ctx, c, batch, max_query * (num_q_heads / c->heads), max_blocks * c->block_size, seen, true);
 }
 plan selected_plan(const pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t tokens, size_t top) {
-    return plan_for(ctx, c, tokens, num_q_heads / c->heads, top * c->block_size);
+    return plan_for(ctx, c, tokens, num_q_heads / c->heads, top * c->block_size, SIZE_MAX, false);
 }
 
 template <bool SELECTED>
@@ -2136,7 +2153,7 @@ pg_status launch_rows(pg_ctx *ctx, const char *fn, const pg_paged_kv4 *c, kv4_at
     if (p.tiles * p.splits >= (1u << 24)) return pg_fail(PG_EUNSUPPORTED, "%s: %zu row tiles in %zu runs are more than a launch takes", fn, p.tiles, p.splits);
     A.splits = (int)p.splits;
     A.row_tiles = (int)p.row_tiles;
-    A.by_length = !SELECTED && p.splits == 1 && A.ba.batch <= RANKED && p.tiles > (size_t)ctx->num_cu * 2;
+    A.by_length = !SELECTED && p.splits == 1 && A.ba.batch > 1 && A.ba.batch <= RANKED && p.tiles > (size_t)ctx->num_cu * 2;
     const dim3 grid((unsigned)(p.tiles * p.splits)), join((unsigned)(p.tiles * p.rows / 4)), block(256);
     return with_width(c->D, [&](auto w) -> pg_status {
         constexpr int D = decltype(w)::value;
@@ -2251,7 +2268,7 @@ PG_API pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *c, con
             return slots == 1 ? prompt(kv4_select_prompt_kernel<D, 1>) : slots == 2 ? prompt(kv4_select_prompt_kernel<D, 2>) :
                    slots == 4 ? prompt(kv4_select_prompt_kernel<D, 4>) : prompt(kv4_select_prompt_kernel<D, 8>);
         }
-        return max_blocks > 256 && tokens * c->heads <= (size_t)ctx->num_cu * 2 ? go(kv4_select_kernel<D, 1024>, 1024) : go(kv4_select_kernel<D, 256>, 256);
+        return max_blocks > 640 && tokens * c->heads <= (size_t)ctx->num_cu ? go(kv4_select_kernel<D, 1024>, 1024) : go(kv4_select_kernel<D, 256>, 256);
     });
 }
 

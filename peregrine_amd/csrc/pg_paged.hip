@@ -48,7 +48,7 @@ __device__ __forceinline__ int last_upto(const int *at, int n, int v) {
 // not, so those that are met come first: a granted request's new blocks begin at the sum of the needs before it, and new entries
 // and slots are flat lists, a thread a place, the request by bisection in LDS.  A slot in a new block comes from the free list like
 // the entry itself, so nothing waits for what this launch writes.  A few loads behind one another bound it: 256 decoding
-// requests 6.0 us, 13.4 with a wavefront a request for entries and slots; 200 prompts with 250 000 slots 10.4 us on 62 workgroups.
+// requests 6.0 us, 13.4 with a wavefront a request for entries and slots; 200 prompts with 223 000 slots 10.4 us on 55 workgroups.
 // Workgroup w does the slots of rows 4096 w .. and on; the first does everything else, and may write lengths and count over their
 // inputs if it is the only one (slots = null: no slots, slot_map_kernel does them).
 __global__ __launch_bounds__(1024) void extend_tables_kernel(const int *seq_lens, const int *new_lens, int batch, int shift, const int *free_list, const int *free_count,
@@ -214,8 +214,8 @@ struct row_max {
 };
 
 // Eight channels of a row a lane, D / 8 lanes a row, TWO rows a lane half a workgroup's apart: both rows' loads are on their way before
-// anything is known of their slots.  Bound by memory: a row's 4 D bytes in, D / 2 + 4 out; 13 600 tokens of 8 heads of 128 in 34 us
-// (3.7 TB/s).
+// anything is known of their slots.  Bound by memory: a row's 4 D bytes in, D / 2 + 4 out; 15 400 tokens of 8 heads of 128 in 34 us
+// (4.2 TB/s).
 template <int D, bool WIDE>
 __global__ __launch_bounds__(256) void kv4_append_kernel(const float *__restrict__ k, const float *__restrict__ v, kv4_view c, size_t token_stride, size_t head_stride,
                                                          int tokens, const int *__restrict__ slots) {
@@ -284,7 +284,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const float *__restrict
     }
 }
 
-// The rows of the named slots as the values they stand for; rows of a slot that is none are 0.
+// The rows of the named slots as the values they stand for; rows of a slot that is none are 0.  Bound by memory: 17 000 tokens of 8
+// heads of 128 in 27 us (5.8 TB/s).
 template <int D>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const int *__restrict__ slots, float *__restrict__ k, kv4_view c, int n, float *__restrict__ v) {
     using R = kv4_rec<D>;

@@ -821,6 +821,79 @@ def test_prompts_replayed_from_a_graph(ctx, hd):
         hip.lib.hipGraphDestroy(graph)
 
 
+def check_some(w, got, q, rows, scale, count, mask=1, window=0, sinks=0, cap=0.0, gone=()):
+    """World.check on `count` rows and heads, the first and the last of each request among them; gone: (request, block) that are none."""
+    starts, group, kv = np.concatenate([[0], np.cumsum(rows)]), q.shape[1] // w.heads, {}
+    picks = [(int(t), int(j)) for t, j in zip(w.rng.integers(0, starts[-1], count), w.rng.integers(0, q.shape[1], count))]
+    picks += [(int(t), 0) for b, n in enumerate(rows) if n for t in (starts[b], starts[b + 1] - 1)]
+    off = size = 0.0
+    for t, j in picks:
+        b = int(np.searchsorted(starts, t, "right")) - 1
+        if b not in kv:
+            at = w.slots(b, np.arange(w.lens[b]))
+            kv[b] = w.ref.f64(0, at), w.ref.f64(1, at)
+        keys, pos = np.arange(w.lens[b]), w.lens[b] - rows[b] + t - starts[b]
+        seen = np.ones(keys.size, bool) if mask == 0 else keys <= pos
+        if mask == 2:
+            seen &= (pos - keys <= window) | (keys < sinks)
+        for x, block in gone:
+            seen &= (x != b) | (keys // w.bs != block)
+        want, bound = R.attend(q[t, j], kv[b][0][:, j // group], kv[b][1][:, j // group], scale, seen, cap)
+        d = np.abs(got[t, j] - want)
+        assert (d <= bound).all(), f"row {t}, head {j}: off by {d.max():.3g}, bound {bound.min():.3g}"
+        off, size = off + (d ** 2).sum(), size + (want ** 2).sum()
+    assert size == 0 or (off / size) ** 0.5 < 3e-6
+
+
+def kernels_of(ctx, call):
+    ctx.profile_begin()
+    call()
+    ctx.sync()
+    return set(ctx.profile_end())
+
+
+@pytest.mark.parametrize("hd,group,bs", [(40, 16, 16), (64, 12, 32), (100, 16, 16), (128, 16, 64), (200, 12, 16), (256, 16, 32)])
+def test_prompts_of_many_requests(ctx, hd, group, bs):
+    """Enough rows for the prompts' own kernels: every mask, requests of no rows and no tokens, blocks that are none, NaN in every
+    slot that is not theirs and in a row that only some see."""
+    heads, lens = 8, [90, 1, 0, 33, 64, 65, 17, 80, 48, 5, 77, 16, 31, 90, 2, 60, 70, 12, 88, 20]
+    w = World(ctx, lens, heads, hd, bs, seed=hd)
+    rows = [min(n, r) for n, r in zip(lens, [90, 1, 0, 20, 64, 30, 17, 79, 0, 5, 40, 16, 31, 1, 2, 60, 33, 12, 88, 20])]
+    q = w.q(sum(rows), heads * group)
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    own = "kv4_prompt_kernel" if hd > 128 else "kv4_prompt32_kernel"
+    for m in (dict(), dict(mask=0), dict(mask=2, window=20, sinks=3), dict(mask=2, window=0, sinks=0), dict(cap=5.0)):
+        s = Step(ctx, w, q, starts)
+        assert own in kernels_of(ctx, lambda: s.attention(**m))
+        check_some(w, s.result(), q, rows, hd ** -0.5, 250, **m)
+    gone = [(0, 1), (4, 0), (15, 60 // bs if bs < 64 else 0)]
+    table = w.table.copy()
+    for i, (b, j) in enumerate(gone):
+        table[b, j] = (-1, w.nb, 2 ** 31 - 1)[i]
+    s = Step(ctx, w, q, starts, table=table)
+    s.attention()
+    got = s.result()
+    check_some(w, got, q, rows, hd ** -0.5, 250, gone=gone)
+    assert np.isfinite(got).all()
+    w.put(w.keys(1), np.full((1, heads, hd), np.nan, F), w.slots(0, [50]))
+    s = Step(ctx, w, q, starts)
+    s.attention()
+    nan = np.isnan(s.result()).all((1, 2))
+    assert (nan == ((np.arange(len(q)) >= 50) & (np.arange(len(q)) < 90))).all() and np.isfinite(s.result()[~nan]).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_long_prompt_divided_between_workgroups(ctx, hd):
+    heads, group, n, rows = 4, 4, 8100, 2048
+    w = World(ctx, [n], heads, hd, 64, seed=hd, poison=False)
+    q = w.q(rows, heads * group)
+    own = "kv4_prompt_kernel" if hd > 128 else "kv4_prompt32_kernel"
+    for m in (dict(), dict(cap=20.0)):
+        s = Step(ctx, w, q, [0, rows])
+        assert kernels_of(ctx, lambda: s.attention(**m)) == {own, "kv4_join_kernel"}
+        check_some(w, s.result(), q, [rows], hd ** -0.5, 40, **m)
+
+
 def test_cpp_host_mirror():
     """tests/cpp/paged_kv4.cpp over the C++ mirror's namespace paged; built by __graft_entry__.build()."""
     import os
