@@ -808,7 +808,9 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
     __builtin_amdgcn_wave_barrier();
 }
 
-// As kv4_rows_kernel, for up to HB rows of a unit: one row tile, wavefronts every fourth tile of 64 tokens.
+// As kv4_rows_kernel, for up to HB rows of a unit: one row tile, wavefronts every fourth tile of 64 tokens.  Bound by memory where
+// contexts are long: 128 requests of 7500 tokens, 8 key heads of 128, a group of 4 202 to 208 us (5.0 to 5.2 TB/s; loads alone 5.5, a
+// copy 4.8), of 8 211.  Three workgroups a CU where the registers reach (with 8 rows they do not: 26 spilled, 347 us).
 template <int D, int HB, bool CAP, bool SELECTED>
 __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void kv4_few_kernel(kv4_attn A) {
     using R = kv4_rec<D>;
@@ -1011,10 +1013,11 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
 
 // ---- prompts --------------------------------------------------------------------------------
 // With many rows the keys' and values' way from codes to operands is what 16 rows at a time would pay for again and again.
-// Here a workgroup has NW wavefronts of RT tiles of 16 rows and makes the operands of 64 tokens once, in LDS, in the order in
-// which the lanes take them; the next 64 tokens' codes are on their way meanwhile, and the two buffers take turns, one
-// barrier a tile.  Scores and probabilities as in kv4_rows_kernel.  What bounds it is the arithmetic on scores: about 17
-// instructions for each of 16 x 64 beside 56 products of the matrix cores.
+// Here a workgroup has eight wavefronts of 16 rows and makes the operands of 64 tokens once, in LDS, in the order in
+// which the lanes take them (four wavefronts the keys', four the values'); the next 64 tokens' codes are on their way meanwhile, and the
+// two buffers take turns, one barrier a tile.  Scores and probabilities as in kv4_rows_kernel.  What bounds it is the arithmetic on
+// scores: about 17 instructions for each of 16 x 64 beside 56 products of the matrix cores.  Heads of 256: 2048 rows at 8192, 16 heads,
+// 487 us (477 TFLOP/s of one product each).
 template <int D>
 struct prompt_lds {
     static constexpr int K = 64 * D, V = 128 * D;  // bytes of a tile's operands
@@ -1331,7 +1334,8 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
 // largest): two more products a step than with three int8 digits on half the depth, and four instructions a score less, of
 // which there are 16 a lane.  Lanes and operands: A and B of a product hold 8 values of its 16 deep side, row or column lane & 31;
 // a result's registers i are rows (i & 3) + 8 (i >> 2) + 4 (lane >> 5), which makes the probabilities of registers 8 s .. 8 s + 7
-// the B operand of step s once the values' tokens stand in that order.
+// the B operand of step s once the values' tokens stand in that order.  2048 rows at 16384, 32 heads of 128: 1095 us (471 TFLOP/s of one
+// product each, twice that executed); vector instructions 51 %, matrix products 39 % of the cycles, which do not overlap much better.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int D>
@@ -1857,7 +1861,8 @@ __device__ __forceinline__ void wave_fence() {
 // f32 products a score.  Then the key that exactly as many blocks reach as are wanted: passes of 8 bits over a histogram in LDS,
 // from the highest bit in which the keys differ, every wavefront with its own sums over the bins, so a pass is one barrier.  Then
 // the blocks over that key, and of those at it the first, in ascending order.  It is a chain of latencies (request, table,
-// summaries, passes): several tiles' loads go out together, queries ahead of everything.
+// summaries, passes): several tiles' loads go out together, queries ahead of everything.  8 rows of 8 key heads over 1024 blocks
+// 20 us: 64 workgroups of 1024 threads, each bound by what one CU loads (about 20 GB/s).
 template <int D, int T>
 __global__ __launch_bounds__(T) void kv4_select_kernel(kv4_pick A) {
     constexpr int NJ = D / 64, W = T / 64, U = T == 256 || D == 256 ? 1 : 4;  // U: tiles of 16 blocks whose loads go out together (few wavefronts: all that they have; many: registers count)
@@ -2258,7 +2263,9 @@ PG_API pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *c, con
             if (lds > (48u << 10)) PG_TRY(pg_allow_dynamic_lds(ctx, reinterpret_cast<const void *>(kernel), lds));
             return pg_launch(ctx, "kv4_select_kernel", kernel, dim3((unsigned)(tokens * c->heads)), dim3(threads), lds, A);
         };
-        // Prompts (four rows a request and more, on the whole) of groups that leave room for other tokens, if the chip has enough of them.
+        // Prompts (four rows a request and more, on the whole) of groups that leave room for other tokens, if the chip has enough of them:
+        // 16 requests of 4 rows, 8 heads of 4 over 62 blocks 7.4 us against 9.9, of 2 rows 11.6 against 8.5; 4 of 8 rows of 2 heads of 1,
+        // which leave ten workgroups, 13.9 against 7.9.
         size_t slots = 1;
         while (slots < (size_t)A.group) slots *= 2;
         const size_t each = 16 / slots, shared_lds = each * lds;
@@ -2268,6 +2275,8 @@ PG_API pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *c, con
             return slots == 1 ? prompt(kv4_select_prompt_kernel<D, 1>) : slots == 2 ? prompt(kv4_select_prompt_kernel<D, 2>) :
                    slots == 4 ? prompt(kv4_select_prompt_kernel<D, 4>) : prompt(kv4_select_prompt_kernel<D, 8>);
         }
+        // 1024 threads where a row has many blocks and the chip has room: 64 rows and heads over 500 / 1000 / 2000 blocks 17 / 23 / 32 us
+        // against 14 / 29 / 52 of 256 threads; 512 of them over 1000 51 against 38.
         return max_blocks > 640 && tokens * c->heads <= (size_t)ctx->num_cu ? go(kv4_select_kernel<D, 1024>, 1024) : go(kv4_select_kernel<D, 256>, 256);
     });
 }
