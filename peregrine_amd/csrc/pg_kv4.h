@@ -18,7 +18,13 @@ struct pg_paged_kv4 {
     size_t num_blocks, block_size, heads, head_dim;
     int D, shift;  // stored channels of a row, log2(block_size)
     mutable pg_dev_block mem, sums_mem;
+    int device;
     void touch(const pg_ctx *ctx) const { mem.touch(ctx); sums_mem.touch(ctx); }
+    pg_status use(const char *fn, const pg_ctx *ctx) const {
+        PG_CHECK_ARG(ctx->device == device, "%s: a cache on device %d, a context on device %d", fn, device, ctx->device);
+        touch(ctx);
+        return PG_OK;
+    }
 };
 
 // What a kernel needs to know of a cache.

@@ -2231,7 +2231,7 @@ PG_API pg_status pg_paged_kv4_attention_dev(pg_ctx *ctx, const pg_paged_kv4 *c, 
     const plan p = dense_plan(ctx, c, num_q_heads, batch, max_query, max_blocks, seen);
     PG_CHECK_ARG(p.bytes == 0 || (scratch_dev && scratch_bytes >= p.bytes && ((uintptr_t)scratch_dev & 15) == 0),
                  "%s: scratch of %zu bytes, %zu are needed (16-byte aligned)", fn, scratch_bytes, p.bytes);
-    c->touch(ctx);
+    PG_TRY(c->use(fn, ctx));
     kv4_attn A = {};
     A.q = q_dev, A.q_token = q_token_stride, A.q_head = q_head_stride;
     A.c = kv4_view_of(c);
@@ -2257,7 +2257,7 @@ PG_API pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *c, con
     const size_t lds = max_blocks * sizeof(uint32_t);
     if (lds > (144u << 10)) return pg_fail(PG_EUNSUPPORTED, "%s: tables of %zu blocks (36864 at most: their scores live in on-chip memory)", fn, max_blocks);
     if (tokens * c->heads >= (1u << 22)) return pg_fail(PG_EUNSUPPORTED, "%s: %zu rows of %zu key heads are more than a launch takes", fn, tokens, c->heads);
-    c->touch(ctx);
+    PG_TRY(c->use(fn, ctx));
     kv4_pick A = {q_dev, q_token_stride, q_head_stride, kv4_view_of(c), {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks},
                   (int)(num_q_heads / c->heads), (int)top_k, (int)first_blocks, (int)recent_blocks, selected_dev};
     return with_width(c->D, [&](auto w) -> pg_status {
@@ -2299,7 +2299,7 @@ PG_API pg_status pg_paged_kv4_attention_selected_dev(pg_ctx *ctx, const pg_paged
     const plan p = selected_plan(ctx, c, num_q_heads, tokens, std::min(top_k, max_blocks));  // (no more scratch than was reported without the table)
     PG_CHECK_ARG(p.bytes == 0 || (scratch_dev && scratch_bytes >= p.bytes && ((uintptr_t)scratch_dev & 15) == 0),
                  "%s: scratch of %zu bytes, %zu are needed (16-byte aligned)", fn, scratch_bytes, p.bytes);
-    c->touch(ctx);
+    PG_TRY(c->use(fn, ctx));
     kv4_attn A = {};
     A.q = q_dev, A.q_token = q_token_stride, A.q_head = q_head_stride;
     A.c = kv4_view_of(c);

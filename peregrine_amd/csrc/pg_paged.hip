@@ -558,6 +558,7 @@ PG_API pg_status pg_paged_kv4_create(pg_ctx *ctx, size_t num_blocks, size_t bloc
     if (!c) return pg_fail(PG_ENOMEM, "pg_paged_kv4_create: out of host memory");
     c->num_blocks = num_blocks, c->block_size = block_size, c->heads = num_kv_heads, c->head_dim = head_dim;
     c->D = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    c->device = ctx->device;
     c->shift = log2_of(block_size);
     const size_t records = num_blocks * num_kv_heads, bytes = records * block_size * (c->D + 8), sums = records * (2 * c->D + 16);
     pg_status st = c->mem.alloc(ctx, bytes);
@@ -603,7 +604,7 @@ PG_API pg_status pg_paged_kv4_append_dev(pg_ctx *ctx, pg_paged_kv4 *c, const flo
     if (tokens == 0) return PG_OK;
     PG_CHECK_ARG(k_dev && v_dev && slots_dev, "pg_paged_kv4_append: null pointer");
     PG_CHECK_ARG(tokens < (1ull << 31) && token_stride < (1ull << 40) && head_stride < (1ull << 40), "pg_paged_kv4_append: %zu rows: out of range", tokens);
-    c->touch(ctx);
+    PG_TRY(c->use("pg_paged_kv4_append", ctx));
     const bool wide = c->head_dim % 4 == 0 && token_stride % 4 == 0 && head_stride % 4 == 0 && (((uintptr_t)k_dev | (uintptr_t)v_dev) & 15) == 0;
     return with_width(c->D, [&](auto w) -> pg_status {
         constexpr int D = decltype(w)::value, PER = 2 * 256 / (D / 8);
@@ -623,7 +624,7 @@ PG_API pg_status pg_paged_kv4_read_dev(pg_ctx *ctx, const pg_paged_kv4 *c, const
     if (n == 0) return PG_OK;
     PG_CHECK_ARG(slots_dev && k_dev && v_dev, "pg_paged_kv4_read: null pointer");
     PG_CHECK_ARG(n < (1ull << 31), "pg_paged_kv4_read: %zu rows: out of range", n);
-    c->touch(ctx);
+    PG_TRY(c->use("pg_paged_kv4_read", ctx));
     return with_width(c->D, [&](auto w) -> pg_status {
         constexpr int D = decltype(w)::value, PER = 256 / (D / 8);
         const size_t most = ROWS_A_LAUNCH / (2 * c->heads), width = c->heads * c->head_dim;
@@ -644,7 +645,7 @@ PG_API pg_status pg_paged_kv4_summarise_dev(pg_ctx *ctx, pg_paged_kv4 *c, const 
     if (tokens == 0 || batch == 0) return PG_OK;
     PG_CHECK_ARG(query_start_dev && seq_lens_dev && block_table_dev, "pg_paged_kv4_summarise: null pointer");
     if ((tokens >> c->shift) + 2 * batch >= (1u << 24)) return pg_fail(PG_EUNSUPPORTED, "pg_paged_kv4_summarise: %zu rows are more than a launch takes", tokens);
-    c->touch(ctx);
+    PG_TRY(c->use("pg_paged_kv4_summarise", ctx));
     const kv4_batch ba = {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks};
     return with_width(c->D, [&](auto w) -> pg_status {
         return pg_launch(ctx, "kv4_summarise_kernel", kv4_summarise_kernel<decltype(w)::value>, dim3((unsigned)((tokens >> c->shift) + 2 * batch), (unsigned)((c->heads + 3) / 4)),
@@ -659,7 +660,7 @@ PG_API pg_status pg_paged_kv4_read_summaries_dev(pg_ctx *ctx, const pg_paged_kv4
     if (n == 0) return PG_OK;
     PG_CHECK_ARG(blocks_dev && lo_dev && hi_dev, "pg_paged_kv4_read_summaries: null pointer");
     PG_CHECK_ARG(n < (1ull << 24), "pg_paged_kv4_read_summaries: %zu blocks: out of range", n);
-    c->touch(ctx);
+    PG_TRY(c->use("pg_paged_kv4_read_summaries", ctx));
     return with_width(c->D, [&](auto w) -> pg_status {
         return pg_launch(ctx, "kv4_read_sums_kernel", kv4_read_sums_kernel<decltype(w)::value>, dim3((unsigned)n), dim3(256), 0, blocks_dev, lo_dev, kv4_view_of(c), hi_dev);
     });

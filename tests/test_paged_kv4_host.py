@@ -190,6 +190,27 @@ def test_summaries_refuse_more_blocks_than_a_launch_takes(host):
     host.lib.pg_paged_kv4_free(host.ctx, c)
 
 
+def test_a_cache_stays_on_its_device(host):
+    """One device here: the context's number (its first word) is changed for the calls."""
+    c = new_cache(host, 64, 16, 2, 64)
+    buf = host.alloc(1 << 16)
+    calls = [("pg_paged_kv4_append_dev", (host.ctx, c, buf, buf, 128, 64, 4, buf)), ("pg_paged_kv4_read_dev", (host.ctx, c, buf, 4, buf, buf)),
+             ("pg_paged_kv4_summarise_dev", (host.ctx, c, buf, buf, 4, 4, buf, 64)), ("pg_paged_kv4_read_summaries_dev", (host.ctx, c, buf, 4, buf, buf)),
+             ("pg_paged_kv4_attention_dev", (host.ctx, c, buf, 512, 64, 8, buf, buf, 4, 4, 1, buf, 4, 0.1, 1, 0, 0, 0.0, buf, 0, buf)),
+             ("pg_paged_kv4_select_dev", (host.ctx, c, buf, 512, 64, 8, buf, buf, 4, 4, buf, 64, 8, 1, 1, buf)),
+             ("pg_paged_kv4_attention_selected_dev", (host.ctx, c, buf, 512, 64, 8, buf, buf, 4, 4, buf, 64, buf, 8, 0.1, 0.0, buf, 0, buf))]
+    device = C.c_int.from_address(host.ctx.value)
+    assert device.value == 0
+    for name, args in calls:
+        host.ok(name, *args)
+        device.value = 1
+        try:
+            assert status(host, name, *args) == EINVAL, name
+        finally:
+            device.value = 0
+    host.lib.pg_paged_kv4_free(host.ctx, c)
+
+
 def test_a_step_is_captured_as_launches_alone(host):
     """Nothing of a step's device forms allocates, waits or copies."""
     c = new_cache(host, 4096, 64, 2, 128)
