@@ -499,7 +499,8 @@ pg_status pg_paged_kv4_attention_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, con
 
 /* Attention over part of a long context.  A block's summary holds, for each key head and channel, the least and the most of
  * its keys, as int8 with one scale m * (1 / 127) (m the largest of their magnitudes): lo = rint(least * ((1 / m) * 127)), hi likewise.
- * pg_paged_kv4_summarise brings those of the blocks up to date that a step's rows fill or end in (after its append);
+ * pg_paged_kv4_summarise brings those of the blocks up to date that a step's rows fill or end in (after its append; tokens / block_size
+ * + 2 batch < 2^24, PG_EUNSUPPORTED);
  * pg_paged_kv4_read_summaries_dev gives lo and hi [n, num_kv_heads, head_dim] of n blocks as values (0 for none). */
 pg_status pg_paged_kv4_summarise(pg_ctx *ctx, pg_paged_kv4 *cache, const int32_t *query_start, const int32_t *seq_lens,
                                  size_t batch, const int32_t *block_table, size_t max_blocks);

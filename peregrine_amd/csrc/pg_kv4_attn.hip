@@ -23,7 +23,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float Q_UNITS = 8323072.f;     // 127 * 2^16: the largest of a query row in fixed point
+constexpr float Q_UNITS = 127 * 65536.f;  // the largest of a query row in fixed point
 constexpr float P_TOP = 1024.f;          // what p d is scaled to where p = 1 and d is the largest step seen
 constexpr float P_MOST = 32768.f;        // ... and may grow to before the running maximum follows
 constexpr float CODE = 1.f / 512.f;      // the value operand is (n - 7.5) / 512: its low codes are f16 subnormals on their way

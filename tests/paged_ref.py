@@ -117,7 +117,7 @@ def attend(q, k, v, scale, seen, cap=0.0):
         return np.zeros(k.shape[-1]), np.zeros(k.shape[-1])
     k, v, q = k[seen], v[seen], q.astype(np.float64)
     s = k @ q * scale
-    u = np.abs(q).max() / 8323072
+    u = np.abs(q).max() / (127 * 65536)
     size = np.abs(scale) * (np.abs(k) @ np.abs(q) + 2 * np.abs(k).max(1) * np.abs(q).sum())
     if cap:
         s = cap * np.tanh(s / cap)
