@@ -326,12 +326,18 @@ __global__ __launch_bounds__(256) void kv4_summarise_kernel(kv4_batch ba, kv4_vi
     using R = kv4_rec<D>;
     constexpr int L = D / 8, G = 64 / L;  // lanes a row, rows at a time
     const int item = blockIdx.x, lane = threadIdx.x & (L - 1), group = (threadIdx.x & 63) / L;
-    int upto = 0;
-    for (int i = threadIdx.x & 63; i - (int)(threadIdx.x & 63) < ba.batch; i += 64)
-        upto += __popcll(__ballot(i < ba.batch && (long)(ba.starts[min(i, ba.batch - 1)] >> c.shift) + 2 * i <= item));
-    const int b = upto - 1;
-    if (b < 0) return;
-    const kv4_request rq = kv4_request_at(ba, b, c.shift);
+    int b = -1;
+    kv4_request rq = {0, 0, 0};
+    for (int at = 0; at < ba.batch; at += 64) {  // a lane a request, with what it asks, so that nothing of it is loaded again
+        const int i = at + (threadIdx.x & 63), j = min(i, ba.batch - 1);
+        const int from = ba.starts[j], to = ba.starts[j + 1], len = ba.lens[j];
+        const uint64_t upto = __ballot(i < ba.batch && (long)(from >> c.shift) + 2 * i <= item);
+        if (!upto) break;
+        const int last = 63 - __builtin_clzll(upto);
+        b = at + last;
+        rq = kv4_request_of(ba, __builtin_amdgcn_readlane(from, last), __builtin_amdgcn_readlane(to, last), __builtin_amdgcn_readlane(len, last), c.shift);
+        if (last < 63) break;
+    }
     if (rq.rows == 0) return;
     const int bs = 1 << c.shift, first = max(rq.len - rq.rows, 0), block = (first >> c.shift) + item - ((rq.first >> c.shift) + 2 * b);
     if (block < 0 || (long)block << c.shift >= rq.len) return;
