@@ -798,6 +798,7 @@ public:
     }
     std::vector<float> attention(const std::vector<float> &q, size_t num_q_heads, const std::vector<int32_t> &query_start, const std::vector<int32_t> &seq_lens,
                                  const std::vector<int32_t> &table, float scale, const AttentionMask &mask, float logit_cap) const {
+        if (mask.offset) throw Panic(PG_EINVAL, "PagedKV4Cache::attention: rows stand at the ends of their requests: the mask's offset is 0");
         const size_t tokens = rows(q, num_q_heads, query_start, seq_lens, table, "PagedKV4Cache::attention");
         std::vector<float> out(q.size());
         check(pg_paged_kv4_attention(gpu_->raw(), h_, q.data(), num_q_heads, query_start.data(), seq_lens.data(), seq_lens.size(), tokens, table.data(), width(seq_lens, table),

@@ -87,6 +87,13 @@ static void run(const GpuContext &gpu) {
         refused = e.status == PG_EINVAL;
     }
     EXPECT(refused, "a short slice was taken");
+    refused = false;
+    try {
+        cache.attention(std::vector<float>(heads * hd), heads, {0, 0, 1}, t.seq_lens, t.table, scale, paged::AttentionMask::Causal(3), 0.0f);
+    } catch (const Panic &e) {
+        refused = e.status == PG_EINVAL;
+    }
+    EXPECT(refused, "a mask's offset was taken");
 }
 
 int main() {
