@@ -126,9 +126,10 @@ __global__ __launch_bounds__(1024) void extend_tables_kernel(const int *seq_lens
         for (int j = max(rows, (int)from_row) + tid; j < to_row; j += 1024) slots[j] = -1;
 }
 
-// The slot map over the chip: a thread a row, its request by bisection.
-__global__ __launch_bounds__(256) void slot_map_kernel(const int *__restrict__ starts, const int *__restrict__ lens, int batch, int shift, const int *__restrict__ table,
-                                                       int max_blocks, const int *__restrict__ granted, int *__restrict__ slots, int max_tokens) {
+// The slot map over the chip: a thread a row, its request by bisection.  lens are those after the step; a granted request's rows
+// begin new_lens before them -- not so many rows before them as it has, which max_tokens may have cut.
+__global__ __launch_bounds__(256) void slot_map_kernel(const int *__restrict__ starts, const int *__restrict__ lens, const int *__restrict__ new_lens, int batch, int shift,
+                                                       const int *__restrict__ table, int max_blocks, const int *__restrict__ granted, int *__restrict__ slots, int max_tokens) {
     const int t = blockIdx.x * 256 + threadIdx.x;
     if (t >= max_tokens) return;
     int slot = -1;
@@ -140,8 +141,8 @@ __global__ __launch_bounds__(256) void slot_map_kernel(const int *__restrict__ s
             else hi = mid - 1;
         }
         if (granted[lo]) {
-            const int pos = lens[lo] - (starts[lo + 1] - t);
-            if (pos >= 0) slot = (int)(((unsigned)table[(size_t)lo * max_blocks + (pos >> shift)] << shift) | (pos & ((1 << shift) - 1)));
+            const int pos = lens[lo] - max(new_lens[lo], 0) + (t - starts[lo]);
+            slot = (int)(((unsigned)table[(size_t)lo * max_blocks + (pos >> shift)] << shift) | (pos & ((1 << shift) - 1)));
         }
     }
     slots[t] = slot;
@@ -476,8 +477,8 @@ PG_API pg_status pg_block_tables_extend_dev(pg_ctx *ctx, const int32_t *seq_lens
                      free_list_dev, free_count_dev, (int)num_blocks, block_table_dev, (int)max_blocks, seq_lens_out_dev, free_count_out_dev, query_start_dev, granted_dev,
                      here ? slots_dev : nullptr, (int)max_tokens));
     if (here) return PG_OK;
-    return pg_launch(ctx, "slot_map_kernel", slot_map_kernel, dim3((unsigned)((max_tokens + 255) / 256)), dim3(256), 0, query_start_dev, seq_lens_out_dev, (int)batch, shift,
-                     block_table_dev, (int)max_blocks, granted_dev, slots_dev, (int)max_tokens);
+    return pg_launch(ctx, "slot_map_kernel", slot_map_kernel, dim3((unsigned)((max_tokens + 255) / 256)), dim3(256), 0, query_start_dev, seq_lens_out_dev,
+                     new_lens_dev, (int)batch, shift, block_table_dev, (int)max_blocks, granted_dev, slots_dev, (int)max_tokens);
 }
 
 PG_API pg_status pg_block_tables_release_dev(pg_ctx *ctx, const int32_t *release_dev, int32_t *seq_lens_dev, size_t batch, size_t block_size, int32_t *block_table_dev,

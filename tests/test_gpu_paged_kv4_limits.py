@@ -1,0 +1,46 @@
+"""The paged 4-bit cache and the block tables on the GPU at the ends of what they take: cut slot maps, entries that are no block,
+rows whose sums are far apart."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from devbuf import DevBuf
+from test_gpu_paged_kv4 import F, extend_ref, ints, lib, ok
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------------ tables
+@pytest.mark.parametrize("batch,most_new,in_place", [(30, 900, False), (30, 900, True), (4097, 6, False), (4097, 6, True)])
+def test_a_slot_map_that_is_too_short_keeps_the_first_rows(ctx, batch, most_new, in_place):
+    """Over several workgroups and in a launch of its own, as over one: a request that the cut goes through keeps its first rows' slots."""
+    rng = np.random.default_rng(batch + in_place)
+    bs = 16
+    lens, add = rng.integers(0, 200, batch).astype(np.int32), rng.integers(0, most_new + 1, batch).astype(np.int32)
+    add[::7] -= 9                                                         # some are negative: they count as 0
+    width = -(-(200 + most_new) // bs)
+    have, more = -(-lens // bs), add.clip(0)
+    need = int((-(-(lens + more) // bs) - have).sum())
+    nb = int(have.sum()) + need
+    ids = rng.permutation(nb).astype(np.int32)
+    table = np.full((batch, width), -1, np.int32)
+    for b, at in enumerate(np.cumsum(have) - have):
+        table[b, :have[b]] = ids[at: at + have[b]]
+    free = np.zeros(nb, np.int32)
+    free[:need] = ids[have.sum():]
+    ends = np.cumsum(more)
+    middle = int(np.searchsorted(ends, 0.7 * ends[-1]))
+    middle += int(np.argmax(more[middle:] > 1))                           # a request of two rows and more
+    for tokens in (int(ends[middle]) - 1, int(ends[middle]), int(ends[middle]) - int(more[middle]) + 1):
+        assert 4096 < tokens < ends[-1]
+        want = extend_ref(lens, add, bs, width, table, free, need, tokens)
+        d = [DevBuf(ctx, host=x) for x in (lens, add, free, ints([need]), table, np.zeros(batch + 1, np.int32), np.zeros(batch, np.int32), np.full(tokens + 2, 77, np.int32))]
+        lens_out, count_out = (d[0], d[3]) if in_place else (DevBuf(ctx, host=np.full(batch, 77, np.int32)), DevBuf(ctx, host=ints([77])))
+        ok(lib().pg_block_tables_extend_dev(ctx.handle, d[0].ptr, d[1].ptr, batch, bs, d[2].ptr, d[3].ptr, nb, d[4].ptr, width, lens_out.ptr, count_out.ptr, d[5].ptr, d[6].ptr,
+                                            d[7].ptr, tokens))
+        slots = d[7].to_host(np.int32)
+        got = [d[4].to_host(np.int32).reshape(batch, width), lens_out.to_host(np.int32), count_out.to_host(np.int32)[0], d[5].to_host(np.int32), d[6].to_host(np.int32), slots[:-2]]
+        for g, w in zip(got, want):
+            assert (np.asarray(g) == np.asarray(w)).all()
+        assert (slots[-2:] == 77).all()
