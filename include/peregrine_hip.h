@@ -433,9 +433,9 @@ pg_status pg_huffman_kv_cache_get_kv_dev(pg_ctx *ctx, const pg_huffman_kv_cache 
  * table has room is granted: its next table entries are taken from the free list (the i-th block
  * handed out is free_list[free_count - 1 - i]) and seq_lens_out[b] = seq_lens[b] + new_lens[b].
  * One that needs no block is always granted; one that is not keeps its length and entries and its
- * rows get slot -1.  slots [max_tokens]: a slot per packed row, -1 behind the last (query_start is
- * cut at max_tokens, which the sum of new_lens is not to pass: the rows behind it get no slot, those before it
- * keep theirs).  seq_lens_out may be seq_lens and
+ * rows get slot -1, as do rows of an entry that is no block.  slots [max_tokens]: a slot per packed row,
+ * -1 behind the last (query_start is cut at max_tokens, which the sum of new_lens is not to pass: the rows
+ * behind it get no slot, those before it keep theirs).  seq_lens_out may be seq_lens and
  * free_count_out may be free_count; all else is distinct.  free_list [num_blocks] is only read. */
 pg_status pg_block_tables_extend(pg_ctx *ctx, const int32_t *seq_lens, const int32_t *new_lens, size_t batch, size_t block_size,
                                  const int32_t *free_list, const int32_t *free_count, size_t num_blocks, int32_t *block_table,

@@ -44,6 +44,11 @@ __device__ __forceinline__ int last_upto(const int *at, int n, int v) {
     return lo;
 }
 
+// The slot of position pos in block phys, -1 where that is no block (its number could wrap to another block's slot).
+__device__ __forceinline__ int slot_of(int phys, int pos, int shift, int num_blocks) {
+    return (unsigned)phys < (unsigned)num_blocks ? phys << shift | (pos & ((1 << shift) - 1)) : -1;
+}
+
 // The requests in runs of 1024, a thread a request: rows and needs are prefix sums.  Needs are counted whether they are met or
 // not, so those that are met come first: a granted request's new blocks begin at the sum of the needs before it, and new entries
 // and slots are flat lists, a thread a place, the request by bisection in LDS.  A slot in a new block comes from the free list like
@@ -110,7 +115,7 @@ __global__ __launch_bounds__(1024) void extend_tables_kernel(const int *seq_lens
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int j = from + tid + 1024 * u;
-                if (j < upto) slots[j] = pos[u] < 0 ? -1 : (int)(((unsigned)phys[u] << shift) | (pos[u] & ((1 << shift) - 1)));
+                if (j < upto) slots[j] = pos[u] < 0 ? -1 : slot_of(phys[u], pos[u], shift, num_blocks);
             }
         }
         rows_before += rows_all;
@@ -129,7 +134,8 @@ __global__ __launch_bounds__(1024) void extend_tables_kernel(const int *seq_lens
 // The slot map over the chip: a thread a row, its request by bisection.  lens are those after the step; a granted request's rows
 // begin new_lens before them -- not so many rows before them as it has, which max_tokens may have cut.
 __global__ __launch_bounds__(256) void slot_map_kernel(const int *__restrict__ starts, const int *__restrict__ lens, const int *__restrict__ new_lens, int batch, int shift,
-                                                       const int *__restrict__ table, int max_blocks, const int *__restrict__ granted, int *__restrict__ slots, int max_tokens) {
+                                                       const int *__restrict__ table, int max_blocks, const int *__restrict__ granted, int *__restrict__ slots, int max_tokens,
+                                                       int num_blocks) {
     const int t = blockIdx.x * 256 + threadIdx.x;
     if (t >= max_tokens) return;
     int slot = -1;
@@ -142,7 +148,7 @@ __global__ __launch_bounds__(256) void slot_map_kernel(const int *__restrict__ s
         }
         if (granted[lo]) {
             const int pos = lens[lo] - max(new_lens[lo], 0) + (t - starts[lo]);
-            slot = (int)(((unsigned)table[(size_t)lo * max_blocks + (pos >> shift)] << shift) | (pos & ((1 << shift) - 1)));
+            slot = slot_of(table[(size_t)lo * max_blocks + (pos >> shift)], pos, shift, num_blocks);
         }
     }
     slots[t] = slot;
@@ -478,7 +484,7 @@ PG_API pg_status pg_block_tables_extend_dev(pg_ctx *ctx, const int32_t *seq_lens
                      here ? slots_dev : nullptr, (int)max_tokens));
     if (here) return PG_OK;
     return pg_launch(ctx, "slot_map_kernel", slot_map_kernel, dim3((unsigned)((max_tokens + 255) / 256)), dim3(256), 0, query_start_dev, seq_lens_out_dev,
-                     new_lens_dev, (int)batch, shift, block_table_dev, (int)max_blocks, granted_dev, slots_dev, (int)max_tokens);
+                     new_lens_dev, (int)batch, shift, block_table_dev, (int)max_blocks, granted_dev, slots_dev, (int)max_tokens, (int)num_blocks);
 }
 
 PG_API pg_status pg_block_tables_release_dev(pg_ctx *ctx, const int32_t *release_dev, int32_t *seq_lens_dev, size_t batch, size_t block_size, int32_t *block_table_dev,

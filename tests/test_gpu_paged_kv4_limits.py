@@ -44,3 +44,30 @@ def test_a_slot_map_that_is_too_short_keeps_the_first_rows(ctx, batch, most_new,
         for g, w in zip(got, want):
             assert (np.asarray(g) == np.asarray(w)).all()
         assert (slots[-2:] == 77).all()
+
+
+# ------------------------------------------------------------------------------------------------------ entries that are no block
+def test_slots_of_entries_that_are_no_block_are_none(ctx):
+    """Old entries of a table and entries of the free list that name no block: -1 for their rows, and no slot of another block."""
+    bs, nb, width = 16, 40, 700
+    bad = ints([-1, nb, 1 << 27, 1 << 28, (1 << 28) + 3, 2 ** 31 - 1, -2 ** 31, -2 ** 31 + 5])
+    for batch, tokens in ((8, 300), (8, 6000), (4097, 6000)):
+        lens, add = np.full(batch, 2 * bs - 3, np.int32), np.full(batch, 1, np.int32)
+        add[:8] = 5                                                       # three rows in the old block, two in a new one
+        table = np.full((batch, width), 7, np.int32)
+        table[:8, 1] = bad
+        free, count = np.concatenate([bad, ints([1, 2])])[::-1].copy(), 10
+        with np.errstate(over="ignore"):                                  # (the reference's slots of such entries, replaced below)
+            want = extend_ref(lens, add, bs, width, table, free, count, tokens)
+        slots = want[5].reshape(-1).astype(np.int64)
+        for r in range(8):
+            slots[5 * r: 5 * r + 3] = -1
+            e = int(want[0][r, 2])
+            slots[5 * r + 3: 5 * r + 5] = [16 * e, 16 * e + 1] if 0 <= e < nb else -1
+        for in_place in (False, True):
+            d = [DevBuf(ctx, host=x) for x in (lens, add, free, ints([count]), table, np.zeros(batch + 1, np.int32), np.zeros(batch, np.int32), np.full(tokens, 77, np.int32))]
+            lens_out, count_out = (d[0], d[3]) if in_place else (DevBuf(ctx, host=lens), DevBuf(ctx, host=ints([0])))
+            ok(lib().pg_block_tables_extend_dev(ctx.handle, d[0].ptr, d[1].ptr, batch, bs, d[2].ptr, d[3].ptr, nb, d[4].ptr, width, lens_out.ptr, count_out.ptr, d[5].ptr,
+                                                d[6].ptr, d[7].ptr, tokens))
+            assert (d[4].to_host(np.int32).reshape(batch, width) == want[0]).all()
+            assert (d[7].to_host(np.int32) == slots).all(), (batch, tokens, in_place)
