@@ -447,7 +447,8 @@ pg_status pg_block_tables_extend_dev(pg_ctx *ctx, const int32_t *seq_lens_dev, c
                                      int32_t *free_count_out_dev, int32_t *query_start_dev, int32_t *granted_dev,
                                      int32_t *slots_dev, size_t max_tokens);
 /* The blocks of every request with release[b] != 0 back onto the free list, in order; its length becomes
- * 0 and its entries -1.  A block that two tables share is the caller's to give back once. */
+ * 0 and its entries -1.  A block that two tables share is the caller's to give back once (the host form refuses
+ * more blocks than there are, the _dev form leaves them out). */
 pg_status pg_block_tables_release(pg_ctx *ctx, const int32_t *release, int32_t *seq_lens, size_t batch, size_t block_size,
                                   int32_t *block_table, size_t max_blocks, int32_t *free_list, int32_t *free_count,
                                   size_t num_blocks);

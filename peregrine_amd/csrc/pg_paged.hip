@@ -452,6 +452,15 @@ pg_status check_tables(const char *fn, size_t batch, size_t block_size, size_t n
     return PG_OK;
 }
 
+// A request's tokens as a table on the host holds them: a length within the table, blocks of the pool.
+pg_status check_request(const char *fn, size_t b, int32_t len, const int32_t *table, size_t block_size, size_t max_blocks, size_t num_blocks) {
+    PG_CHECK_ARG(len >= 0 && (size_t)len <= max_blocks * block_size, "%s: request %zu has %d tokens, its table room for %zu", fn, b, len, max_blocks * block_size);
+    const size_t used = ((size_t)len + block_size - 1) / block_size;
+    for (size_t j = 0; j < used; ++j)
+        PG_CHECK_ARG(table[j] >= 0 && (size_t)table[j] < num_blocks, "%s: request %zu's block %zu is %d of %zu", fn, b, j, table[j], num_blocks);
+    return PG_OK;
+}
+
 }  // namespace
 
 pg_status pg_kv4_check_step(const char *fn, const pg_paged_kv4 *c, size_t num_q_heads, size_t batch, size_t tokens, size_t max_blocks) {
@@ -510,6 +519,7 @@ PG_API pg_status pg_block_tables_extend(pg_ctx *ctx, const int32_t *seq_lens, co
     size_t rows = 0;
     for (size_t b = 0; b < batch; ++b) {
         PG_CHECK_ARG(seq_lens[b] >= 0 && new_lens[b] >= 0, "pg_block_tables_extend: request %zu has %d tokens and %d new ones", b, seq_lens[b], new_lens[b]);
+        PG_TRY(check_request("pg_block_tables_extend", b, seq_lens[b], block_table + b * max_blocks, block_size, max_blocks, num_blocks));
         rows += (size_t)new_lens[b];
     }
     PG_CHECK_ARG(rows <= max_tokens, "pg_block_tables_extend: %zu new tokens, a slot map of %zu", rows, max_tokens);
@@ -542,6 +552,13 @@ PG_API pg_status pg_block_tables_release(pg_ctx *ctx, const int32_t *release, in
     if (batch == 0) return PG_OK;
     PG_CHECK_ARG(release && seq_lens && block_table && free_list && free_count, "pg_block_tables_release: null pointer");
     PG_CHECK_ARG(*free_count >= 0 && (size_t)*free_count <= num_blocks, "pg_block_tables_release: %d free blocks of %zu", *free_count, num_blocks);
+    size_t back = (size_t)*free_count;
+    for (size_t b = 0; b < batch; ++b)
+        if (release[b]) {
+            PG_TRY(check_request("pg_block_tables_release", b, seq_lens[b], block_table + b * max_blocks, block_size, max_blocks, num_blocks));
+            back += ((size_t)seq_lens[b] + block_size - 1) / block_size;
+        }
+    PG_CHECK_ARG(back <= num_blocks, "pg_block_tables_release: %zu free blocks of %zu: one is given back twice", back, num_blocks);
     const size_t w = sizeof(int32_t);
     pg_dev_block flags, lens, table, list, count;
     PG_TRY(pg_host_in(ctx, release, batch * w, flags));
