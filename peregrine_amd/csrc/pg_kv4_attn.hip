@@ -2207,6 +2207,7 @@ PG_API pg_status pg_paged_kv4_attention_scratch(pg_ctx *ctx, const pg_paged_kv4 
 PG_API pg_status pg_paged_kv4_selected_scratch(pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t tokens, size_t top_k, size_t *bytes) {
     PG_TRY(pg_use(ctx));
     PG_TRY(pg_kv4_check_step("pg_paged_kv4_selected_scratch", c, num_q_heads, 0, tokens, 1));
+    PG_CHECK_ARG(top_k < (1ull << 31) && top_k * c->block_size < (1ull << 31), "pg_paged_kv4_selected_scratch: %zu blocks: out of range", top_k);
     PG_CHECK_ARG(bytes != nullptr, "pg_paged_kv4_selected_scratch: null output");
     *bytes = selected_plan(ctx, c, num_q_heads, tokens, top_k).bytes;
     return PG_OK;
@@ -2292,7 +2293,7 @@ PG_API pg_status pg_paged_kv4_attention_selected_dev(pg_ctx *ctx, const pg_paged
     PG_TRY(pg_use(ctx));
     PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
     PG_TRY(check_score(fn, scale, logit_cap));
-    PG_CHECK_ARG(top_k > 0 && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
+    PG_CHECK_ARG(top_k > 0 && top_k < (1ull << 31) && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
     if (tokens == 0 || batch == 0) return PG_OK;
     PG_CHECK_ARG(q_dev && query_start_dev && seq_lens_dev && block_table_dev && selected_dev && out_dev, "%s: null pointer", fn);
     PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
@@ -2418,7 +2419,7 @@ PG_API pg_status pg_paged_kv4_attention_selected(pg_ctx *ctx, const pg_paged_kv4
     PG_TRY(pg_use(ctx));
     PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
     PG_TRY(check_score(fn, scale, logit_cap));
-    PG_CHECK_ARG(top_k > 0 && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
+    PG_CHECK_ARG(top_k > 0 && top_k < (1ull << 31) && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
     if (tokens == 0 || batch == 0) return PG_OK;
     PG_CHECK_ARG(q && query_start && seq_lens && block_table && selected && out, "%s: null pointer", fn);
     PG_TRY(check_host_step(fn, c, query_start, seq_lens, batch, tokens, block_table, max_blocks));

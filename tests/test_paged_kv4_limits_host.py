@@ -1,10 +1,12 @@
 """Refusals of the block tables and the paged 4-bit cache at the ends of what they take, without a GPU (the library's own objects on a
 HIP runtime in host memory that notes kernels instead of running them)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 from test_host_runtime import host  # noqa: F401  (the fixture)
-from test_paged_kv4_host import EINVAL, extend_args, i32, p, status
+from test_paged_kv4_host import EINVAL, extend_args, i32, new_cache, p, status, step
 
 
 def table(*rows):
@@ -47,3 +49,33 @@ def test_release_refuses_what_is_no_request_and_more_blocks_than_there_are(host,
     host.lib.pghost_clear_launches()
     assert status(host, "pg_block_tables_release", *args) == EINVAL, wrong
     assert host.lib.pghost_num_launches() == 0
+
+
+WRAPS = [(1 << 60) + 1, (1 << 60) + 8, 1 << 60, 1 << 63, 1 << 27]        # times 16 tokens a block: past 64 bits, or past 31
+
+
+@pytest.mark.parametrize("many", WRAPS)
+def test_tables_and_choices_whose_tokens_wrap_are_refused(host, many):
+    c, buf, n = new_cache(host), host.alloc(1 << 12), C.c_size_t()
+    dense = lambda width: (host.ctx, c, buf, 256, 64, 4, buf, buf, 2, 3, 2, buf, width, 0.125, 1, 0, 0, 0.0, buf, 1 << 14, buf)  # noqa: E731
+    chosen = lambda width, top: (host.ctx, c, buf, 256, 64, 4, buf, buf, 2, 3, buf, width, buf, top, 0.125, 0.0, buf, 1 << 14, buf)  # noqa: E731
+    select = lambda width: (host.ctx, c, buf, 256, 64, 4, buf, buf, 2, 3, buf, width, 2, 1, 1, buf)  # noqa: E731
+    calls = [("pg_paged_kv4_attention_dev", dense, (2,)), ("pg_paged_kv4_attention_selected_dev", chosen, (2, 2)), ("pg_paged_kv4_select_dev", select, (2,)),
+             ("pg_paged_kv4_summarise_dev", lambda width: (host.ctx, c, buf, buf, 2, 3, buf, width), (2,)),
+             ("pg_paged_kv4_attention_scratch", lambda width: (host.ctx, c, 4, 2, 2, width, C.byref(n)), (2,)),
+             ("pg_paged_kv4_selected_scratch", lambda top: (host.ctx, c, 4, 3, top, C.byref(n)), (2,))]
+    for name, args, good in calls:
+        host.ok(name, *args(*good))
+        host.lib.pghost_clear_launches()
+        for at in range(len(good)):
+            assert status(host, name, *args(*good[:at], many, *good[at + 1:])) == EINVAL, name
+        assert host.lib.pghost_num_launches() == 0
+    a, keep = step(host, c, width=many, top=many)
+    for name, args in (("pg_paged_kv4_attention", ("q", "heads", "starts", "lens", "batch", "tokens", "table", "width", "scale", "mask", "window", "sinks", "cap", "out")),
+                       ("pg_paged_kv4_summarise", ("starts", "lens", "batch", "table", "width")),
+                       ("pg_paged_kv4_select", ("q", "heads", "starts", "lens", "batch", "tokens", "table", "width", "top", "first", "recent", "selected"))):
+        assert status(host, name, host.ctx, c, *(a[x] for x in args)) == EINVAL, name
+    a["width"] = 2
+    args = ("q", "heads", "starts", "lens", "batch", "tokens", "table", "width", "selected", "top", "scale", "cap", "out")
+    assert status(host, "pg_paged_kv4_attention_selected", host.ctx, c, *(a[x] for x in args)) == EINVAL
+    host.lib.pg_paged_kv4_free(host.ctx, c)
