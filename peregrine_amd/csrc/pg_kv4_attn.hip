@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         w[i] = sm[i][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][row] - m);
-        l += w[i] == 0.f ? 0.f : w[i] * sl[i][row];
+        l += w[i] * sl[i][row];  // (a weight of 0 drops no NaN; where nothing was seen the sums are 0)
     }
     float *out;
     float by = 1.f;
@@ -540,7 +540,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
         const int d = part + 16 * i;
         float v = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v += w[j] == 0.f ? 0.f : w[j] * so[j][row][d];
+        for (int j = 0; j < 4; ++j) v += w[j] * so[j][row][d];
         if (d < most) out[d] = v * by;
     }
 }
@@ -988,7 +988,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         w[i] = sm[i][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][row] - m);
-        l += w[i] == 0.f ? 0.f : w[i] * sl[i][row];
+        l += w[i] * sl[i][row];  // (a weight of 0 drops no NaN; where nothing was seen the sums are 0)
     }
     float *out;
     float by = 1.f;
@@ -1006,7 +1006,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
         const int d = part + TPR * i;
         float v = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v += w[j] == 0.f ? 0.f : w[j] * fmaf(so[j][row][d] + so[j][HB + row][d], sback[j], sz[j][row]);
+        for (int j = 0; j < 4; ++j) v += w[j] * fmaf(so[j][row][d] + so[j][HB + row][d], sback[j], sz[j][row]);
         if (d < most) out[d] = v * by;
     }
 }
@@ -1703,14 +1703,14 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(kv4_attn A) {
         const int s = s0 + lane, n = min(64, A.splits - s0);
         const float ms = s < A.splits ? part[s * NEXT + RT * D + row] : -INFINITY;
         const float w = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-        float mine = w == 0.f ? 0.f : w * part[s * NEXT + RT * D + 16 + row];
+        float mine = s < A.splits ? w * part[s * NEXT + RT * D + 16 + row] : 0.f;
         mine = over_wave(mine, kv4_add{});
         l += mine;
         const float *rows_at = part + s0 * NEXT + row * D + lane;
         auto add = [&](int j, const float (&x)[D / 64]) {
             const float wj = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) o[i] += wj == 0.f ? 0.f : wj * x[i];  // (a run that saw nothing may hold anything)
+            for (int i = 0; i < D / 64; ++i) o[i] += wj * x[i];  // (a weight of 0 drops no NaN; a run that saw nothing holds zeros)
         };
         int j = 0;
         for (; j + 8 <= n; j += 8) {  // eight splits' rows on their way at once

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from devbuf import DevBuf
-from test_gpu_paged_kv4 import F, extend_ref, ints, lib, ok
+from test_gpu_paged_kv4 import F, Step, World, extend_ref, ints, kernels_of, lib, ok
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,61 @@ def test_slots_of_entries_that_are_no_block_are_none(ctx):
                                                 d[6].ptr, d[7].ptr, tokens))
             assert (d[4].to_host(np.int32).reshape(batch, width) == want[0]).all()
             assert (d[7].to_host(np.int32) == slots).all(), (batch, tokens, in_place)
+
+
+# ------------------------------------------------------------------------------------------------------ rows far apart
+# hd, key heads, group, rows, tokens, kernels: every kernel of attention, its keys in one run and divided.
+FEW, ROWS, P32, P256, JOIN = "kv4_few_kernel", "kv4_rows_kernel", "kv4_prompt32_kernel", "kv4_prompt_kernel", "kv4_join_kernel"
+SHORT = [(64, 1, 4, 1, 600, {FEW}), (128, 2, 3, 1, 600, {FEW}), (256, 1, 4, 1, 450, {FEW}), (64, 1, 8, 1, 600, {FEW}), (100, 1, 4, 2, 600, {FEW}), (256, 1, 6, 1, 450, {FEW}),
+         (64, 1, 16, 1, 600, {ROWS}), (128, 1, 4, 5, 600, {ROWS}), (256, 2, 16, 1, 450, {ROWS})]
+LONG = [(128, 1, 4, 1, 5000, {FEW, JOIN}), (64, 2, 8, 1, 5000, {FEW, JOIN}), (256, 1, 3, 1, 3000, {FEW, JOIN}), (128, 1, 16, 1, 5000, {ROWS, JOIN}), (200, 1, 4, 5, 3000, {ROWS, JOIN})]
+PROMPTS = [(64, 8, 16, 400, 600, {P32}), (100, 8, 16, 400, 600, {P32}), (128, 8, 16, 400, 600, {P32}), (250, 8, 16, 400, 600, {P256})]
+DIVIDED = [(128, 4, 4, 2048, 8100, {P32, JOIN}), (256, 4, 4, 2048, 8100, {P256, JOIN})]
+
+
+def one_request(ctx, hd, heads, group, rows, n, seed=0):
+    w = World(ctx, [n], heads, hd, 16 if n < 1000 else 64, seed=hd + group + seed, poison=False)
+    return w, w.q(rows, heads * group)
+
+
+@pytest.mark.parametrize("hd,heads,group,rows,n,kernels", SHORT + LONG + PROMPTS[2:] + DIVIDED)
+def test_what_is_not_finite_is_not_lost_beside_a_key_of_all_the_weight(ctx, hd, heads, group, rows, n, kernels):
+    """A NaN key or value reaches every row that sees it, also where another key is so far above it that its weight is 0 in f32, in
+    whichever of a row's tiles and runs the two lie."""
+    w, q = one_request(ctx, hd, heads, group, rows, n)
+    q[:] = 8
+    zero, loud = np.zeros((1, heads, hd), F), np.full((1, heads, hd), 4, F)     # scores of 0 and of 32 sqrt(hd): 256 and more
+    keys, values = np.zeros((n, heads, hd), F), w.rng.standard_normal((n, heads, hd)).astype(F)
+    w.put(keys, values, w.slots(0, np.arange(n)))
+    nan = np.full((1, heads, hd), np.nan, F)
+    first = n - rows                                                      # the first row's own token
+    s = Step(ctx, w, q, [0, rows])
+    for at in (5, first):
+        w.put(loud, values[[at]], w.slots(0, [at]))
+        for p in [1, 130, first - 1, n - 1] if rows > 100 else [1, 70, 130, 200, 290, n // 2, n // 2 + 70, first - 1, n - 1]:
+            if p == at:
+                continue
+            for k, v in ((zero, nan), (nan, values[[p]])):
+                w.put(k, v, w.slots(0, [p]))
+                assert kernels_of(ctx, s.attention) == kernels
+                got = s.result()
+                sees = first + np.arange(rows) >= p
+                assert np.isnan(got[sees]).all(), f"loud at {at}, NaN at {p}: {np.isfinite(got[sees]).any(-1).sum()} rows lost it"
+                assert np.isfinite(got[~sees]).all()
+            w.put(zero, values[[p]], w.slots(0, [p]))
+        w.put(zero, values[[at]], w.slots(0, [at]))
+
+
+def test_what_is_not_finite_is_not_lost_in_selected_blocks(ctx):
+    for hd, group, n in ((128, 4, 5000), (64, 16, 5000), (128, 8, 500)):
+        w, q = one_request(ctx, hd, 1, group, 1, n)
+        q[:] = 8
+        keys, values = np.zeros((n, 1, hd), F), w.rng.standard_normal((n, 1, hd)).astype(F)
+        keys[9] = 4
+        w.put(keys, values, w.slots(0, np.arange(n)))
+        sel = np.arange(-(-n // w.bs), dtype=np.int32)[None, None]
+        assert np.isfinite(w.cache.attention_selected(q, [0, 1], w.lens, w.table, sel, hd ** -0.5)).all()
+        for p in (0, 140, n // 2, n - 1):
+            w.put(keys[[p]], np.full((1, 1, hd), np.nan, F), w.slots(0, [p]))
+            assert np.isnan(w.cache.attention_selected(q, [0, 1], w.lens, w.table, sel, hd ** -0.5)).all(), p
+            w.put(keys[[p]], values[[p]], w.slots(0, [p]))
