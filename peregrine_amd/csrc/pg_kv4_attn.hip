@@ -3,7 +3,7 @@
 // With a key row's values z + d (n - 7.5) a score is  d (q . (n - 8)) + (z + d / 2) sum(q):  a product of small whole
 // numbers, which the int8 matrix cores do exactly once q is in fixed point (23 bits under its row's largest, as three digits of
 // 8), and two FMAs.  With a value row's the output is  sum_t (p_t d_t) (n_t - 7.5) + sum_t p_t z_t:  the f16 matrix cores
-// take n - 7.5 as it is and p_t d_t as two f16 (22 bits).  No key or value is dequantised; one pass over the rows keeps
+// take n - 7.5 as it is and p_t d_t as two f16 (22 bits, and 2^-34 of the row's largest).  No key or value is dequantised; one pass over the rows keeps
 // the running maximum and sum of the softmax.
 //
 // The lanes' operands come straight from the rows as they lie in memory.  S^T = K Q^T: a lane holds 16 bytes of one of 16
@@ -24,7 +24,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float Q_UNITS = 127 * 65536.f;  // the largest of a query row in fixed point
-constexpr float P_TOP = 1024.f;          // what p d is scaled to where p = 1 and d is the largest step seen
+constexpr float P_TOP = 1024.f;          // what a row's largest p d so far is scaled to (over half of it, not all)
 constexpr float P_MOST = 32768.f;        // ... and may grow to before the running maximum follows
 constexpr float CODE = 1.f / 512.f;      // the value operand is (n - 7.5) / 512: its low codes are f16 subnormals on their way
 
@@ -204,10 +204,16 @@ __device__ __forceinline__ void settle_all() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// The power of two over a value step, 2^-117 at least, so that P_TOP over it is finite (steps are 2^-120 and more: such a one is
-// still taken as 2^7).
-__device__ __forceinline__ float step_over(float most) {
-    return __builtin_bit_cast(float, max((__builtin_bit_cast(uint32_t, most) & 0x7f800000u) + 0x00800000u, 10u << 23));
+// What a row's p d are scaled by on their way to two f16: P_TOP over the power of two above `peak`, the largest p d that the row has
+// seen.  By weight, not by the largest step: the low half ends at 2^-25, which is 2^-34 of the peak, so a value row of any size costs the
+// others no bits unless it is that much of the output.  A peak under 2^-118 is taken as that, so that the power is finite.
+__device__ __forceinline__ float norm_over(float peak) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, P_TOP) + (127u << 23) - max((__builtin_bit_cast(uint32_t, peak) & 0x7f800000u) + 0x00800000u, 10u << 23));
+}
+// 1 / (norm CODE), and f now / before, of such powers of two: by their exponents, so that nothing in between leaves f32's range.
+__device__ __forceinline__ float back_from(float norm) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, 1.f / CODE) + (127u << 23) - __builtin_bit_cast(uint32_t, norm)); }
+__device__ __forceinline__ float rescaled(float f, float now, float before) {
+    return __builtin_ldexpf(f, (__builtin_bit_cast(int, now) - __builtin_bit_cast(int, before)) >> 23);
 }
 
 // The running softmax of a wavefront's 16 rows: O^T in the accumulators (this lane's row, channels of D / 4 in a run).
@@ -217,8 +223,7 @@ struct softmax_rows {
     f32x4 o[NV];
     float m, l, zsum;  // maximum (log2), sums over this lane's tokens
     bool set;          // whether m is one (the same in a row's four lanes)
-    float step;        // power of two over every value step seen, 0 if none (the same in all lanes)
-    float norm;        // P_TOP / step
+    float peak, norm;  // the largest p d seen when the maximum last moved or p d outgrew its scale, and that scale (the same too)
 };
 
 __device__ __forceinline__ uint32_t meta_at(const uint4 &m, int i) { return i == 0 ? m.x : i == 1 ? m.y : i == 2 ? m.z : m.w; }
@@ -276,31 +281,24 @@ __device__ __forceinline__ void take_tile(bool masked, const kv_tile<D> &t, cons
             dv[i] = seen ? dv[i] : 0.f;
         }
     float p[8], pd[8], sum;
-    uint32_t top;
     auto weigh = [&] {
         sum = 0.f;
-        top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             p[i] = __builtin_amdgcn_exp2f(s[i]);
             sum += p[i];
-            pd[i] = p[i] * (dv[i] * a.norm);
-            top = max(top, __builtin_bit_cast(uint32_t, pd[i]));  // (none is negative: the bits are in order, NaN last)
+            pd[i] = p[i] * dv[i];
         }
     };
     weigh();
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, pd[i] * a.norm));  // (none is negative: the bits are in order, NaN last)
     bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < 1.2676506e30f);  // 2^100; a NaN is off too
     if (!a.set) off = true;
     {
-        uint32_t steps = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) steps = max(steps, __builtin_bit_cast(uint32_t, dv[i]));
-        off |= steps > __builtin_bit_cast(uint32_t, a.step);
         if (__ballot(off)) {
-            float most = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) most = fmaxf(most, dv[i]);
-            // The slow way: the rows' maxima and the largest step follow, what was summed is brought to them.
+            // The slow way: the rows' maxima and scales follow, what was summed is brought to them.
             float at = s[0];
 #pragma unroll
             for (int i = 1; i < 8; ++i) at = fmaxf(at, s[i]);
@@ -312,21 +310,19 @@ __device__ __forceinline__ void take_tile(bool masked, const kv_tile<D> &t, cons
                 a.m += at;
                 a.set = true;
             }
-            most = over_wave(most, kv4_max{});
-            float fo = f;
-            if (most > a.step) {
-                const float step = step_over(most);
-                fo *= a.step / step;
-                a.step = step;
-                a.norm = P_TOP / step;
-            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] -= shift;
+            weigh();
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, pd[i]);  // (a NaN is passed over)
+            a.peak = fmaxf(a.peak * f, max_groups(most));
+            const float norm = norm_over(a.peak), fo = rescaled(f, norm, a.norm);
+            a.norm = norm;
             a.l *= f;
             a.zsum *= f;
 #pragma unroll
             for (int n = 0; n < NV; ++n) a.o[n] *= fo;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] -= shift;
-            weigh();
         }
     }
     a.l += sum;
@@ -336,6 +332,7 @@ __device__ __forceinline__ void take_tile(bool masked, const kv_tile<D> &t, cons
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         zs = fmaf(p[i], zv[i], zs);
+        pd[i] *= a.norm;
         ph[i] = (_Float16)pd[i];
     }
     a.zsum += zs;
@@ -485,7 +482,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
     softmax_rows<D> a;
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) a.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    a.m = 0.f, a.l = 0.f, a.zsum = 0.f, a.set = false, a.step = 0.f, a.norm = 0.f;
+    a.m = 0.f, a.l = 0.f, a.zsum = 0.f, a.set = false, a.peak = 0.f, a.norm = norm_over(0.f);
 
     auto take = [&] {
         const bool whole = max(t.pos[0], t.pos[1]) + 15 <= low_pos && (!windowed || high_pos - min(t.pos[0], t.pos[1]) <= A.window);
@@ -501,7 +498,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
     // Four wavefronts' sums into one.
     a.l = over_groups(a.l);
     a.zsum = over_groups(a.zsum);
-    const float back = a.step * (1.f / (P_TOP * CODE));
+    const float back = back_from(a.norm);
     constexpr int RUN = D / 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -617,8 +614,15 @@ struct softmax_few {
     f32x4 o[D / 16];                  // O^T: this lane's column, channels of D / 4 in a run
     float m[4], l[4], zsum[4];        // of this lane's heads; the sums over this lane's tokens
     bool set[4];
-    float step, norm;
+    float peak[4];                    // their largest p d when last looked for (its scale is made again for each tile: registers count)
 };
+
+// What lanes of a wavefront wrote to LDS is there for its others.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 constexpr int P_ROW = 72;  // f16 from one row of probabilities to the next: 64 and a shift of four banks
 
@@ -694,11 +698,9 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
             dv[p] = any ? dv[p] : 0.f;
         }
     float pd[NT][4], sum[4], zs[4], total;
-    uint32_t top;
     auto weigh_as = [&](auto masked_) {
         constexpr bool MASKED = decltype(masked_)::value;
         total = 0.f;
-        top = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             sum[i] = zs[i] = 0.f;
@@ -708,8 +710,7 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
                 const bool none = MASKED && s[p][i] == -INFINITY;  // (a token that another row sees may be NaN)
                 sum[i] += pr;
                 zs[i] = fmaf(pr, none ? 0.f : zv[p], zs[i]);
-                pd[p][i] = pr * ((none ? 0.f : dv[p]) * a.norm);
-                top = max(top, __builtin_bit_cast(uint32_t, pd[p][i]));  // (none is negative: the bits are in order, NaN last)
+                pd[p][i] = pr * (none ? 0.f : dv[p]);
             }
             total += sum[i];
         }
@@ -719,12 +720,14 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
         else weigh_as(std::false_type{});
     };
     weigh();
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int p = 0; p < NT; ++p) top = max(top, __builtin_bit_cast(uint32_t, pd[p][i] * norm_over(a.peak[i])));  // (none is negative: the bits are in order, NaN last)
     bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(total < 1.2676506e30f);  // 2^100; a NaN is off too
-    const uint32_t steps = max(__builtin_bit_cast(uint32_t, dv[0]), __builtin_bit_cast(uint32_t, dv[NT - 1]));
-    off |= !(a.set[0] && a.set[1] && a.set[2] && a.set[3]) || steps > __builtin_bit_cast(uint32_t, a.step);
+    off |= !(a.set[0] && a.set[1] && a.set[2] && a.set[3]);
     if (__ballot(off)) {
-        float most = fmaxf(0.f, dv[0]);
-        if (NT == 2) most = fmaxf(most, dv[NT - 1]);
         float f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -742,23 +745,20 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
             a.l[i] *= f[i];
             a.zsum[i] *= f[i];
         }
-        most = over_wave(most, kv4_max{});
-        // the column's head: its factor from a lane that has it
-        float fo = 1.f;
+        weigh();
+        float fo = 1.f;  // of the column's head, from a lane that has it
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float fi = HB == 4 ? f[i] : __shfl(f[i], 16 * (c >> 2 & 1));
+            float most = fmaxf(0.f, pd[0][i]);  // (a NaN is passed over)
+            if (NT == 2) most = fmaxf(most, pd[NT - 1][i]);
+            const float before = norm_over(a.peak[i]);
+            a.peak[i] = fmaxf(a.peak[i] * f[i], over_heads<HB>(most, kv4_max{}));
+            const float fs = rescaled(f[i], norm_over(a.peak[i]), before);
+            const float fi = HB == 4 ? fs : __shfl(fs, 16 * (c >> 2 & 1));
             fo = (c & 3) == i ? fi : fo;
-        }
-        if (most > a.step) {
-            const float step = step_over(most);
-            fo *= a.step / step;
-            a.step = step;
-            a.norm = P_TOP / step;
         }
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) a.o[n] *= fo;
-        weigh();
     }
     float minus = -1.f;
     asm("" : "+s"(minus));  // (not a subtraction, so that one instruction takes the f16 as it is)
@@ -770,16 +770,15 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int head = HB == 4 ? i : 4 * (g & 1) + i;
-            const _Float16 hi = (_Float16)pd[p][i];
+            const float x = pd[p][i] * norm_over(a.peak[i]);
+            const _Float16 hi = (_Float16)x;
             pbuf[head * P_ROW + at] = hi;
-            pbuf[(HB + head) * P_ROW + at] = (_Float16)fmaf((float)hi, minus, pd[p][i]);
+            pbuf[(HB + head) * P_ROW + at] = (_Float16)fmaf((float)hi, minus, x);
         }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) a.l[i] += sum[i], a.zsum[i] += zs[i];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_fence();
     const f16x2 low_by = {(_Float16)32768.f, (_Float16)32768.f}, high_by = {(_Float16)2048.f, (_Float16)2048.f};
     const f16x2 centre = {(_Float16)(-7.5f * CODE), (_Float16)(-7.5f * CODE)};
 #pragma unroll
@@ -816,7 +815,12 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
     using R = kv4_rec<D>;
     constexpr int STRIDE = D + 4;
     __shared__ __attribute__((aligned(16))) char lds[4 * 2 * HB * STRIDE * 4 > 4 * 2 * HB * P_ROW * 2 ? 4 * 2 * HB * STRIDE * 4 : 4 * 2 * HB * P_ROW * 2];
-    __shared__ float sm[4][HB], sl[4][HB], sz[4][HB], sback[4];
+    __shared__ float sm[4][HB], sl[4][HB], sz[4][HB], sback[4][HB];
+    // Eight rows of 256 leave no registers for what a tile needs once of each row (factors, position, digits' sums): it waits in LDS, as
+    // spilled registers come back behind the tile's own loads.  64 requests of 4000 tokens, 4 key heads: 59 us (75 spilled), capped
+    // logits 60 (87).
+    constexpr bool LEAN = D == 256 && HB == 8;
+    __shared__ __attribute__((aligned(16))) float of_rows[4][3][LEAN ? 2 : 1][4], of_digits[4][2][LEAN ? 4 : 1][4];
     auto so = reinterpret_cast<float(*)[2 * HB][STRIDE]>(lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
     unsigned id = blockIdx.x;
@@ -933,17 +937,33 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
             row_pos[i] = mine < rows ? pos_of(mine) : -1;
         }
     }
+    if (LEAN && c == 0 && g < HB / 4) {
+        *reinterpret_cast<f32x4 *>(of_rows[wave][0][g]) = f32x4{c1[0], c1[1], c1[2], c1[3]};
+        *reinterpret_cast<f32x4 *>(of_rows[wave][1][g]) = f32x4{sq[0], sq[1], sq[2], sq[3]};
+        *reinterpret_cast<i32x4 *>(of_rows[wave][2][g]) = i32x4{row_pos[0], row_pos[1], row_pos[2], row_pos[3]};
+    }
+    if (LEAN && c == 0)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) *reinterpret_cast<i32x4 *>(of_digits[wave][k][g]) = q.start[k * (q_few<D, HB>::SETS - 1)];
+    wave_fence();
     const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
 
     softmax_few<D> a;
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) a.o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a.m[i] = a.l[i] = a.zsum[i] = 0.f, a.set[i] = false;
-    a.step = a.norm = 0.f;
+    for (int i = 0; i < 4; ++i) a.m[i] = a.l[i] = a.zsum[i] = a.peak[i] = 0.f, a.set[i] = false;
     _Float16 *pbuf = reinterpret_cast<_Float16 *>(lds) + wave * 2 * HB * P_ROW;
 
     auto take = [&] {
+        if constexpr (LEAN) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) q.start[k] = *reinterpret_cast<const i32x4 *>(of_digits[wave][k][g]);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(of_rows[wave][0][g & 1]), y = *reinterpret_cast<const f32x4 *>(of_rows[wave][1][g & 1]);
+            const i32x4 p = *reinterpret_cast<const i32x4 *>(of_rows[wave][2][g & 1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c1[i] = x[i], sq[i] = y[i], row_pos[i] = p[i];
+        }
         const int far = max(max(t.pos[0], t.pos[1]), max(t.pos[2], t.pos[3])), close = min(min(t.pos[0], t.pos[1]), min(t.pos[2], t.pos[3]));
         const bool whole = far + 15 <= low_pos && (!windowed || high_pos - close <= A.window);
         take_tile64<D, HB, CAP>(!whole, t, q, a, row_pos, window, A.sinks, c1, sq, cap_log2e, inv_cap, lane, pbuf);
@@ -978,8 +998,8 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
             sm[wave][h] = a.set[i] ? a.m[i] : a.l[i] == 0.f ? -INFINITY : 0.f;
             sl[wave][h] = a.l[i];
             sz[wave][h] = a.zsum[i];
+            sback[wave][h] = back_from(norm_over(a.peak[i]));
         }
-    if (lane == 0) sback[wave] = a.step * (1.f / (P_TOP * CODE));
     __syncthreads();
     constexpr int TPR = 256 / HB;
     const int row = threadIdx.x / TPR, part = threadIdx.x % TPR;
@@ -1006,7 +1026,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
         const int d = part + TPR * i;
         float v = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v += w[j] * fmaf(so[j][row][d] + so[j][HB + row][d], sback[j], sz[j][row]);
+        for (int j = 0; j < 4; ++j) v += w[j] * fmaf(so[j][row][d] + so[j][HB + row][d], sback[j][row], sz[j][row]);
         if (d < most) out[d] = v * by;
     }
 }
@@ -1154,7 +1174,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
     const int row_pos = live ? pos_of(r) : -1;
     const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;
     f32x4 o[NV];
-    float m = 0.f, l = 0.f, zsum = 0.f, step = 0.f, norm = 0.f;
+    float m = 0.f, l = 0.f, zsum = 0.f, peak = 0.f, norm = norm_over(0.f);
     bool set = false;
 #pragma unroll
     for (int n = 0; n < NV; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1204,36 +1224,21 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
                 }
             }
             float p[8], pd[8], sum;
-            uint32_t top;
             auto weigh = [&] {
-                top = 0;
                 sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     p[i] = __builtin_amdgcn_exp2f(s[i]);
                     sum += p[i];
-                    pd[i] = p[i] * (dv[i] * norm);
-                    top = max(top, __builtin_bit_cast(uint32_t, pd[i]));
+                    pd[i] = p[i] * dv[i];
                 }
             };
             weigh();
-            uint32_t steps = 0;
+            uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) steps = max(steps, __builtin_bit_cast(uint32_t, dv[i]));
-            bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || steps > __builtin_bit_cast(uint32_t, step);
-            off |= !set || !(sum < 1.2676506e30f);
+            for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, pd[i] * norm));
+            const bool off = !set || top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < 1.2676506e30f);
             if (__ballot(off)) {
-                float most = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) most = fmaxf(most, dv[i]);
-                most = over_wave(most, kv4_max{});
-                float fs = 1.f;
-                if (most > step) {
-                    const float next = step_over(most);
-                    fs = step / next;
-                    step = next;
-                    norm = P_TOP / next;
-                }
                 float at = s[0];
 #pragma unroll
                 for (int i = 1; i < 8; ++i) at = fmaxf(at, s[i]);
@@ -1248,10 +1253,15 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
                 }
                 l *= f;
                 zsum *= f;
-                f *= fs;
-#pragma unroll
-                for (int n = 0; n < NV; ++n) o[n] *= f;
                 weigh();
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = fmaxf(most, pd[i]);  // (a NaN is passed over)
+                peak = fmaxf(peak * f, max_groups(most));
+                const float next = norm_over(peak), fo = rescaled(f, next, norm);
+                norm = next;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) o[n] *= fo;
             }
             f16x8 ph, pl;
             float minus = -1.f;
@@ -1261,6 +1271,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 zs = fmaf(p[i], zv[i], zs);
+                pd[i] *= norm;
                 ph[i] = (_Float16)pd[i];
             }
 #pragma unroll
@@ -1296,7 +1307,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
     }
 
     settle_all();
-    const float back = step * (1.f / (P_TOP * CODE));
+    const float back = back_from(norm);
     const float ls = over_groups(l), zs = over_groups(zsum);
     if (r >= rows) return;
     float *out;
@@ -1505,7 +1516,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-    float m = 0.f, l = 0.f, zsum = 0.f, step = 0.f, norm = 0.f;
+    float m = 0.f, l = 0.f, zsum = 0.f, peak = 0.f, norm = norm_over(0.f);
     bool set = false;
 
     auto take = [&](bool masked, int buf) {
@@ -1540,11 +1551,11 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                     s[i] = (far >= 0) & ((window < 0) | (far <= window) | (key < A.sinks)) ? s[i] : -INFINITY;
                 }
             float pd[16], sum, zs;
-            uint32_t top, steps;
+            uint32_t top;
             auto weigh_as = [&](auto masked_) {
                 constexpr bool MASKED = decltype(masked_)::value;
                 sum = zs = 0.f;
-                top = steps = 0;
+                top = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const f32x4 vd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][2][32 * w + 8 * j + 4 * half]), vz = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][3][32 * w + 8 * j + 4 * half]);
@@ -1555,9 +1566,8 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                         const float d = none ? 0.f : vd[i], z = none ? 0.f : vz[i];
                         sum += p;
                         zs = fmaf(p, z, zs);
-                        pd[4 * j + i] = p * (d * norm);
+                        pd[4 * j + i] = p * d * norm;
                         top = max(top, __builtin_bit_cast(uint32_t, pd[4 * j + i]));
-                        steps = max(steps, __builtin_bit_cast(uint32_t, d));
                     }
                 }
             };
@@ -1566,9 +1576,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                 else weigh_as(std::false_type{});
             };
             weigh();
-            if (__ballot(!set || top > __builtin_bit_cast(uint32_t, P_MOST) || steps > __builtin_bit_cast(uint32_t, step) || !(sum < 1.2676506e30f))) {
-                float most = steps < 0x7f800000u ? __builtin_bit_cast(float, steps) : 0.f;  // (a step of NaN reaches what it may and is no scale)
-                most = over_wave(most, kv4_max{});
+            if (__ballot(!set || top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < 1.2676506e30f))) {
                 float at = s[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) at = fmaxf(at, s[i]);
@@ -1583,14 +1591,18 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                 }
                 l *= f;
                 zsum *= f;
-                if (most > step) {
-                    const float next = step_over(most);
-                    f *= step / next;
-                    step = next;
-                    norm = P_TOP / next;
-                }
+                float most = 0.f;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 vd = *reinterpret_cast<const f32x4 *>(&lds.meta[buf][2][32 * w + 8 * j + 4 * half]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = fmaxf(most, __builtin_amdgcn_exp2f(s[4 * j + i]) * vd[i]);  // (a NaN is passed over: masked ones are 0)
+                }
+                peak = fmaxf(peak * f, over_halves(most, kv4_max{}));
+                const float next = norm_over(peak), fo = rescaled(f, next, norm);
+                norm = next;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[dt] *= fo;
                 weigh();
             }
             l += sum;
@@ -1632,7 +1644,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
     l = over_halves(l, kv4_add{});
     zsum = over_halves(zsum, kv4_add{});
     if (!live) return;
-    const float back = step * (1.f / (P_TOP * CODE));
+    const float back = back_from(norm);
     float *out;
     float by = 1.f;
     if (A.splits > 1) {
@@ -1849,13 +1861,6 @@ __device__ __forceinline__ void bin_of(const uint32_t *bins, uint32_t want, int 
     bin = (uint32_t)__builtin_amdgcn_readlane((int)at, who);
     left = (uint32_t)__builtin_amdgcn_readlane((int)rest, who);
 }
-// What lanes of a wavefront wrote to LDS is there for its others.
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // One workgroup: one query token and key head.  Scores of 16 blocks a wavefront at a time -- rows of the product are the
 // group's query rows (x where positive, x where negative), columns the blocks (hi, lo), whole numbers throughout, and two
 // f32 products a score.  Then the key that exactly as many blocks reach as are wanted: passes of 8 bits over a histogram in LDS,

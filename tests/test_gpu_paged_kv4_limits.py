@@ -5,6 +5,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import paged_ref as R
 from devbuf import DevBuf
 from test_gpu_paged_kv4 import F, Step, World, extend_ref, ints, kernels_of, lib, ok
 
@@ -129,3 +130,56 @@ def test_what_is_not_finite_is_not_lost_in_selected_blocks(ctx):
             w.put(keys[[p]], np.full((1, 1, hd), np.nan, F), w.slots(0, [p]))
             assert np.isnan(w.cache.attention_selected(q, [0, 1], w.lens, w.table, sel, hd ** -0.5)).all(), p
             w.put(keys[[p]], values[[p]], w.slots(0, [p]))
+
+
+def run(ctx, w, q, kernels, **m):
+    s = Step(ctx, w, q, [0, len(q)])
+    assert kernels_of(ctx, lambda: s.attention(**m)) == kernels
+    return s.result()
+
+
+def attend_by_weight(q, k, v, scale, seen):
+    """R.attend's value, and a bound in which a value row counts by its weight: p d is two f16, 2^-21 of it and an end of at most
+    2^-25 where the largest p d that the row has seen so far is scaled to 2^9 at least, so 2^-34 of that, times |n - 7.5| <= 7.5: with
+    7.5 d at most 1.02 of the value row's largest, 2^-33 of the largest p |v| for each of N keys.  All else as there."""
+    want, _ = R.attend(q, k, v, scale, seen)
+    k, v, q = k[seen], v[seen], q.astype(np.float64)
+    s = k @ q * scale
+    size = np.abs(scale) * (np.abs(k) @ np.abs(q) + 2 * np.abs(k).max(1) * np.abs(q).sum())
+    m = s.max()
+    err = np.abs(scale) * np.abs(q).max() / (127 * 65536) * np.abs(k).sum(1) + 2.0 ** -24 * (8 * size + 2 * (np.abs(s) + abs(m)) / np.log(2)) + 2.0 ** -22
+    p = np.exp(s - m)
+    p /= p.sum()
+    each = p * np.abs(v).max(1)
+    return want, 2 * ((err + 2.0 ** -21 + (len(p) + 64) * 2.0 ** -24) * each).sum() + 2.0 ** -33 * len(p) * each.max()
+
+
+def check_by_weight(w, got, q, rows, scale, count):
+    at = w.slots(0, np.arange(w.lens[0]))
+    k, v, group, first = w.ref.f64(0, at), w.ref.f64(1, at), q.shape[1] // w.heads, w.lens[0] - rows
+    picks = [(t, j) for t in range(rows) for j in range(q.shape[1])]
+    if len(picks) > count:
+        picks = [picks[i] for i in w.rng.permutation(len(picks))[:count]] + [(0, 0), (rows - 1, q.shape[1] - 1)]
+    off = size = 0.0
+    for t, j in picks:
+        h = j // group
+        want, bound = attend_by_weight(q[t, j], k[:, h], v[:, h], scale, np.arange(w.lens[0]) <= first + t)
+        d = np.abs(got[t, j] - want)
+        assert (d <= bound).all(), f"row {t}, head {j}: off by {d.max():.3g}, bound {bound:.3g}"
+        off, size = off + (d ** 2).sum(), size + (want ** 2).sum()
+    assert (off / size) ** 0.5 < 3e-6, f"2-norm off by {(off / size) ** 0.5:.3g}"
+
+
+@pytest.mark.parametrize("hd,heads,group,rows,n,kernels", SHORT + LONG[:4] + PROMPTS + DIVIDED)
+def test_large_values_of_no_weight_take_no_bits(ctx, hd, heads, group, rows, n, kernels):
+    """Values far larger than the others' on keys whose weight is next to none: alone, in every fourth tile, in all that come first."""
+    w, q = one_request(ctx, hd, heads, group, rows, n, seed=1)
+    q[:] = 1 + 0.1 * w.rng.standard_normal(q.shape)
+    at = np.arange(n)
+    for which, gap, ratio in ((at == 0, 60, 2.0 ** 20), (at < n // 4, 60, 2.0 ** 20), (at % 256 < 64, 90, 2.0 ** 60), (at == 300, 200, 2.0 ** 110)):
+        k = (0.3 * w.rng.standard_normal((n, heads, hd))).astype(F)
+        v = w.rng.standard_normal((n, heads, hd)).astype(F)
+        k[which] -= F(gap / hd ** 0.5)
+        v[which] *= F(ratio)
+        w.put(k, v, w.slots(0, at))
+        check_by_weight(w, run(ctx, w, q, kernels), q, rows, hd ** -0.5, 40)
