@@ -26,6 +26,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float Q_UNITS = 127 * 65536.f;  // the largest of a query row in fixed point
 constexpr float P_TOP = 1024.f;          // what a row's largest p d so far is scaled to (over half of it, not all)
 constexpr float P_MOST = 32768.f;        // ... and may grow to before the running maximum follows
+constexpr float P_SUM = 65536.f;         // what a lane's p of a tile may sum to before it does: sums of p z over 2^20 keys stay finite for values up to 2^90
 constexpr float CODE = 1.f / 512.f;      // the value operand is (n - 7.5) / 512: its low codes are f16 subnormals on their way
 
 struct kv4_attn {
@@ -294,7 +295,7 @@ __device__ __forceinline__ void take_tile(bool masked, const kv_tile<D> &t, cons
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, pd[i] * a.norm));  // (none is negative: the bits are in order, NaN last)
-    bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < 1.2676506e30f);  // 2^100; a NaN is off too
+    bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < P_SUM);  // (a NaN is off too)
     if (!a.set) off = true;
     {
         if (__ballot(off)) {
@@ -725,7 +726,7 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int p = 0; p < NT; ++p) top = max(top, __builtin_bit_cast(uint32_t, pd[p][i] * norm_over(a.peak[i])));  // (none is negative: the bits are in order, NaN last)
-    bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(total < 1.2676506e30f);  // 2^100; a NaN is off too
+    bool off = top > __builtin_bit_cast(uint32_t, P_MOST) || !(total < P_SUM);  // (a NaN is off too)
     off |= !(a.set[0] && a.set[1] && a.set[2] && a.set[3]);
     if (__ballot(off)) {
         float f[4];
@@ -1237,7 +1238,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, pd[i] * norm));
-            const bool off = !set || top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < 1.2676506e30f);
+            const bool off = !set || top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < P_SUM);
             if (__ballot(off)) {
                 float at = s[0];
 #pragma unroll
@@ -1576,7 +1577,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
                 else weigh_as(std::false_type{});
             };
             weigh();
-            if (__ballot(!set || top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < 1.2676506e30f))) {
+            if (__ballot(!set || top > __builtin_bit_cast(uint32_t, P_MOST) || !(sum < P_SUM))) {
                 float at = s[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) at = fmaxf(at, s[i]);

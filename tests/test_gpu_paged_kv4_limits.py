@@ -183,3 +183,17 @@ def test_large_values_of_no_weight_take_no_bits(ctx, hd, heads, group, rows, n, 
         v[which] *= F(ratio)
         w.put(k, v, w.slots(0, at))
         check_by_weight(w, run(ctx, w, q, kernels), q, rows, hd ** -0.5, 40)
+
+
+@pytest.mark.parametrize("hd,heads,group,rows,n,kernels", SHORT + LONG + PROMPTS + DIVIDED[:1])
+def test_large_constant_values_under_rising_scores(ctx, hd, heads, group, rows, n, kernels):
+    """Value rows of one number, whose steps are 0, and scores that rise by 60 behind the first tiles: the sums of p z stay finite."""
+    w, q = one_request(ctx, hd, heads, group, rows, n, seed=2)
+    q[:] = 1
+    k, v = np.zeros((n, heads, hd), F), np.full((n, heads, hd), 2.0 ** 85, F)
+    k[min(300, n - rows):] = F(60 / hd ** 0.5)
+    for sign in (1, -1):
+        w.put(k, sign * v, w.slots(0, np.arange(n)))
+        got = run(ctx, w, q, kernels)
+        # p's error is common to the sums of p z and of p; each is of n + 64 roundings
+        assert np.abs(got / (sign * 2.0 ** 85) - 1).max() <= 2 * (n + 64) * 2.0 ** -24
