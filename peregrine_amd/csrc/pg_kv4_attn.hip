@@ -1342,7 +1342,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
 }
 
 // The same for heads up to 128 on 32 x 32 products: a wavefront has 32 rows, so each operand that it takes from LDS serves twice the
-// rows.  Keys go through the f16 matrix cores too, against q as two f16 (scaled by a power of two to 1 .. 2 at the row's
+// rows.  Keys go through the f16 matrix cores too, against q as two f16 (scaled by a power of two to 512 .. 1024 at the row's
 // largest): two more products a step than with three int8 digits on half the depth, and four instructions a score less, of
 // which there are 16 a lane.  Lanes and operands: A and B of a product hold 8 values of its 16 deep side, row or column lane & 31;
 // a result's registers i are rows (i & 3) + 8 (i >> 2) + 4 (lane >> 5), which makes the probabilities of registers 8 s .. 8 s + 7
@@ -1493,9 +1493,9 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
             }
         top = over_halves(top, kv4_umax{});
         const bool bad = top >= 0x7f800000u, none = bad || top < 0x0d800000u;  // 2^-100: scores of 0
-        // to 1 .. 2 by a power of two (of which the inverse is one too: 2^-100 .. 2^127)
+        // to 512 .. 1024 (1 / CODE, which the keys' operands are short of) by a power of two: 2^109 .. 2^-118 for 2^-100 .. 2^127
         const uint32_t exponent = none ? 127u << 23 : top & 0x7f800000u;
-        const float by = none ? 0.f : __builtin_bit_cast(float, (254u << 23) - exponent), back = __builtin_bit_cast(float, exponent);
+        const float by = none ? 0.f : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, 1.f / CODE) + (127u << 23) - exponent), back = __builtin_bit_cast(float, exponent);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -1507,8 +1507,8 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
             }
         sum = over_halves(sum, kv4_add{});
         const float unit = bad ? __builtin_nanf("") : back * A.scale * (CAP ? 1.f : LOG2E);
-        c1 = unit * (1.f / CODE);
-        sq = sum * unit;
+        c1 = unit;
+        sq = sum * CODE * unit;
     }
     const int row_pos = live ? pos_of(r) : -1;
     const float cap_log2e = CAP ? A.cap * LOG2E : 0.f, inv_cap = CAP ? 1.f / A.cap : 0.f;

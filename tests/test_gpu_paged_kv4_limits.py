@@ -7,7 +7,7 @@ import pytest
 
 import paged_ref as R
 from devbuf import DevBuf
-from test_gpu_paged_kv4 import F, Step, World, extend_ref, ints, kernels_of, lib, ok
+from test_gpu_paged_kv4 import F, Step, World, check_some, extend_ref, ints, kernels_of, lib, ok
 
 pytestmark = pytest.mark.gpu
 
@@ -197,3 +197,14 @@ def test_large_constant_values_under_rising_scores(ctx, hd, heads, group, rows, 
         got = run(ctx, w, q, kernels)
         # p's error is common to the sums of p z and of p; each is of n + 64 roundings
         assert np.abs(got / (sign * 2.0 ** 85) - 1).max() <= 2 * (n + 64) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("hd,heads,group,rows,n,kernels", [SHORT[0], SHORT[1], SHORT[3], SHORT[6], SHORT[7], SHORT[8]] + PROMPTS)
+def test_queries_of_the_largest_numbers(ctx, hd, heads, group, rows, n, kernels):
+    """Rows whose largest is 2^127 and more, over keys near the smallest: ordinary scores, the same on every kernel."""
+    w, q = one_request(ctx, hd, heads, group, rows, n, seed=3)
+    q *= F(1e36)
+    q[..., 3] = F(2e38) * np.where(np.arange(heads * group) % 2, 1, -1)
+    k = (1.5e-37 * w.rng.standard_normal((n, heads, hd))).astype(F)
+    w.put(k, w.rng.standard_normal((n, heads, hd)).astype(F), w.slots(0, np.arange(n)))
+    check_some(w, run(ctx, w, q, kernels), q, [rows], hd ** -0.5, 60)
