@@ -436,7 +436,11 @@ pg_status pg_huffman_kv_cache_get_kv_dev(pg_ctx *ctx, const pg_huffman_kv_cache 
  * rows get slot -1, as do rows of an entry that is no block.  slots [max_tokens]: a slot per packed row,
  * -1 behind the last (query_start is cut at max_tokens, which the sum of new_lens is not to pass: the rows
  * behind it get no slot, those before it keep theirs).  seq_lens_out may be seq_lens and
- * free_count_out may be free_count; all else is distinct.  free_list [num_blocks] is only read. */
+ * free_count_out may be free_count; all else is distinct.  free_list [num_blocks] is only read.
+ * The rows of a request that is not granted stay in query_start: the _dev calls of the step's attention treat them
+ * as the last rows of the tokens that the request has (0 before its first) and touch no other request for them, so
+ * `granted` says whose outputs to drop.  The host forms refuse a request with more rows than tokens: such a step
+ * goes to them with a query_start that leaves those rows out. */
 pg_status pg_block_tables_extend(pg_ctx *ctx, const int32_t *seq_lens, const int32_t *new_lens, size_t batch, size_t block_size,
                                  const int32_t *free_list, const int32_t *free_count, size_t num_blocks, int32_t *block_table,
                                  size_t max_blocks, int32_t *seq_lens_out, int32_t *free_count_out, int32_t *query_start,

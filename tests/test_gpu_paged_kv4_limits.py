@@ -7,7 +7,7 @@ import pytest
 
 import paged_ref as R
 from devbuf import DevBuf
-from test_gpu_paged_kv4 import F, Step, World, check_some, extend_ref, ints, kernels_of, lib, ok
+from test_gpu_paged_kv4 import F, Step, World, bits, check_some, extend_ref, ints, kernels_of, lib, ok
 
 pytestmark = pytest.mark.gpu
 
@@ -208,3 +208,56 @@ def test_queries_of_the_largest_numbers(ctx, hd, heads, group, rows, n, kernels)
     k = (1.5e-37 * w.rng.standard_normal((n, heads, hd))).astype(F)
     w.put(k, w.rng.standard_normal((n, heads, hd)).astype(F), w.slots(0, np.arange(n)))
     check_some(w, run(ctx, w, q, kernels), q, [rows], hd ** -0.5, 60)
+
+
+# ------------------------------------------------------------------------------------------------------ refused requests
+def test_rows_of_a_refused_request_change_nothing_for_the_others(ctx):
+    """What pg_block_tables_extend_dev refuses keeps its rows in the packed step: they are not stored, they get what rows at the end of
+    the request's old tokens get (0 before its first), and the other requests' rows, blocks and summaries are as without them."""
+    heads, group, hd, bs, top = 2, 4, 64, 16, 3
+    w = World(ctx, [40, 70, 3, 90], heads, hd, bs, seed=2, spare=8)
+    w.cache.summarise([0, 40, 110, 113, 203], w.lens, w.table)
+    rows, n = [4, 12, 30, 2], 48                                          # the middle ones need a block, and there is none
+    used = set(w.table[w.table >= 0])
+    free = ints([b for b in range(w.nb) if b not in used] + [0] * len(used))
+    new_table = np.concatenate([w.table, np.full((4, 2), -1, np.int32)], 1)
+    d = [DevBuf(ctx, host=x) for x in (w.lens, ints(rows), free, ints([0]), new_table, np.zeros(4, np.int32), ints([0]), np.zeros(5, np.int32), np.zeros(4, np.int32),
+                                       np.zeros(n, np.int32))]
+    ok(lib().pg_block_tables_extend_dev(ctx.handle, d[0].ptr, d[1].ptr, 4, bs, d[2].ptr, d[3].ptr, w.nb, d[4].ptr, w.width + 2, d[5].ptr, d[6].ptr, d[7].ptr, d[8].ptr, d[9].ptr, n))
+    lens, starts, granted, slots = (d[i].to_host(np.int32) for i in (5, 7, 8, 9))
+    assert list(granted) == [1, 0, 0, 1] and list(lens) == [44, 70, 3, 92] and (slots[4:46] == -1).all() and (slots[:4] >= 0).all()
+    k, v, q = w.keys(n), w.rng.standard_normal((n, heads, hd)).astype(F), w.q(n, heads * group)
+    before = [x[slots_of] for x in w.cache.read(np.arange(w.nb * bs)) for slots_of in [w.slots(1, np.arange(70))]]
+    w.put(k, v, slots)
+    table = d[4].to_host(np.int32).reshape(4, -1)
+
+    def step(starts, lens, table, q):
+        """(outputs, chosen blocks, outputs over them, summaries of every block) of the step's `_dev` calls."""
+        s, sel = Step(ctx, w, q, starts, lens=lens, table=table), DevBuf(ctx, host=np.full((len(q), heads, top), -9, np.int32))
+        at, h, c = (heads * group * hd, hd, heads * group, s.d[0].ptr, s.d[1].ptr, s.batch, len(q)), ctx.handle, w.cache._h
+        ok(lib().pg_paged_kv4_summarise_dev(h, c, s.d[0].ptr, s.d[1].ptr, s.batch, len(q), s.d[2].ptr, s.width))
+        s.attention()
+        out = s.result()
+        ok(lib().pg_paged_kv4_select_dev(h, c, s.d[3].ptr, *at, s.d[2].ptr, s.width, top, 1, 1, sel.ptr))
+        size = C.c_size_t()
+        ok(lib().pg_paged_kv4_selected_scratch(h, c, heads * group, len(q), top, C.byref(size)))
+        scratch, sums = DevBuf(ctx, max(16, size.value)), [DevBuf(ctx, host=np.zeros((w.nb, heads, hd), F)) for _ in range(2)]
+        ok(lib().pg_paged_kv4_attention_selected_dev(h, c, s.d[3].ptr, *at, s.d[2].ptr, s.width, sel.ptr, top, hd ** -0.5, 0.0, scratch.ptr, size.value, s.out.ptr))
+        every = DevBuf(ctx, host=np.arange(w.nb, dtype=np.int32))
+        ok(lib().pg_paged_kv4_read_summaries_dev(h, c, every.ptr, w.nb, sums[0].ptr, sums[1].ptr))
+        return out, sel.to_host(np.int32).reshape(len(q), heads, top), s.result(), [x.to_host(np.uint32) for x in sums]
+
+    keep = np.r_[0:4, 46:48]
+    alone = step([0, 4, 6], lens[[0, 3]], table[[0, 3]], q[keep])
+    whole = step(starts, lens, table, q)
+    for a, b in zip(alone[:3], whole[:3]):
+        assert (np.asarray(a).view(np.uint32) == np.asarray(b)[keep].view(np.uint32)).all()
+    assert all((a == b).all() for a, b in zip(alone[3], whole[3]))
+    for a, b in zip(before, w.cache.read(w.slots(1, np.arange(70)))):
+        assert (bits(a) == bits(b)).all()
+    w.lens, w.table = lens, table
+    old = World.__new__(World)
+    old.__dict__.update(w.__dict__, lens=lens[1:2], table=table[1:2])
+    for out in (whole[0], whole[2]):
+        assert np.isfinite(out).all() and (out[16:43] == 0).all()         # 30 rows over 3 tokens: 27 are before the first
+    old.check(whole[0][4:16], q[4:16], [12], hd ** -0.5)
