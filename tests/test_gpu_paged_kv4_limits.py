@@ -261,3 +261,79 @@ def test_rows_of_a_refused_request_change_nothing_for_the_others(ctx):
     for out in (whole[0], whole[2]):
         assert np.isfinite(out).all() and (out[16:43] == 0).all()         # 30 rows over 3 tokens: 27 are before the first
     old.check(whole[0][4:16], q[4:16], [12], hd ** -0.5)
+
+
+# ------------------------------------------------------------------------------------------------------ prompts' own kernels
+@pytest.mark.parametrize("hd", [40, 63, 64, 100, 125, 128, 200, 250, 256])
+def test_own_kernels_of_prompts_take_strided_queries_and_leave_rows_behind(ctx, hd):
+    """test_prompts_from_strided_queries_and_rows_before_the_first_token with rows enough for the prompts' own kernels."""
+    heads, group, lens, rows = 8, 16, [500, 60], [420, 100]
+    own, n = P256 if hd > 128 else P32, heads * group
+    w = World(ctx, lens, heads, hd, 16, seed=hd)
+    q = w.q(sum(rows) + 3, n)
+    starts, got = [0, 420, 520], []
+    for pad in (0, 1, 4):
+        x = np.full((q.shape[0], n, hd + pad), np.nan, F)
+        x[..., :hd] = q
+        buf, s = DevBuf(ctx, host=x), Step(ctx, w, q, starts)
+        assert kernels_of(ctx, lambda: s.attention(strides=(n * (hd + pad), hd + pad), q=buf.ptr)) == {own}
+        got.append(s.result())
+    assert (bits(got[0]) == bits(got[1])).all() and (bits(got[0]) == bits(got[2])).all()
+    seen = np.r_[0:420, 460:520]
+    assert (got[0][420:460] == 0).all() and (got[0][520:] == 123).all()
+    check_some(w, got[0][seen], q[seen], [420, 60], hd ** -0.5, 100)
+    s = Step(ctx, w, q, starts, max_query=390)
+    assert kernels_of(ctx, s.attention) == {own}
+    cut = s.result()
+    assert (cut[390:420] == 123).all() and (bits(cut[:390]) == bits(got[0][:390])).all() and (bits(cut[420:]) == bits(got[0][420:])).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_own_kernels_of_prompts_near_the_smallest_values(ctx, hd):
+    n, rows, heads, group = 500, 400, 8, 16
+    w, q = one_request(ctx, hd, heads, group, rows, n)
+    for top in (1e-35, 2e-34):
+        v = (w.rng.standard_normal((n, heads, hd)) * np.exp(w.rng.uniform(-3, 0, (n, heads, 1))) * top / 3).astype(F)
+        v[:70], v[100] = 0, 0
+        w.put(w.keys(n), v, w.slots(0, np.arange(n)))
+        check_some(w, run(ctx, w, q, {P256 if hd > 128 else P32}), q, [rows], hd ** -0.5, 60)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_own_kernels_of_prompts_replayed_from_a_graph(ctx, hd):
+    """Captured once; other queries, lengths and tables at each replay, eager work of the same kind between."""
+    from test_gpu_graph_replay import Hip
+    hip, heads, group, rows = Hip(), 8, 16, [300, 120]
+    w = World(ctx, [700, 400], heads, hd, 16, seed=hd, poison=False)
+    q = w.q(sum(rows), heads * group)
+    s, e = (Step(ctx, w, q, [0, 300, 420]) for _ in range(2))
+    own, m = P256 if hd > 128 else P32, dict(mask=2, window=300, sinks=4)
+    assert kernels_of(ctx, lambda: s.attention(**m)) == {own}
+    ctx.sync()
+    graph, ex = hip.capture(ctx.stream, lambda: s.attention(**m))
+    try:
+        for i in range(4):
+            lens, x = ints([700 - 100 * i, 400 - 70 * i]), w.q(sum(rows), heads * group)
+            table = w.table if i % 2 == 0 else np.where(w.table >= 0, w.rng.permutation(w.nb).astype(np.int32)[w.table], -1).astype(np.int32)
+            for y in (s, e):
+                for b, a in ((y.d[1], lens), (y.d[2], table), (y.d[3], x)):
+                    ok(lib().pg_memcpy_h2d(ctx.handle, b.ptr, C.c_void_p(a.ctypes.data), a.nbytes))
+            e.attention(**m)
+            ctx.sync()
+            hip.ok(hip.lib.hipGraphLaunch(ex, ctx.stream), "hipGraphLaunch")
+            ctx.sync()
+            assert (bits(s.result()) == bits(e.result())).all(), f"replay {i}"
+            if i == 0:
+                check_some(w, s.result(), x, rows, hd ** -0.5, 60, **m)
+    finally:
+        hip.lib.hipGraphExecDestroy(ex)
+        hip.lib.hipGraphDestroy(graph)
+
+
+@pytest.mark.parametrize("hd,heads,group,rows,n,kernels", [(128, 2, 4, 1, 5000, {FEW, JOIN}), (64, 2, 2, 3, 5000, {FEW, JOIN}), (256, 1, 7, 1, 5000, {FEW, JOIN}),
+                                                           (128, 2, 4, 9, 5000, {ROWS, JOIN}), (64, 1, 16, 3, 5000, {ROWS, JOIN}), (256, 1, 4, 4, 5000, {ROWS, JOIN})] + DIVIDED)
+def test_windows_with_sinks_over_divided_keys(ctx, hd, heads, group, rows, n, kernels):
+    """Sinks and window cut by the borders of the runs, runs in which some rows or all see nothing."""
+    w, q = one_request(ctx, hd, heads, group, rows, n, seed=4)
+    for m in (dict(window=2000, sinks=4), dict(window=3000, sinks=700), dict(window=2000, sinks=700, cap=5.0), dict(window=3000, sinks=0)):
+        check_some(w, run(ctx, w, q, kernels, mask=2, **m), q, [rows], hd ** -0.5, 24, mask=2, **m)
