@@ -533,7 +533,7 @@ pg_status pg_paged_kv4_select_dev(pg_ctx *ctx, const pg_paged_kv4 *cache, const 
                                   size_t max_blocks, size_t top_k, size_t first_blocks, size_t recent_blocks,
                                   int32_t *selected_dev);
 /* pg_paged_kv4_attention, causal, over the selected blocks alone.  An entry that is not above the one before it, or
- * behind the row's own block, contributes nothing (the host form refuses it). */
+ * behind the row's own block, contributes nothing (the host form refuses it, and any behind a -1). */
 pg_status pg_paged_kv4_selected_scratch(pg_ctx *ctx, const pg_paged_kv4 *cache, size_t num_q_heads, size_t tokens, size_t top_k,
                                         size_t *bytes);
 pg_status pg_paged_kv4_attention_selected(pg_ctx *ctx, const pg_paged_kv4 *cache, const float *q, size_t num_q_heads,

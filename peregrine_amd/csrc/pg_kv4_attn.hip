@@ -2437,7 +2437,7 @@ PG_API pg_status pg_paged_kv4_attention_selected(pg_ctx *ctx, const pg_paged_kv4
             for (size_t h = 0; h < c->heads; ++h) {
                 const int32_t *s = selected + (t * c->heads + h) * top_k;
                 for (size_t i = 0; i < top_k; ++i)
-                    PG_CHECK_ARG(s[i] == -1 || (s[i] >= 0 && s[i] <= pos / (int64_t)c->block_size && (i == 0 || s[i] > s[i - 1])),
+                    PG_CHECK_ARG(s[i] == -1 || (s[i] >= 0 && s[i] <= pos / (int64_t)c->block_size && (i == 0 || (s[i - 1] >= 0 && s[i] > s[i - 1]))),
                                  "%s: row %zu, key head %zu: block %d as number %zu (ascending, up to the row's own %lld, -1 behind them)", fn, t, h, s[i], i,
                                  (long long)(pos / (int64_t)c->block_size));
             }

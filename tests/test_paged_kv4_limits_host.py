@@ -79,3 +79,15 @@ def test_tables_and_choices_whose_tokens_wrap_are_refused(host, many):
     args = ("q", "heads", "starts", "lens", "batch", "tokens", "table", "width", "selected", "top", "scale", "cap", "out")
     assert status(host, "pg_paged_kv4_attention_selected", host.ctx, c, *(a[x] for x in args)) == EINVAL
     host.lib.pg_paged_kv4_free(host.ctx, c)
+
+
+@pytest.mark.parametrize("row", [[-1, 0, 1], [0, -1, 1], [0, -1, 0], [-1, -1, 0], [1, -1, 0]])
+def test_chosen_blocks_behind_a_gap_are_refused(host, row):
+    c = new_cache(host)
+    args = ("q", "heads", "starts", "lens", "batch", "tokens", "table", "width", "selected", "top", "scale", "cap", "out")
+    for sel, want in (([0, 1, -1], None), ([0, -1, -1], None), ([-1, -1, -1], None), (row, EINVAL)):
+        a, keep = step(host, c, selected=np.array([[sel] * 2] * 2 + [[[0, -1, -1]] * 2], np.int32), top=3)
+        host.lib.pghost_clear_launches()
+        st = status(host, "pg_paged_kv4_attention_selected", host.ctx, c, *(a[x] for x in args))
+        assert (st == EINVAL) == (want == EINVAL) and (host.lib.pghost_num_launches() == 0) == (want == EINVAL), sel
+    host.lib.pg_paged_kv4_free(host.ctx, c)
