@@ -387,6 +387,14 @@ __device__ __forceinline__ int by_length(const kv4_batch &ba, int rank) {
     return __builtin_amdgcn_readfirstlane(chosen);
 }
 
+// How many of a list of `top` entries there are to look at: of ascending ones no more than the row has blocks (`own`), but all where
+// others are left out ahead of one that counts.  The whole wavefront asks, each for the same answer.
+__device__ __forceinline__ int entries_upto(const int *picked, int top, int own, int lane) {
+    bool behind = false;
+    for (int i = own + lane; i < top; i += 64) behind |= picked[i] >= 0;
+    return __ballot(behind) ? top : min(top, own);
+}
+
 // One workgroup: 16 query rows of one key head (the rows of a request's tokens and of the head's group, token by token; or
 // with SELECTED the group's rows of one token) over one of `splits` runs of their keys, its four wavefronts every fourth
 // tile of 32 tokens.
@@ -428,7 +436,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
     const int *picked = nullptr;
     if (SELECTED) {
         picked = A.selected + ((size_t)unit * A.c.heads + head) * A.top;
-        const int blocks = high_pos < 0 ? 0 : min(A.top, (high_pos >> shift) + 1);
+        const int blocks = high_pos < 0 ? 0 : entries_upto(picked, A.top, (high_pos >> shift) + 1, lane);
         tiles = (int)((((long)blocks << shift) + 31) >> 5);
     } else {
         const int to = max(high_pos + 1, 0);
@@ -849,7 +857,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
     const int *picked = nullptr;
     if (SELECTED) {
         picked = A.selected + ((size_t)unit * A.c.heads + head) * A.top;
-        const int blocks = high_pos < 0 ? 0 : min(A.top, (high_pos >> shift) + 1);
+        const int blocks = high_pos < 0 ? 0 : entries_upto(picked, A.top, (high_pos >> shift) + 1, lane);
         tiles = (int)((((long)blocks << shift) + 63) >> 6);
     } else {
         const int to = max(high_pos + 1, 0);

@@ -337,3 +337,23 @@ def test_windows_with_sinks_over_divided_keys(ctx, hd, heads, group, rows, n, ke
     w, q = one_request(ctx, hd, heads, group, rows, n, seed=4)
     for m in (dict(window=2000, sinks=4), dict(window=3000, sinks=700), dict(window=2000, sinks=700, cap=5.0), dict(window=3000, sinks=0)):
         check_some(w, run(ctx, w, q, kernels, mask=2, **m), q, [rows], hd ** -0.5, 24, mask=2, **m)
+
+
+# ------------------------------------------------------------------------------------------------------ chosen blocks
+@pytest.mark.parametrize("hd,group", [(64, 4), (128, 8), (64, 16), (256, 3), (256, 16)])
+def test_chosen_entries_count_wherever_they_stand_in_the_list(ctx, hd, group):
+    """Entries that contribute nothing ahead of ones that do, in contexts of fewer blocks than the list has entries."""
+    w = World(ctx, [40, 40, 20, 300, 40], 1, hd, 16, seed=hd + group)
+    lists = [[-1, 0, 1, 2, -1, -1], [7, -1, 0, -1, 1, 2], [-1, -1, -1, -1, 0, 1], [-1, 3, 5, -1, 8, 18], [5, -1, -1, -1, -1, 1]]
+    blocks = [[0, 1, 2], [0, 1, 2], [0, 1], [3, 5, 8, 18], [1]]
+    q, top = w.q(5, group), 70
+    sel = np.full((5, 1, top), -1, np.int32)
+    for t, x in enumerate(lists):
+        sel[t, 0, :len(x) - 1], sel[t, 0, top - 1 - t] = x[:-1], x[-1]       # the last one far behind the others
+    n = C.c_size_t()
+    ok(lib().pg_paged_kv4_selected_scratch(ctx.handle, w.cache._h, group, 5, top, C.byref(n)))
+    d = [DevBuf(ctx, host=x) for x in (np.arange(6, dtype=np.int32), w.lens, w.table, q, sel, np.zeros_like(q))]
+    scratch = DevBuf(ctx, max(16, n.value))
+    ok(lib().pg_paged_kv4_attention_selected_dev(ctx.handle, w.cache._h, d[3].ptr, group * hd, hd, group, d[0].ptr, d[1].ptr, 5, 5, d[2].ptr, w.width, d[4].ptr, top, hd ** -0.5,
+                                                 0.0, scratch.ptr, n.value, d[5].ptr))
+    w.check(d[5].to_host(F).reshape(q.shape), q, [1] * 5, hd ** -0.5, only=lambda t, h: blocks[t])
