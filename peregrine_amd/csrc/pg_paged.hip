@@ -177,7 +177,7 @@ __global__ __launch_bounds__(1024) void release_tables_kernel(const int *release
         __syncthreads();
         long all, mine = tid < run ? valid[tid] : 0, none = 0, no_sum;
         below_sums(mine, none, part, &all, &no_sum);
-        first[tid] = (int)mine;
+        first[tid] = (int)min(mine, (long)num_blocks);  // (tables that share blocks can hold more than 31 bits count)
         __syncthreads();
         for (int i = tid >> 6; i < run; i += 16)
             if (release[at + i]) {

@@ -357,3 +357,18 @@ def test_chosen_entries_count_wherever_they_stand_in_the_list(ctx, hd, group):
     ok(lib().pg_paged_kv4_attention_selected_dev(ctx.handle, w.cache._h, d[3].ptr, group * hd, hd, group, d[0].ptr, d[1].ptr, 5, 5, d[2].ptr, w.width, d[4].ptr, top, hd ** -0.5,
                                                  0.0, scratch.ptr, n.value, d[5].ptr))
     w.check(d[5].to_host(F).reshape(q.shape), q, [1] * 5, hd ** -0.5, only=lambda t, h: blocks[t])
+
+
+@pytest.mark.parametrize("batch", [40, 1030, 2050])
+def test_release_of_more_blocks_than_there_are_fills_the_list_and_no_more(ctx, batch):
+    """The same blocks in many tables: the first that fit go onto the list, in order, and nothing is written behind it."""
+    nb, width = 50, 7
+    table = np.arange(batch * width, dtype=np.int32).reshape(batch, width) % nb
+    table[::3, 2] = -1
+    lens, free = np.full(batch, 16 * width, np.int32), np.full(nb + 4, 77, np.int32)
+    d = [DevBuf(ctx, host=x) for x in (np.ones(batch, np.int32), lens, table, free, ints([5]))]
+    ok(lib().pg_block_tables_release_dev(ctx.handle, d[0].ptr, d[1].ptr, batch, 16, d[2].ptr, width, d[3].ptr, d[4].ptr, nb))
+    got = d[3].to_host(np.int32)
+    given = table.reshape(-1)[table.reshape(-1) >= 0][: nb - 5]
+    assert (got[:5] == 77).all() and (got[5:nb] == given).all() and (got[nb:] == 77).all() and d[4].to_host(np.int32)[0] == nb
+    assert (d[1].to_host(np.int32) == 0).all() and (d[2].to_host(np.int32) == -1).all()
