@@ -2252,7 +2252,7 @@ PG_API pg_status pg_paged_kv4_attention_dev(pg_ctx *ctx, const pg_paged_kv4 *c, 
     A.c = kv4_view_of(c);
     A.ba = {query_start_dev, seq_lens_dev, block_table_dev, (int)batch, (int)tokens, (int)max_blocks};
     A.scale = scale, A.cap = logit_cap, A.mask = mask_kind;
-    A.window = (int)(window > 0x3fffffffu ? 0x3fffffffu : window), A.sinks = (int)(sink_tokens > 0x3fffffffu ? 0x3fffffffu : sink_tokens);
+    A.window = (int)std::min<size_t>(window, 0x7fffffffu), A.sinks = (int)std::min<size_t>(sink_tokens, 0x7fffffffu);
     A.group = (int)(num_q_heads / c->heads), A.q_heads = (int)num_q_heads, A.max_query = (int)max_query;
     A.part = static_cast<float *>(scratch_dev), A.out = out_dev;
     return launch_rows<false>(ctx, fn, c, A, p);

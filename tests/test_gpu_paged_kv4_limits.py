@@ -372,3 +372,24 @@ def test_release_of_more_blocks_than_there_are_fills_the_list_and_no_more(ctx, b
     given = table.reshape(-1)[table.reshape(-1) >= 0][: nb - 5]
     assert (got[:5] == 77).all() and (got[5:nb] == given).all() and (got[nb:] == 77).all() and d[4].to_host(np.int32)[0] == nb
     assert (d[1].to_host(np.int32) == 0).all() and (d[2].to_host(np.int32) == -1).all()
+
+
+def test_windows_of_more_than_two_to_the_thirty_tokens(ctx):
+    """A context of that length, all but a few of its blocks none: a window that reaches its first tokens shows them."""
+    hd, group, bs, far = 64, 4, 256, 1 << 30
+    n = far + 300
+    w = World(ctx, [600], 1, hd, bs, seed=1, poison=False)               # three blocks: the first, the second and the last of the context
+    table = np.full((1, -(-n // bs)), -1, np.int32)
+    table[0, :2], table[0, -1] = w.table[0, :2], w.table[0, 2]
+    q = w.q(1, group)
+    keys = np.concatenate([np.arange(2 * bs), np.arange(n // bs * bs, n)])    # positions that have a block
+    at = R.slots_of(table[0], keys, bs)
+    w.put(w.keys(len(at)), w.rng.standard_normal((len(at), 1, hd)).astype(F), at.astype(np.int32))
+    k, v = w.ref.f64(0, at), w.ref.f64(1, at)
+    for window in (far + 100, far + 299, far - 1, (1 << 31) - 1, 1 << 40):
+        s = Step(ctx, w, q, [0, 1], lens=ints([n]), table=table)
+        s.attention(mask=2, window=window)
+        got = s.result()
+        for j in range(group):
+            want, bound = R.attend(q[0, j], k[:, 0], v[:, 0], hd ** -0.5, n - 1 - keys <= window)
+            assert (np.abs(got[0, j] - want) <= bound).all(), window
