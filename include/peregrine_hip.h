@@ -465,7 +465,8 @@ pg_status pg_block_tables_release_dev(pg_ctx *ctx, const int32_t *release_dev, i
  *   z = bf16(lo / 2 + hi / 2), h = max(hi - z, z - lo) over the row's least and most, d = h * (1 / 7.5) rounded up
  *   to bfloat16 (at least 2^-120, or 0 where h is 0), n = clamp(rint((x - z) * (1 / d) + 7.5), 0, 15), every
  *   operation rounded to f32.
- * A row with a value that is not finite is NaN as a whole.  head_dim <= 256; num_blocks * block_size < 2^31. */
+ * A row with a value that is not finite, or whose z or h is not, is NaN as a whole.  head_dim <= 256; num_blocks *
+ * block_size < 2^31, a step's max_blocks * block_size <= 2^31 - 256. */
 typedef struct pg_paged_kv4 pg_paged_kv4;
 pg_status pg_paged_kv4_create(pg_ctx *ctx, size_t num_blocks, size_t block_size, size_t num_kv_heads, size_t head_dim,
                               pg_paged_kv4 **out);

@@ -13,6 +13,11 @@
 #pragma once
 #include "pg_internal.h"
 
+// The position of what is in no block: beyond every query, and so far under 2^31 that a tile's places behind it are still counted in 32
+// bits.  A table holds no more tokens than that.
+constexpr int KV4_NOWHERE = 0x7fffff00;
+constexpr size_t PG_KV4_MAX_TOKENS = KV4_NOWHERE;
+
 struct pg_paged_kv4 {
     uint8_t *data, *sums;
     size_t num_blocks, block_size, heads, head_dim;

@@ -453,7 +453,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
         int at[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            int phys = -1, pos = 0x7fffff00;
+            int phys = -1, pos = KV4_NOWHERE;
             if (SELECTED) {
                 const int v = 32 * tile + 16 * s, e = v >> shift;
                 if (e < A.top) {
@@ -472,10 +472,10 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && !CAP) ? 3 : 2) void kv
             }
             phys = __builtin_amdgcn_readfirstlane(phys);
             pos = __builtin_amdgcn_readfirstlane(pos);
-            if ((unsigned)phys >= (unsigned)A.c.num_blocks) phys = 0, pos = 0x7fffff00;
+            if ((unsigned)phys >= (unsigned)A.c.num_blocks) phys = 0, pos = KV4_NOWHERE;
             t.pos[s] = pos;
             at[s] = pos & (bs - 1);
-            if (pos == 0x7fffff00) at[s] = 0;
+            if (pos == KV4_NOWHERE) at[s] = 0;
             rec[s] = A.c.data + ((size_t)phys * A.c.heads + head) * R::bytes(shift);
         }
         load_tile<D>(rec, at, shift, lane, t);
@@ -874,7 +874,7 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
         int at[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            int phys = -1, pos = 0x7fffff00;
+            int phys = -1, pos = KV4_NOWHERE;
             if (SELECTED) {
                 const int v = 64 * tile + 16 * u, e = v >> shift;
                 if (e < A.top) {
@@ -893,9 +893,9 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
             }
             phys = __builtin_amdgcn_readfirstlane(phys);
             pos = __builtin_amdgcn_readfirstlane(pos);
-            if ((unsigned)phys >= (unsigned)A.c.num_blocks) phys = 0, pos = 0x7fffff00;
+            if ((unsigned)phys >= (unsigned)A.c.num_blocks) phys = 0, pos = KV4_NOWHERE;
             t.pos[u] = pos;
-            at[u] = pos == 0x7fffff00 ? 0 : pos & (bs - 1);
+            at[u] = pos == KV4_NOWHERE ? 0 : pos & (bs - 1);
             rec[u] = A.c.data + ((size_t)phys * A.c.heads + head) * R::bytes(shift);
         }
 #pragma unroll
@@ -1306,7 +1306,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
             for (int r = 0; r < 4; ++r) {
                 const int p = first + 16 * r;
                 const bool ok = (p <= group_high) & ((unsigned)table[min(p, group_high) >> shift] < (unsigned)A.c.num_blocks);
-                run_pos[r] = ok ? p : 0x7fffff00;
+                run_pos[r] = ok ? p : KV4_NOWHERE;
                 there &= ok;
             }
             take(!there || first + 63 > low_pos || (windowed && high_pos - first > window), run_pos, buf);
@@ -1420,7 +1420,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prompt32_kernel(kv4_attn A) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const bool ok = (unsigned)phys[r] < (unsigned)A.c.num_blocks;
-            next_pos[r] = ok ? first + 16 * r : 0x7fffff00;
+            next_pos[r] = ok ? first + 16 * r : KV4_NOWHERE;
             phys[r] = ok ? phys[r] : 0;
         }
         const int of_lane = lane < 32 ? (lane < 16 ? phys[0] : phys[1]) : (lane < 48 ? phys[2] : phys[3]);
@@ -2221,7 +2221,7 @@ PG_API pg_status pg_paged_kv4_attention_scratch(pg_ctx *ctx, const pg_paged_kv4 
 PG_API pg_status pg_paged_kv4_selected_scratch(pg_ctx *ctx, const pg_paged_kv4 *c, size_t num_q_heads, size_t tokens, size_t top_k, size_t *bytes) {
     PG_TRY(pg_use(ctx));
     PG_TRY(pg_kv4_check_step("pg_paged_kv4_selected_scratch", c, num_q_heads, 0, tokens, 1));
-    PG_CHECK_ARG(top_k < (1ull << 31) && top_k * c->block_size < (1ull << 31), "pg_paged_kv4_selected_scratch: %zu blocks: out of range", top_k);
+    PG_CHECK_ARG(top_k < (1ull << 31) && top_k * c->block_size <= PG_KV4_MAX_TOKENS, "pg_paged_kv4_selected_scratch: %zu blocks: out of range", top_k);
     PG_CHECK_ARG(bytes != nullptr, "pg_paged_kv4_selected_scratch: null output");
     *bytes = selected_plan(ctx, c, num_q_heads, tokens, top_k).bytes;
     return PG_OK;
@@ -2307,7 +2307,7 @@ PG_API pg_status pg_paged_kv4_attention_selected_dev(pg_ctx *ctx, const pg_paged
     PG_TRY(pg_use(ctx));
     PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
     PG_TRY(check_score(fn, scale, logit_cap));
-    PG_CHECK_ARG(top_k > 0 && top_k < (1ull << 31) && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
+    PG_CHECK_ARG(top_k > 0 && top_k < (1ull << 31) && top_k * c->block_size <= PG_KV4_MAX_TOKENS, "%s: %zu blocks: out of range", fn, top_k);
     if (tokens == 0 || batch == 0) return PG_OK;
     PG_CHECK_ARG(q_dev && query_start_dev && seq_lens_dev && block_table_dev && selected_dev && out_dev, "%s: null pointer", fn);
     PG_CHECK_ARG(q_token_stride < (1ull << 40) && q_head_stride < (1ull << 40), "%s: strides out of range", fn);
@@ -2433,7 +2433,7 @@ PG_API pg_status pg_paged_kv4_attention_selected(pg_ctx *ctx, const pg_paged_kv4
     PG_TRY(pg_use(ctx));
     PG_TRY(pg_kv4_check_step(fn, c, num_q_heads, batch, tokens, max_blocks));
     PG_TRY(check_score(fn, scale, logit_cap));
-    PG_CHECK_ARG(top_k > 0 && top_k < (1ull << 31) && top_k * c->block_size < (1ull << 31), "%s: %zu blocks: out of range", fn, top_k);
+    PG_CHECK_ARG(top_k > 0 && top_k < (1ull << 31) && top_k * c->block_size <= PG_KV4_MAX_TOKENS, "%s: %zu blocks: out of range", fn, top_k);
     if (tokens == 0 || batch == 0) return PG_OK;
     PG_CHECK_ARG(q && query_start && seq_lens && block_table && selected && out, "%s: null pointer", fn);
     PG_TRY(check_host_step(fn, c, query_start, seq_lens, batch, tokens, block_table, max_blocks));

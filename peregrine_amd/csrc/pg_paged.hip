@@ -467,8 +467,8 @@ pg_status pg_kv4_check_step(const char *fn, const pg_paged_kv4 *c, size_t num_q_
     PG_CHECK_ARG(c != nullptr, "%s: null cache", fn);
     PG_CHECK_ARG(num_q_heads > 0 && num_q_heads % c->heads == 0 && num_q_heads <= 65535, "%s: %zu query heads over %zu key heads", fn, num_q_heads, c->heads);
     PG_CHECK_ARG(batch <= 65535, "%s: %zu requests (65535 at most)", fn, batch);
-    PG_CHECK_ARG(tokens < (1ull << 31) && max_blocks > 0 && max_blocks < (1ull << 31) && max_blocks * c->block_size < (1ull << 31), "%s: %zu rows, tables of %zu blocks: out of range", fn, tokens,
-                 max_blocks);
+    PG_CHECK_ARG(tokens < (1ull << 31) && max_blocks > 0 && max_blocks < (1ull << 31) && max_blocks * c->block_size <= PG_KV4_MAX_TOKENS,
+                 "%s: %zu rows, tables of %zu blocks: out of range", fn, tokens, max_blocks);
     return PG_OK;
 }
 

@@ -81,6 +81,21 @@ def test_tables_and_choices_whose_tokens_wrap_are_refused(host, many):
     host.lib.pg_paged_kv4_free(host.ctx, c)
 
 
+def test_tables_end_short_of_the_position_that_stands_for_none(host):
+    """2^31 - 256 tokens: positions there and a tile behind them are still numbers of 32 bits."""
+    most = (2 ** 31 - 256) // 16
+    c, buf, n = new_cache(host), host.alloc(1 << 12), C.c_size_t()
+    dense = lambda width: (host.ctx, c, buf, 256, 64, 4, buf, buf, 2, 3, 2, buf, width, 0.125, 1, 0, 0, 0.0, buf, 1 << 40, buf)  # noqa: E731
+    chosen = lambda top: (host.ctx, c, buf, 256, 64, 4, buf, buf, 2, 3, buf, 8, buf, top, 0.125, 0.0, buf, 1 << 40, buf)  # noqa: E731
+    for name, args in (("pg_paged_kv4_attention_dev", dense), ("pg_paged_kv4_attention_selected_dev", chosen),
+                       ("pg_paged_kv4_attention_scratch", lambda width: (host.ctx, c, 4, 2, 2, width, C.byref(n))),
+                       ("pg_paged_kv4_selected_scratch", lambda top: (host.ctx, c, 4, 3, top, C.byref(n)))):
+        host.ok(name, *args(most))
+        for more in (most + 1, (1 << 27) - 1):
+            assert status(host, name, *args(more)) == EINVAL, name
+    host.lib.pg_paged_kv4_free(host.ctx, c)
+
+
 @pytest.mark.parametrize("row", [[-1, 0, 1], [0, -1, 1], [0, -1, 0], [-1, -1, 0], [1, -1, 0]])
 def test_chosen_blocks_behind_a_gap_are_refused(host, row):
     c = new_cache(host)
