@@ -11,8 +11,20 @@ from .llama import AttentionMask
 from .quant import _ptr
 
 
+def _ints(a, what):
+    """`a` as 32-bit integers; numbers that are none are refused, not wrapped."""
+    a = np.asarray(a)
+    if a.dtype == np.int32:
+        return np.ascontiguousarray(a)
+    with np.errstate(invalid="ignore"):
+        b = np.ascontiguousarray(a, np.int32)
+    if not (b == a).all():
+        raise ValueError(f"{what}: not 32-bit integers")
+    return b
+
+
 def _i32(a, n, what):
-    a = np.ascontiguousarray(a, np.int32).reshape(-1)
+    a = _ints(a, what).reshape(-1)
     if a.size != n:
         raise ValueError(f"{what}: {a.size} values, not {n}")
     return a
@@ -65,8 +77,8 @@ class PagedKV4Cache:
         return a
 
     def _step(self, query_start, seq_lens, block_table):
-        lens = np.ascontiguousarray(seq_lens, np.int32).reshape(-1)
-        table = np.ascontiguousarray(block_table, np.int32)
+        lens = _ints(seq_lens, "seq_lens").reshape(-1)
+        table = _ints(block_table, "block_table")
         if table.ndim != 2 or table.shape[0] != lens.size:
             raise ValueError("block_table is not [batch, max_blocks]")
         return _i32(query_start, lens.size + 1, "query_start"), lens, table
@@ -87,7 +99,7 @@ class PagedKV4Cache:
 
     def read(self, slots):
         """(k, v) of the slots, [n, num_kv_heads, head_dim] each, as the values that the codes stand for."""
-        slots = np.ascontiguousarray(slots, np.int32).reshape(-1)
+        slots = _ints(slots, "PagedKV4Cache.read: slots").reshape(-1)
         k, v = (np.zeros((slots.size, self.num_kv_heads, self.head_dim), np.float32) for _ in range(2))
         _ffi.check(_ffi.lib.pg_paged_kv4_read(self.ctx.handle, self._h, _ptr(slots), slots.size, _ptr(k.reshape(-1)), _ptr(v.reshape(-1))))
         return k, v
@@ -124,7 +136,7 @@ class PagedKV4Cache:
         """Causal attention over the selected blocks alone."""
         q = self._rows(q, "q")
         starts, lens, table = self._step(query_start, seq_lens, block_table)
-        sel = np.ascontiguousarray(selected, np.int32)
+        sel = _ints(selected, "PagedKV4Cache.attention_selected: selected")
         if sel.ndim != 3 or sel.shape[:2] != (q.shape[0], self.num_kv_heads):
             raise ValueError("PagedKV4Cache.attention_selected: selected is not [tokens, num_kv_heads, top_k]")
         out = np.zeros_like(q)

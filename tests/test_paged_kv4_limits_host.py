@@ -106,3 +106,21 @@ def test_chosen_blocks_behind_a_gap_are_refused(host, row):
         st = status(host, "pg_paged_kv4_attention_selected", host.ctx, c, *(a[x] for x in args))
         assert (st == EINVAL) == (want == EINVAL) and (host.lib.pghost_num_launches() == 0) == (want == EINVAL), sel
     host.lib.pg_paged_kv4_free(host.ctx, c)
+
+
+def test_mirror_refuses_numbers_that_32_bits_do_not_hold():
+    """They would have become others: slot 2^32 + 3 slot 3.  No context is made."""
+    from peregrine_amd import paged
+
+    c = paged.PagedKV4Cache.__new__(paged.PagedKV4Cache)
+    c.num_kv_heads, c.head_dim, c._h = 2, 64, None
+    t = paged.BlockTables.__new__(paged.BlockTables)
+    t.batch = 2
+    k, q, ok_table = np.zeros((3, 2, 64)), np.zeros((3, 4, 64)), np.zeros((1, 2), np.int64)
+    for bad in (2 ** 32 + 3, 2 ** 31, -2 ** 31 - 1, 0.5, float("nan")):
+        for call in (lambda: c.append(k, k, [0, 1, bad]), lambda: c.read([bad]), lambda: t.extend([1, bad]), lambda: c.attention(q, [0, bad], [5], ok_table, 0.1),
+                     lambda: c.attention(q, [0, 3], [bad], ok_table, 0.1), lambda: c.summarise([0, 3], [5], np.array([[0, bad]])),
+                     lambda: c.attention_selected(q, [0, 3], [5], ok_table, np.full((3, 2, 1), bad), 0.1)):
+            with pytest.raises(ValueError, match="32-bit"):
+                call()
+    assert (paged._ints([1.0, -1.0], "x") == [1, -1]).all() and paged._ints(np.zeros((2, 0)), "x").dtype == np.int32
