@@ -3,8 +3,8 @@
 // With a key row's values z + d (n - 7.5) a score is  d (q . (n - 8)) + (z + d / 2) sum(q):  a product of small whole
 // numbers, which the int8 matrix cores do exactly once q is in fixed point (23 bits under its row's largest, as three digits of
 // 8), and two FMAs.  With a value row's the output is  sum_t (p_t d_t) (n_t - 7.5) + sum_t p_t z_t:  the f16 matrix cores
-// take n - 7.5 as it is and p_t d_t as two f16 (22 bits, and 2^-34 of the row's largest).  No key or value is dequantised; one pass over the rows keeps
-// the running maximum and sum of the softmax.
+// take n - 7.5 as it is and p_t d_t as two f16 (22 bits, ending 2^-34 under the row's largest).  No key or value is
+// dequantised; one pass over the rows keeps the running maximum and sum of the softmax.
 //
 // The lanes' operands come straight from the rows as they lie in memory.  S^T = K Q^T: a lane holds 16 bytes of one of 16
 // tokens' keys, (x & 0x0f0f0f0f) and (x >> 4 & 0x0f0f0f0f) are 8 int8 channels in an order that the digits of q share.
@@ -817,8 +817,8 @@ __device__ __forceinline__ void take_tile64(bool masked, const kv_tile64<D> &t, 
 }
 
 // As kv4_rows_kernel, for up to HB rows of a unit: one row tile, wavefronts every fourth tile of 64 tokens.  Bound by memory where
-// contexts are long: 128 requests of 7500 tokens, 8 key heads of 128, a group of 4 202 to 208 us (5.0 to 5.2 TB/s; loads alone 5.5, a
-// copy 4.8), of 8 211.  Three workgroups a CU where the registers reach (with 8 rows they do not: 26 spilled, 347 us).
+// contexts are long: 128 requests of 7500 tokens, 8 key heads of 128, a group of 4 198 to 200 us (5.2 TB/s; loads alone 5.5, a
+// copy 4.8), of 8 201 to 205.  Three workgroups a CU where the registers reach (with 8 rows they do not: 26 spilled, 347 us).
 template <int D, int HB, bool CAP, bool SELECTED>
 __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void kv4_few_kernel(kv4_attn A) {
     using R = kv4_rec<D>;
@@ -1045,8 +1045,8 @@ __global__ __launch_bounds__(256, D == 64 || (D == 128 && HB == 4) ? 3 : 2) void
 // Here a workgroup has eight wavefronts of 16 rows and makes the operands of 64 tokens once, in LDS, in the order in
 // which the lanes take them (four wavefronts the keys', four the values'); the next 64 tokens' codes are on their way meanwhile, and the
 // two buffers take turns, one barrier a tile.  Scores and probabilities as in kv4_rows_kernel.  What bounds it is the arithmetic on
-// scores: about 17 instructions for each of 16 x 64 beside 56 products of the matrix cores.  Heads of 256: 2048 rows at 8192, 16 heads,
-// 487 us (477 TFLOP/s of one product each).
+// scores: about 17 instructions for each of 16 x 64 beside 112 products of the matrix cores.  Heads of 256: the last 2048 rows of 8192, 16
+// heads, 470 us (512 TFLOP/s of one product each).
 template <int D>
 struct prompt_lds {
     static constexpr int K = 64 * D, V = 128 * D;  // bytes of a tile's operands
@@ -1355,7 +1355,7 @@ __global__ __launch_bounds__(512, 2) void kv4_prompt_kernel(kv4_attn A) {
 // which there are 16 a lane.  Lanes and operands: A and B of a product hold 8 values of its 16 deep side, row or column lane & 31;
 // a result's registers i are rows (i & 3) + 8 (i >> 2) + 4 (lane >> 5), which makes the probabilities of registers 8 s .. 8 s + 7
 // the B operand of step s once the values' tokens stand in that order.  2048 rows at 16384, 32 heads of 128: 1095 us (471 TFLOP/s of one
-// product each, twice that executed); vector instructions 51 %, matrix products 39 % of the cycles, which do not overlap much better.
+// product each, twice that executed); vector instructions 51 %, matrix products 40 % of the cycles, which do not overlap much better.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int D>
