@@ -206,8 +206,8 @@ __device__ __forceinline__ void settle_all() {
 }
 
 // What a row's p d are scaled by on their way to two f16: P_TOP over the power of two above `peak`, the largest p d that the row has
-// seen.  By weight, not by the largest step: the low half ends at 2^-25, which is 2^-34 of the peak, so a value row of any size costs the
-// others no bits unless it is that much of the output.  A peak under 2^-118 is taken as that, so that the power is finite.
+// seen.  By weight, not by the largest step: the low half ends at 2^-25, which is 2^-34 of the peak, so a large value row takes bits from
+// the others only as far as it outweighs them in the output too.  A peak under 2^-118 is taken as that, so that the power is finite.
 __device__ __forceinline__ float norm_over(float peak) {
     return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, P_TOP) + (127u << 23) - max((__builtin_bit_cast(uint32_t, peak) & 0x7f800000u) + 0x00800000u, 10u << 23));
 }
