@@ -1,6 +1,6 @@
 """No instruction of the paged attention reads a matrix product's result before it is there: the hardware does not hold a vector
 instruction back, the compiler counts the wait, and where a branch lies between the two it has been seen to count one way only.
-Checked over the assembly that this build's own source compiles to, along every way from a product.  CPU only."""
+Checked over the assembly that the library's own source compiles to, along every way from a product.  CPU only."""
 import os
 import re
 import shutil
